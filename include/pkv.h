@@ -360,6 +360,63 @@ int pkv_rope_q(const uint16_t *x, int64_t x_tok_stride, int64_t x_head_stride, u
                const double *freqs_t, int t_rows, int t_cols, const double *freqs_y, int y_rows,
                int y_cols, const double *freqs_x, int x_rows, int x_cols, pkv_stream_t stream);
 
+/* ---- the token path around the cache: layer norm, rotary positions ---------
+ * Element types of the tensors below.  Everything is computed in fp32 and
+ * rounded once to the tensor's type.  No counterparts in the reference, whose
+ * model leaves these to torch. */
+#define PKV_BF16 0
+#define PKV_FP16 1
+#define PKV_FP32 2
+
+/*
+ * Layer norm of `rows` rows of `cols` channels:
+ *   y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps),
+ * w = weight, or 1 + weight when one_plus (a DiT block's modulation).
+ * weight / bias: [groups, cols] (either may be NULL), row r uses row
+ * r / (rows / groups); groups divides rows.  dtype: x and y; wtype: weight and
+ * bias (dtype or PKV_FP32).  Rows are x_row_stride / y_row_stride elements
+ * apart, channels contiguous.  cols <= 2^20.  mean / rstd: fp32 [rows], saved for the backward pass
+ * (nullable).
+ */
+int pkv_layer_norm(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
+                   int dtype, int wtype, int64_t rows, int64_t cols, int64_t groups, float eps,
+                   int one_plus, void *y, int64_t y_row_stride, float *mean, float *rstd,
+                   pkv_stream_t stream);
+
+/*
+ * Gradients of pkv_layer_norm: dx [rows, cols] (dtype), dweight / dbias
+ * [groups, cols] (wtype); each may be NULL when it is not wanted.  mean /
+ * rstd: those pkv_layer_norm saved.  The column sums go through `workspace`
+ * (pkv_layer_norm_workspace_bytes, overwritten; needed when dweight or dbias
+ * is) in a fixed order: the same inputs give the same bits.  dx may be dy.
+ */
+int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups);
+int pkv_layer_norm_backward(const void *dy, int64_t dy_row_stride, const void *x,
+                            int64_t x_row_stride, const void *weight, const float *mean,
+                            const float *rstd, int dtype, int wtype, int64_t rows, int64_t cols,
+                            int64_t groups, int one_plus, void *dx, int64_t dx_row_stride,
+                            void *dweight, void *dbias, void *workspace, int64_t workspace_bytes,
+                            pkv_stream_t stream);
+
+/*
+ * Rotary positions of a query and a key tensor in one launch (either may have
+ * 0 heads): pair p < pairs of every head of token t turns by
+ * positions[t * axes + axis[p]] * inv_freq[p], its result times `scale`;
+ * pairs are elements (2p, 2p + 1), or (p, p + pairs) when `half`; elements
+ * from 2 * pairs on are copied.  inverse != 0 turns the other way (the
+ * gradient's pass).  Token t, head h starts at base + t * tok_stride + h *
+ * head_stride (elements).  positions: int64 [tokens, axes] (1-4 axes);
+ * inv_freq: float64 [pairs] radians a position; axis: int32 [pairs] (may be NULL for one axis;
+ * entries outside 0 .. axes - 1 are clamped).  pairs <= 2048.  x and out may be the same memory.
+ */
+int pkv_rotary(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int q_heads,
+               void *q_out, int64_t qo_tok_stride, int64_t qo_head_stride, const void *k,
+               int64_t k_tok_stride, int64_t k_head_stride, int k_heads, void *k_out,
+               int64_t ko_tok_stride, int64_t ko_head_stride, int dtype, int64_t tokens,
+               int head_dim, const int64_t *positions, int axes, const double *inv_freq,
+               const int32_t *axis, int pairs, int half, float scale, int inverse,
+               pkv_stream_t stream);
+
 /*
  * Head-parallel exchange layout copy (around the NCCL all-to-all of a layer
  * step split over ranks by heads): for each source i < count (<= 4), token

@@ -27,8 +27,10 @@ CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA, "bin", "nvcc")
 
 CU_SOURCES = ["pkv_update.cu", "pkv_merge.cu", "pkv_plan.cu", "pkv_pack.cu", "pkv_attn.cu",
-              "pkv_attend.cu", "pkv_legacy.cu", "pkv_rope.cu", "pkv_exchange.cu"]
-HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh"]
+              "pkv_attend.cu", "pkv_legacy.cu", "pkv_rope.cu", "pkv_exchange.cu", "pkv_norm.cu",
+              "pkv_rotary.cu"]
+BIND_SOURCES = ["adahead_bind.cpp", "token_bind.cpp"]
+HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh", "pkv_vec.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
            "--ptxas-options=-v"] + ARCH
@@ -81,18 +83,25 @@ def build(jobs: int = 8, force: bool = False, verbose: bool = False) -> str:
         _run([NVCC] + ARCH + ["-shared", "-o", libpkv] + objs)
 
     incs, tlib, abi = torch_paths()
-    bind_src = os.path.join(CSRC, "adahead_bind.cpp")
-    bind_obj = os.path.join(BUILD, "adahead_bind.o")
-    if force or _stale(bind_obj, [bind_src, os.path.join(INC, "pkv.h")]):
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-               "-I", INC, "-I", os.path.join(CUDA, "include"),
-               "-I", sysconfig.get_paths()["include"]]
-        for i in incs:
-            cmd += ["-I", i]
-        _run(cmd + ["-c", bind_src, "-o", bind_obj])
+
+    def compile_bind(src: str) -> str:
+        obj = os.path.join(BUILD, src.replace(".cpp", ".o"))
+        path = os.path.join(CSRC, src)
+        if force or _stale(obj, [path, os.path.join(INC, "pkv.h")]):
+            cmd = ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                   "-I", INC, "-I", os.path.join(CUDA, "include"),
+                   "-I", sysconfig.get_paths()["include"]]
+            for i in incs:
+                cmd += ["-I", i]
+            _run(cmd + ["-c", path, "-o", obj])
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        binds = list(ex.map(compile_bind, BIND_SOURCES))
     glue = os.path.join(LIB, "_adahead.so")
-    if force or _stale(glue, [bind_obj, libpkv]):
-        _run(["g++", "-shared", "-o", glue, bind_obj, "-L", LIB, "-lpkv", "-L", tlib,
+    if force or _stale(glue, binds + [libpkv]):
+        _run(["g++", "-shared", "-o", glue] + binds +
+             ["-L", LIB, "-lpkv", "-L", tlib,
               "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
               "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib])
     return glue

@@ -1,0 +1,552 @@
+// Layer norm, forward and backward, with the modulation a DiT block applies.
+//
+// Forward, per row of C channels:
+//   mu = sum(x) / C,  rstd = 1 / sqrt(sum((x - mu)^2) / C + eps)
+//   y  = (x - mu) * rstd * w + b,    w = weight (+ 1 when one_plus)
+// Backward, with xh = (x - mu) * rstd and g = dy * w:
+//   dx = rstd * (g - sum(g) / C - xh * sum(g * xh) / C)
+//   dw = sum over rows of dy * xh,  db = sum over rows of dy
+// weight and bias are [G, C]: row r uses row r / (rows / G), so one launch
+// normalises and modulates every frame or video of a batch.
+//
+// Both passes are bound by HBM: forward reads x and writes y, backward reads
+// x and dy and writes dx.  A row stays in registers between the statistics
+// and the result (mean first, then the centred squares: no cancellation), so
+// each tensor crosses HBM once.  All sums are fp32.
+//
+// dw / db: a CTA owns a contiguous range of a group's rows and every column
+// (thread = fixed columns), keeps its column sums in registers over its rows
+// and writes them to a [parts, 2, C] workspace once; a second kernel adds the
+// parts in order.  No atomics: the result does not depend on timing.
+#include "pkv_vec.cuh"
+
+namespace pkv {
+namespace {
+
+constexpr int kNormThreads = 256;
+constexpr int64_t kMaxCols = int64_t(1) << 20;
+
+struct NormArgs {
+  const void* x;
+  const void* w;
+  const void* b;
+  void* y;
+  float* mean;
+  float* rstd;
+  int64_t x_rs, y_rs, rows, rows_per_group;
+  int C;
+  float eps, plus;
+};
+
+// Sum over the threads of a block (whole warps), the same in every thread.
+// `red` holds 32 floats and is free again after the next barrier.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_sum(v);
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) return v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+  for (int i = 0; i < nw; ++i) s += red[i];
+  return s;
+}
+
+// One row per warp (kWarpRow) or per block; V elements a vector, NV vectors
+// a thread in registers.
+template <typename TX, typename TW, int V, int NV, bool kWarpRow>
+__global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(NormArgs a) {
+  __shared__ float red[2][32];
+  const int tpr = kWarpRow ? 32 : blockDim.x;
+  const int tid = kWarpRow ? (threadIdx.x & 31) : threadIdx.x;
+  const int64_t row = kWarpRow ? blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5)
+                               : int64_t(blockIdx.x);
+  if (row >= a.rows) return;  // whole warps (kWarpRow) or whole blocks
+  const int nvec = a.C / V;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
+  float f[NV][V];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = tid + i * tpr;
+    if (j < nvec) {
+      const Vec<TX, V> t = ld_vec<TX, V>(x + j * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[i][e] = to_f32(t.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
+    }
+  }
+  const float inv_c = 1.0f / float(a.C);
+  const float mu = (kWarpRow ? warp_sum(s) : block_sum(s, red[0])) * inv_c;
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (tid + i * tpr < nvec)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[i][e] -= mu;
+        q = fmaf(f[i][e], f[i][e], q);
+      }
+  const float rstd = rsqrtf((kWarpRow ? warp_sum(q) : block_sum(q, red[1])) * inv_c + a.eps);
+  if (tid == 0) {
+    if (a.mean) a.mean[row] = mu;
+    if (a.rstd) a.rstd[row] = rstd;
+  }
+  const int64_t g = row / a.rows_per_group;
+  const TW* w = a.w ? static_cast<const TW*>(a.w) + g * a.C : nullptr;
+  const TW* b = a.b ? static_cast<const TW*>(a.b) + g * a.C : nullptr;
+  TX* y = static_cast<TX*>(a.y) + row * a.y_rs;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = tid + i * tpr;
+    if (j < nvec) {
+      float r[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) r[e] = f[i][e] * rstd;
+      float t2[V];
+      if (w) {
+        ld_f32<TW, V>(w + j * V, t2);
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] *= t2[e] + a.plus;
+      }
+      if (b) {
+        ld_f32<TW, V>(b + j * V, t2);
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] += t2[e];
+      }
+      Vec<TX, V> t;
+#pragma unroll
+      for (int e = 0; e < V; ++e) t.v[e] = from_f32<TX>(r[e]);
+      st_vec<TX, V>(y + j * V, t);
+    }
+  }
+}
+
+// Rows too long for registers: the row is read three times, from L2 after the
+// first.
+template <typename TX, typename TW>
+__global__ void __launch_bounds__(1024) norm_fwd_long_kernel(NormArgs a) {
+  __shared__ float red[2][32];
+  const int64_t row = blockIdx.x;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
+  float s = 0.0f;
+  for (int j = threadIdx.x; j < a.C; j += blockDim.x) s += to_f32(x[j]);
+  const float mu = block_sum(s, red[0]) / float(a.C);
+  float q = 0.0f;
+  for (int j = threadIdx.x; j < a.C; j += blockDim.x) {
+    const float d = to_f32(x[j]) - mu;
+    q = fmaf(d, d, q);
+  }
+  const float rstd = rsqrtf(block_sum(q, red[1]) / float(a.C) + a.eps);
+  if (threadIdx.x == 0) {
+    if (a.mean) a.mean[row] = mu;
+    if (a.rstd) a.rstd[row] = rstd;
+  }
+  const int64_t g = row / a.rows_per_group;
+  const TW* w = a.w ? static_cast<const TW*>(a.w) + g * a.C : nullptr;
+  const TW* b = a.b ? static_cast<const TW*>(a.b) + g * a.C : nullptr;
+  TX* y = static_cast<TX*>(a.y) + row * a.y_rs;
+  for (int j = threadIdx.x; j < a.C; j += blockDim.x) {
+    float r = (to_f32(x[j]) - mu) * rstd;
+    if (w) r *= to_f32(w[j]) + a.plus;
+    if (b) r += to_f32(b[j]);
+    y[j] = from_f32<TX>(r);
+  }
+}
+
+struct NormBwdArgs {
+  const void* dy;
+  const void* x;
+  const void* w;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  float* part;  // [groups * parts][2][C] column sums, or nullptr
+  int64_t dy_rs, x_rs, dx_rs, rows_per_group;
+  int C, parts;
+  float plus;
+};
+
+constexpr int kBwdRows = 2;  // rows of one reduction round
+
+// CTA (group, part): its rows, every column.
+template <typename TX, typename TW, int V, int NV>
+__global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(NormBwdArgs a) {
+  __shared__ float red[2][2 * kBwdRows][8];
+  const int tid = threadIdx.x, nthr = blockDim.x, nw = nthr >> 5;
+  const int64_t grp = blockIdx.x / a.parts;
+  const int p = int(blockIdx.x - grp * a.parts);
+  const int64_t r0 = grp * a.rows_per_group + a.rows_per_group * p / a.parts;
+  const int64_t r1 = grp * a.rows_per_group + a.rows_per_group * (p + 1) / a.parts;
+  const int nvec = a.C / V;
+  const float inv_c = 1.0f / float(a.C);
+  const TW* wp = a.w ? static_cast<const TW*>(a.w) + grp * a.C : nullptr;
+  float w[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = tid + i * nthr;
+    const bool have = wp && j < nvec;
+    if (have) ld_f32<TW, V>(wp + j * V, w[i]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      w[i][e] = have ? w[i][e] + a.plus : 1.0f;
+      aw[i][e] = ab[i][e] = 0.0f;
+    }
+  }
+  int round = 0;
+  for (int64_t r = r0; r < r1; r += kBwdRows, ++round) {
+    Vec<TX, V> vx[kBwdRows][NV], vd[kBwdRows][NV];
+    float mu[kBwdRows], rs[kBwdRows], c1[kBwdRows], c2[kBwdRows];
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      const bool live = r + k < r1;
+      const TX* x = static_cast<const TX*>(a.x) + (r + k) * a.x_rs;
+      const TX* d = static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs;
+      mu[k] = live ? a.mean[r + k] : 0.0f;
+      rs[k] = live ? a.rstd[r + k] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = tid + i * nthr;
+        if (live && j < nvec) {
+          vx[k][i] = ld_vec<TX, V>(x + j * V);
+          vd[k][i] = ld_vec<TX, V>(d + j * V);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            vx[k][i].v[e] = from_f32<TX>(0.0f);
+            vd[k][i].v[e] = from_f32<TX>(0.0f);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      c1[k] = c2[k] = 0.0f;
+      const bool live = r + k < r1;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (live && tid + i * nthr < nvec)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float d = to_f32(vd[k][i].v[e]);
+            const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
+            const float g = d * w[i][e];
+            c1[k] += g;
+            c2[k] = fmaf(g, xh, c2[k]);
+            aw[i][e] = fmaf(d, xh, aw[i][e]);
+            ab[i][e] += d;
+          }
+      c1[k] = warp_sum(c1[k]);
+      c2[k] = warp_sum(c2[k]);
+    }
+    // two buffers in turn: a warp may write the next round's while another
+    // still reads this one's
+    float(*buf)[8] = red[round & 1];
+    if ((tid & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < kBwdRows; ++k) {
+        buf[2 * k][tid >> 5] = c1[k];
+        buf[2 * k + 1][tid >> 5] = c2[k];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      c1[k] = c2[k] = 0.0f;
+      for (int i = 0; i < nw; ++i) {
+        c1[k] += buf[2 * k][i];
+        c2[k] += buf[2 * k + 1][i];
+      }
+      c1[k] *= inv_c;
+      c2[k] *= inv_c;
+    }
+    if (a.dx != nullptr) {
+#pragma unroll
+      for (int k = 0; k < kBwdRows; ++k) {
+        if (r + k >= r1) break;
+        TX* dx = static_cast<TX*>(a.dx) + (r + k) * a.dx_rs;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int j = tid + i * nthr;
+          if (j < nvec) {
+            Vec<TX, V> t;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
+              const float g = to_f32(vd[k][i].v[e]) * w[i][e];
+              t.v[e] = from_f32<TX>(rs[k] * (g - c1[k] - xh * c2[k]));
+            }
+            st_vec<TX, V>(dx + j * V, t);
+          }
+        }
+      }
+    }
+  }
+  if (a.part != nullptr) {
+    float* pw = a.part + int64_t(blockIdx.x) * 2 * a.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = tid + i * nthr;
+      if (j < nvec)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          pw[j * V + e] = aw[i][e];
+          pw[a.C + j * V + e] = ab[i][e];
+        }
+    }
+  }
+}
+
+// Rows too long for registers: dx by one CTA a row ...
+template <typename TX, typename TW>
+__global__ void __launch_bounds__(1024) norm_bwd_long_kernel(NormBwdArgs a) {
+  __shared__ float red[2][32];
+  const int64_t row = blockIdx.x;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
+  const TX* d = static_cast<const TX*>(a.dy) + row * a.dy_rs;
+  TX* dx = static_cast<TX*>(a.dx) + row * a.dx_rs;
+  const TW* w = a.w ? static_cast<const TW*>(a.w) + row / a.rows_per_group * a.C : nullptr;
+  const float mu = a.mean[row], rs = a.rstd[row];
+  float c1 = 0.0f, c2 = 0.0f;
+  for (int j = threadIdx.x; j < a.C; j += blockDim.x) {
+    const float g = to_f32(d[j]) * (w ? to_f32(w[j]) + a.plus : 1.0f);
+    c1 += g;
+    c2 = fmaf(g, (to_f32(x[j]) - mu) * rs, c2);
+  }
+  c1 = block_sum(c1, red[0]) / float(a.C);
+  c2 = block_sum(c2, red[1]) / float(a.C);
+  for (int j = threadIdx.x; j < a.C; j += blockDim.x) {
+    const float g = to_f32(d[j]) * (w ? to_f32(w[j]) + a.plus : 1.0f);
+    dx[j] = from_f32<TX>(rs * (g - c1 - (to_f32(x[j]) - mu) * rs * c2));
+  }
+}
+
+// ... and the column sums by one thread a column of a (group, part).
+template <typename TX>
+__global__ void __launch_bounds__(kNormThreads) norm_cols_kernel(NormBwdArgs a) {
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  if (c >= a.C) return;
+  const int64_t grp = blockIdx.x / a.parts;
+  const int p = int(blockIdx.x - grp * a.parts);
+  const int64_t r0 = grp * a.rows_per_group + a.rows_per_group * p / a.parts;
+  const int64_t r1 = grp * a.rows_per_group + a.rows_per_group * (p + 1) / a.parts;
+  float sw = 0.0f, sb = 0.0f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const float d = to_f32(static_cast<const TX*>(a.dy)[r * a.dy_rs + c]);
+    const float xh = (to_f32(static_cast<const TX*>(a.x)[r * a.x_rs + c]) - a.mean[r]) * a.rstd[r];
+    sw = fmaf(d, xh, sw);
+    sb += d;
+  }
+  a.part[int64_t(blockIdx.x) * 2 * a.C + c] = sw;
+  a.part[int64_t(blockIdx.x) * 2 * a.C + a.C + c] = sb;
+}
+
+// Column sums of a group's parts, in order, rounded to the weight's type.
+// 32 columns x 8 slices of the parts a block; the slices meet in shared memory.
+template <typename TW>
+__global__ void __launch_bounds__(256)
+    norm_parts_kernel(const float* part, int parts, int C, TW* dw, TW* db) {
+  __shared__ float sm[8][2][32];
+  const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5;
+  const int c = blockIdx.y * 32 + lane;
+  const int64_t grp = blockIdx.x;
+  float sw = 0.0f, sb = 0.0f;
+  if (c < C)
+    for (int p = sl; p < parts; p += 8) {
+      const float* q = part + (grp * parts + p) * 2 * int64_t(C);
+      sw += q[c];
+      sb += q[C + c];
+    }
+  sm[sl][0][lane] = sw;
+  sm[sl][1][lane] = sb;
+  __syncthreads();
+  if (sl != 0 || c >= C) return;
+  sw = sb = 0.0f;
+  for (int i = 0; i < 8; ++i) {
+    sw += sm[i][0][lane];
+    sb += sm[i][1][lane];
+  }
+  if (dw) dw[grp * C + c] = from_f32<TW>(sw);
+  if (db) db[grp * C + c] = from_f32<TW>(sb);
+}
+
+// Parts of a group in the backward pass: about two CTAs an SM over all
+// groups, at least kBwdRows rows each.
+int64_t bwd_parts(int64_t rows_per_group, int64_t groups) {
+  const int64_t want = (int64_t(sm_count()) * 2 + groups - 1) / groups;
+  const int64_t most = (rows_per_group + kBwdRows - 1) / kBwdRows;
+  const int64_t p = want < most ? want : most;
+  return p < 1 ? 1 : p;
+}
+
+constexpr int round_warp(int n) { return (n + 31) / 32 * 32; }
+
+template <typename TX, typename TW, int V>
+int launch_fwd(const NormArgs& a, cudaStream_t s) {
+  const int nvec = a.C / V;
+  // a warp a row while its lanes hold the row (V * 6 elements each) and the
+  // rows fill the GPU; else a block a row
+  if (nvec <= 32 * 6 && a.rows >= int64_t(sm_count()) * 4) {
+    const int per = kNormThreads / 32;
+    const int64_t grid = (a.rows + per - 1) / per;
+    if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+    if (nvec <= 32)
+      norm_fwd_kernel<TX, TW, V, 1, true><<<int(grid), kNormThreads, 0, s>>>(a);
+    else if (nvec <= 64)
+      norm_fwd_kernel<TX, TW, V, 2, true><<<int(grid), kNormThreads, 0, s>>>(a);
+    else if (nvec <= 128)
+      norm_fwd_kernel<TX, TW, V, 4, true><<<int(grid), kNormThreads, 0, s>>>(a);
+    else
+      norm_fwd_kernel<TX, TW, V, 6, true><<<int(grid), kNormThreads, 0, s>>>(a);
+    return launch_status();
+  }
+  if (a.rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  const int grid = int(a.rows);
+  const int thr = nvec < kNormThreads ? round_warp(nvec) : kNormThreads;
+  if (nvec <= kNormThreads)
+    norm_fwd_kernel<TX, TW, V, 1, false><<<grid, thr, 0, s>>>(a);
+  else if (nvec <= 2 * kNormThreads)
+    norm_fwd_kernel<TX, TW, V, 2, false><<<grid, thr, 0, s>>>(a);
+  else if (nvec <= 4 * kNormThreads)
+    norm_fwd_kernel<TX, TW, V, 4, false><<<grid, thr, 0, s>>>(a);
+  else if (nvec <= 8 * kNormThreads)
+    norm_fwd_kernel<TX, TW, V, 8, false><<<grid, thr, 0, s>>>(a);
+  else
+    norm_fwd_long_kernel<TX, TW><<<grid, 1024, 0, s>>>(a);
+  return launch_status();
+}
+
+template <typename TX, typename TW, int V>
+int launch_bwd(const NormBwdArgs& a, int64_t groups, cudaStream_t s) {
+  const int nvec = a.C / V;
+  const int64_t grid = groups * a.parts;
+  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  const int thr = nvec < kNormThreads ? round_warp(nvec) : kNormThreads;
+  if (nvec <= kNormThreads)
+    norm_bwd_kernel<TX, TW, V, 1><<<int(grid), thr, 0, s>>>(a);
+  else if (nvec <= 2 * kNormThreads)
+    norm_bwd_kernel<TX, TW, V, 2><<<int(grid), thr, 0, s>>>(a);
+  else if (nvec <= 4 * kNormThreads)
+    norm_bwd_kernel<TX, TW, V, 4><<<int(grid), thr, 0, s>>>(a);
+  else {
+    const int64_t rows = groups * a.rows_per_group;
+    if (rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+    if (a.dx) norm_bwd_long_kernel<TX, TW><<<int(rows), 1024, 0, s>>>(a);
+    const dim3 cols(unsigned(grid), unsigned((a.C + kNormThreads - 1) / kNormThreads));
+    if (a.part) norm_cols_kernel<TX><<<cols, kNormThreads, 0, s>>>(a);
+  }
+  return launch_status();
+}
+
+template <typename TX, typename TW>
+int run_fwd(const NormArgs& a, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(TX);
+  if (a.C % V == 0 && vec_ok(a.x, a.x_rs, V, sizeof(TX)) &&
+      vec_ok(a.y, a.y_rs, V, sizeof(TX)) && vec_ok(a.w, 0, 16, 1) && vec_ok(a.b, 0, 16, 1))
+    return launch_fwd<TX, TW, V>(a, s);
+  return launch_fwd<TX, TW, 1>(a, s);
+}
+
+template <typename TX, typename TW>
+int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(TX);
+  int rc;
+  if (a.C % V == 0 && vec_ok(a.x, a.x_rs, V, sizeof(TX)) &&
+      vec_ok(a.dy, a.dy_rs, V, sizeof(TX)) && vec_ok(a.dx, a.dx_rs, V, sizeof(TX)) &&
+      vec_ok(a.w, 0, 16, 1))
+    rc = launch_bwd<TX, TW, V>(a, groups, s);
+  else
+    rc = launch_bwd<TX, TW, 1>(a, groups, s);
+  if (rc != PKV_OK || a.part == nullptr) return rc;
+  const dim3 grid(unsigned(groups), unsigned((a.C + 31) / 32));
+  norm_parts_kernel<TW><<<grid, 256, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
+                                             static_cast<TW*>(db));
+  return launch_status();
+}
+
+bool norm_types(int dtype, int wtype) {
+  return dtype >= PKV_BF16 && dtype <= PKV_FP32 && (wtype == dtype || wtype == PKV_FP32);
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups) {
+  if (rows <= 0 || cols <= 0 || groups <= 0 || rows % groups != 0) return 0;
+  return groups * bwd_parts(rows / groups, groups) * 2 * cols * 4;
+}
+
+extern "C" int pkv_layer_norm(const void* x, int64_t x_row_stride, const void* weight,
+                              const void* bias, int dtype, int wtype, int64_t rows, int64_t cols,
+                              int64_t groups, float eps, int one_plus, void* y,
+                              int64_t y_row_stride, float* mean, float* rstd,
+                              pkv_stream_t stream) {
+  if (rows < 0 || cols <= 0 || groups <= 0 || !norm_types(dtype, wtype)) return PKV_EINVAL;
+  if (rows == 0) return PKV_OK;
+  if (!x || !y || rows % groups != 0 || !(eps >= 0.0f)) return PKV_EINVAL;
+  if (cols > kMaxCols) return PKV_EUNSUPPORTED;
+  NormArgs a{};
+  a.x = x;
+  a.w = weight;
+  a.b = bias;
+  a.y = y;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.x_rs = x_row_stride;
+  a.y_rs = y_row_stride;
+  a.rows = rows;
+  a.rows_per_group = rows / groups;
+  a.C = int(cols);
+  a.eps = eps;
+  a.plus = one_plus ? 1.0f : 0.0f;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (dtype == PKV_BF16)
+    return wtype == PKV_FP32 ? run_fwd<__nv_bfloat16, float>(a, s)
+                             : run_fwd<__nv_bfloat16, __nv_bfloat16>(a, s);
+  if (dtype == PKV_FP16)
+    return wtype == PKV_FP32 ? run_fwd<__half, float>(a, s) : run_fwd<__half, __half>(a, s);
+  return run_fwd<float, float>(a, s);
+}
+
+extern "C" int pkv_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* x,
+                                       int64_t x_row_stride, const void* weight,
+                                       const float* mean, const float* rstd, int dtype, int wtype,
+                                       int64_t rows, int64_t cols, int64_t groups, int one_plus,
+                                       void* dx, int64_t dx_row_stride, void* dweight,
+                                       void* dbias, void* workspace, int64_t workspace_bytes,
+                                       pkv_stream_t stream) {
+  if (rows <= 0 || cols <= 0 || groups <= 0 || !norm_types(dtype, wtype)) return PKV_EINVAL;
+  if (!dy || !x || !mean || !rstd || rows % groups != 0) return PKV_EINVAL;
+  if (cols > kMaxCols) return PKV_EUNSUPPORTED;
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  if (!sums && !dx) return PKV_OK;
+  if (sums && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
+               workspace_bytes < pkv_layer_norm_workspace_bytes(rows, cols, groups)))
+    return PKV_EINVAL;
+  NormBwdArgs a{};
+  a.dy = dy;
+  a.x = x;
+  a.w = weight;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.dx = dx;
+  a.part = sums ? static_cast<float*>(workspace) : nullptr;
+  a.dy_rs = dy_row_stride;
+  a.x_rs = x_row_stride;
+  a.dx_rs = dx_row_stride;
+  a.rows_per_group = rows / groups;
+  a.C = int(cols);
+  a.parts = int(bwd_parts(rows / groups, groups));
+  a.plus = one_plus ? 1.0f : 0.0f;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (dtype == PKV_BF16)
+    return wtype == PKV_FP32
+               ? run_bwd<__nv_bfloat16, float>(a, groups, dweight, dbias, s)
+               : run_bwd<__nv_bfloat16, __nv_bfloat16>(a, groups, dweight, dbias, s);
+  if (dtype == PKV_FP16)
+    return wtype == PKV_FP32 ? run_bwd<__half, float>(a, groups, dweight, dbias, s)
+                             : run_bwd<__half, __half>(a, groups, dweight, dbias, s);
+  return run_bwd<float, float>(a, groups, dweight, dbias, s);
+}

@@ -1,0 +1,198 @@
+// Rotary positions of queries and keys: 1 to 4 position axes, interleaved or
+// half pairing, any leading part of the head, fp32 arithmetic.
+//
+// Pair p < P of a head belongs to axis a = axis[p] and turns by
+//   phi = position[token][a] * inv_freq[p]
+//   (u, v) -> scale * (u cos phi - v sin phi, u sin phi + v cos phi)
+// with (u, v) = elements (2p, 2p + 1) (interleaved) or (p, p + P) (half);
+// elements from 2P on are copied.  `inverse` turns by -phi: the transpose,
+// which is the gradient's pass.
+//
+// Bound by HBM: every element is read and written once.  A block owns a few
+// tokens: its threads first work out the tokens' cosines and sines once into
+// shared memory (the angle is the same in every head of q and of k), then
+// stream the heads of q and k through registers in accesses of up to 16
+// bytes.  No frequency tables in memory, so a position may be any int64: the
+// turn count position * inv_freq / 2 pi is formed and reduced in float64 (a
+// position of 10^6 at fp32 would be off by a tenth of a radian), and the
+// reduced angle goes through sincospif with its rounding remainder added back
+// to first order, so cos and sin are good to fp32's last bit.
+#include "pkv_vec.cuh"
+
+namespace pkv {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTable = 2048;  // (token, pair) entries of a block's table
+constexpr int kRotAxes = 4;
+
+struct RotSide {
+  const void* x;
+  void* out;
+  int64_t x_tok, x_head, o_tok, o_head;
+  int heads;
+};
+
+struct RotArgs {
+  RotSide s[2];
+  int64_t tokens;
+  const int64_t* pos;
+  const double* inv_freq;
+  const int32_t* axis;  // nullptr: one axis
+  int n_axes, D, P, half, tile;
+  float scale, sign;
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
+  __shared__ float2 tab[kRotTable];
+  const int64_t t0 = blockIdx.x * int64_t(a.tile);
+  const int nt = int(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
+  for (int i = threadIdx.x; i < nt * a.P; i += kRotThreads) {
+    const int t = i / a.P, p = i - t * a.P;
+    int ax = a.axis ? a.axis[p] : 0;
+    ax = ax < 0 ? 0 : (ax >= a.n_axes ? a.n_axes - 1 : ax);
+    const double turns = double(a.pos[(t0 + t) * a.n_axes + ax]) *
+                         (a.inv_freq[p] * 0.15915494309189533577);  // 1 / (2 pi)
+    const double x = 2.0 * (turns - rint(turns));                   // half turns, [-1, 1]
+    const float hi = float(x), lo = float(x - double(hi)) * 3.14159265f;
+    float s, c;
+    sincospif(hi, &s, &c);
+    tab[i] = make_float2(fmaf(-lo, s, c) * a.scale, fmaf(lo, c, s) * a.scale * a.sign);
+  }
+  __syncthreads();
+  const int turn = a.P / V;                 // units of V pairs of a head
+  const int units = turn + (a.D - 2 * a.P) / V;  // and of V copied elements
+  const int h0 = a.s[0].heads, heads = h0 + a.s[1].heads;
+  const int n = nt * heads * units;
+  for (int i = threadIdx.x; i < n; i += kRotThreads) {
+    const int u = i % units, th = i / units;
+    const int t = th / heads;
+    int h = th - t * heads;
+    const bool second = h >= h0;
+    if (second) h -= h0;
+    const RotSide& sd = a.s[second ? 1 : 0];
+    const T* x = static_cast<const T*>(sd.x) + (t0 + t) * sd.x_tok + h * sd.x_head;
+    T* o = static_cast<T*>(sd.out) + (t0 + t) * sd.o_tok + h * sd.o_head;
+    if (u >= turn) {
+      const int e = 2 * a.P + (u - turn) * V;
+      st_vec<T, V>(o + e, ld_vec<T, V>(x + e));
+      continue;
+    }
+    const float2* cs = tab + t * a.P + u * V;
+    const int e0 = a.half ? u * V : 2 * u * V;
+    const int e1 = a.half ? a.P + u * V : 2 * u * V + V;
+    const Vec<T, V> x0 = ld_vec<T, V>(x + e0), x1 = ld_vec<T, V>(x + e1);
+    Vec<T, V> y0, y1;
+    if (a.half) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = to_f32(x0.v[j]), q = to_f32(x1.v[j]);
+        const float2 w = cs[j];
+        y0.v[j] = from_f32<T>(p * w.x - q * w.y);
+        y1.v[j] = from_f32<T>(p * w.y + q * w.x);
+      }
+    } else {
+      T in[2 * V], r[2 * V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        in[j] = x0.v[j];
+        in[V + j] = x1.v[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = to_f32(in[2 * j]), q = to_f32(in[2 * j + 1]);
+        const float2 w = cs[j];
+        r[2 * j] = from_f32<T>(p * w.x - q * w.y);
+        r[2 * j + 1] = from_f32<T>(p * w.y + q * w.x);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y0.v[j] = r[j];
+        y1.v[j] = r[V + j];
+      }
+    }
+    st_vec<T, V>(o + e0, y0);
+    st_vec<T, V>(o + e1, y1);
+  }
+}
+
+template <typename T, int V>
+bool rot_fits(const RotArgs& a) {
+  if (a.P % V || a.D % V) return false;
+  for (const RotSide& s : a.s) {
+    if (s.heads == 0) continue;
+    if (!vec_ok(s.x, s.x_tok, V, sizeof(T)) || !vec_ok(s.out, s.o_tok, V, sizeof(T)) ||
+        s.x_head % V || s.o_head % V)
+      return false;
+  }
+  return true;
+}
+
+template <typename T>
+int run_rotary(const RotArgs& a, int64_t grid, cudaStream_t s) {
+  // the widest access that divides the pairs, the head, the strides and the
+  // addresses
+  constexpr int kWide = 16 / sizeof(T);
+  if (rot_fits<T, kWide>(a))
+    rotary_kernel<T, kWide><<<int(grid), kRotThreads, 0, s>>>(a);
+  else if (kWide > 4 && rot_fits<T, 4>(a))
+    rotary_kernel<T, 4><<<int(grid), kRotThreads, 0, s>>>(a);
+  else if (rot_fits<T, 2>(a))
+    rotary_kernel<T, 2><<<int(grid), kRotThreads, 0, s>>>(a);
+  else
+    rotary_kernel<T, 1><<<int(grid), kRotThreads, 0, s>>>(a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int pkv_rotary(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int q_heads,
+                          void* q_out, int64_t qo_tok_stride, int64_t qo_head_stride,
+                          const void* k, int64_t k_tok_stride, int64_t k_head_stride, int k_heads,
+                          void* k_out, int64_t ko_tok_stride, int64_t ko_head_stride, int dtype,
+                          int64_t tokens, int head_dim, const int64_t* positions, int axes,
+                          const double* inv_freq, const int32_t* axis, int pairs, int half,
+                          float scale, int inverse, pkv_stream_t stream) {
+  if (dtype < PKV_BF16 || dtype > PKV_FP32 || tokens < 0 || q_heads < 0 || k_heads < 0)
+    return PKV_EINVAL;
+  if (tokens == 0 || q_heads + k_heads == 0) return PKV_OK;
+  if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || head_dim <= 0 || pairs < 0 ||
+      2 * int64_t(pairs) > head_dim || axes < 1 || axes > kRotAxes || (axes > 1 && !axis) ||
+      (pairs > 0 && (!positions || !inv_freq)))
+    return PKV_EINVAL;
+  if (pairs > kRotTable || head_dim > 65536 || q_heads > 65536 || k_heads > 65536)
+    return PKV_EUNSUPPORTED;
+  RotArgs a{};
+  a.s[0] = {q, q_out, q_tok_stride, q_head_stride, qo_tok_stride, qo_head_stride, q_heads};
+  a.s[1] = {k, k_out, k_tok_stride, k_head_stride, ko_tok_stride, ko_head_stride, k_heads};
+  a.tokens = tokens;
+  a.pos = positions;
+  a.inv_freq = inv_freq;
+  a.axis = axes > 1 ? axis : nullptr;
+  a.n_axes = axes;
+  a.D = head_dim;
+  a.P = pairs;
+  a.half = half;
+  a.scale = scale;
+  a.sign = inverse ? -1.0f : 1.0f;
+  // tokens of a block: its table of angles fits, its elements count in 32
+  // bits, and there are blocks for every SM
+  int64_t tile = pairs > 0 ? kRotTable / pairs : 64;
+  const int64_t row = int64_t(q_heads + k_heads) * head_dim;
+  const int64_t fill = (tokens + sm_count() * 8 - 1) / (int64_t(sm_count()) * 8);
+  if (tile > 8) tile = 8;
+  if (tile > fill) tile = fill;
+  if (tile < 1) tile = 1;
+  if (tile * row >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  a.tile = int(tile);
+  const int64_t grid = (tokens + tile - 1) / tile;
+  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (dtype == PKV_BF16) return run_rotary<__nv_bfloat16>(a, grid, s);
+  if (dtype == PKV_FP16) return run_rotary<__half>(a, grid, s);
+  return run_rotary<float>(a, grid, s);
+}

@@ -1,0 +1,84 @@
+// Element types and small vectors of the token-path kernels (layer norm,
+// rotary positions): every value is computed in fp32 and rounded once to the
+// tensor's type when it is stored.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "pkv_common.cuh"
+
+namespace pkv {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+  return __half2float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// N consecutive elements, loaded and stored as one access of N * sizeof(T)
+// bytes (<= 16) when the address is a multiple of that.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Vec {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> ld_vec(const T* p) {
+  return *reinterpret_cast<const Vec<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void st_vec(T* p, const Vec<T, N>& v) {
+  *reinterpret_cast<Vec<T, N>*>(p) = v;
+}
+
+// N consecutive elements as fp32, in accesses of up to 16 bytes (aligned to
+// that where N > 1).
+template <typename T, int N>
+__device__ __forceinline__ void ld_f32(const T* p, float (&f)[N]) {
+  constexpr int M = N * sizeof(T) > 16 ? int(16 / sizeof(T)) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += M) {
+    const Vec<T, M> t = ld_vec<T, M>(p + i);
+#pragma unroll
+    for (int e = 0; e < M; ++e) f[i + e] = to_f32(t.v[e]);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Whether `p` and a row stride (elements) keep every row on a boundary of n
+// elements of `size` bytes.
+inline bool vec_ok(const void* p, int64_t row_stride, int n, int size) {
+  return p == nullptr ||
+         (reinterpret_cast<uintptr_t>(p) % (uintptr_t(n) * size) == 0 && row_stride % n == 0);
+}
+
+}  // namespace pkv

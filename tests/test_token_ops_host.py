@@ -1,0 +1,99 @@
+"""Host side of the token-path operators, without a GPU: the frequency tables,
+the argument checks of the Python entry points and of the C ABI (an error code
+before anything is launched)."""
+from __future__ import annotations
+
+import ctypes
+import math
+import os
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+EINVAL, EUNSUPPORTED = 1, 4
+LIB = os.path.join(ROOT, "pyramid-forcing_b200", "pyramidkv", "lib", "libpkv.so")
+I64, INT, PTR, FLT = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_float
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return ctypes.CDLL(LIB)
+
+
+def test_frequency_tables():
+    from pyramidkv.rope import axial_frequencies, rotary_frequencies
+    inv, s = rotary_frequencies(8)
+    assert s == 1.0 and torch.allclose(inv, torch.tensor([1.0, 0.1, 0.01, 0.001],
+                                                         dtype=torch.float64))
+    lin, _ = rotary_frequencies(8, scaling="linear", factor=4.0)
+    assert torch.equal(lin, inv / 4)
+    ntk, _ = rotary_frequencies(8, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1.0 and math.isclose(float(ntk[-1]), float(inv[-1]) / 4, rel_tol=1e-12)
+    yarn, s = rotary_frequencies(64, scaling="yarn", factor=4.0, original_length=2048)
+    full = rotary_frequencies(64)[0]
+    turns = 2048 * full / (2 * math.pi)
+    assert torch.equal(yarn[turns >= 32], full[turns >= 32])
+    assert torch.allclose(yarn[turns <= 1], full[turns <= 1] / 4, rtol=1e-15)
+    between = (turns < 32) & (turns > 1)
+    assert between.any() and ((yarn < full) & (yarn > full / 4))[between].all()
+    assert math.isclose(s, 0.1 * math.log(4) + 1)
+    inv, axis = axial_frequencies((44, 42, 42))
+    assert inv.numel() == 64 and axis.tolist() == [0] * 22 + [1] * 21 + [2] * 21
+    assert inv[22] == inv[43] == 1.0 and axis.dtype == torch.int32
+    for bad in (dict(dim=7), dict(dim=8, scaling="other"), dict(dim=8, factor=0.5)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**bad)
+
+
+def test_python_entry_points_refuse_cpu_tensors():
+    from pyramidkv.norm import layer_norm
+    from pyramidkv.rope import rotary_apply
+    with pytest.raises(ValueError, match="CUDA"):
+        layer_norm(torch.zeros(2, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        rotary_apply(torch.zeros(2, 1, 4), torch.zeros(2, dtype=torch.int64),
+                     torch.ones(2, dtype=torch.float64))
+
+
+def test_layer_norm_abi_checks(lib):
+    p = PTR(256)  # never dereferenced: every call below is refused
+
+    def fwd(x=p, rs=8, dt=0, wt=0, rows=4, cols=8, groups=1, eps=1e-6, y=p):
+        return lib.pkv_layer_norm(x, I64(rs), p, p, INT(dt), INT(wt), I64(rows), I64(cols),
+                                  I64(groups), FLT(eps), INT(0), y, I64(8), None, None, None)
+    for bad in (dict(rows=-1), dict(cols=0), dict(groups=0), dict(groups=3), dict(dt=3),
+                dict(dt=2, wt=0), dict(dt=0, wt=1), dict(x=None), dict(y=None), dict(eps=-1.0),
+                dict(eps=float("nan"))):
+        assert fwd(**bad) == EINVAL, bad
+    assert fwd(cols=(1 << 20) + 1) == EUNSUPPORTED
+    assert fwd(rows=0) == 0
+
+    lib.pkv_layer_norm_workspace_bytes.restype = I64
+    need = lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8), I64(2))
+    assert need == 2 * 1 * 2 * 8 * 4           # two rows a group: one part
+    assert lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8), I64(3)) == 0
+
+    def bwd(dy=p, x=p, mean=p, dt=0, wt=0, rows=4, cols=8, groups=2, dw=p, ws=p, size=need):
+        return lib.pkv_layer_norm_backward(
+            dy, I64(8), x, I64(8), p, mean, p, INT(dt), INT(wt), I64(rows), I64(cols),
+            I64(groups), INT(0), p, I64(8), dw, None, ws, I64(size), None)
+    for bad in (dict(dy=None), dict(x=None), dict(mean=None), dict(rows=0), dict(groups=3),
+                dict(ws=None), dict(size=need - 1), dict(ws=PTR(258)), dict(wt=1)):
+        assert bwd(**bad) == EINVAL, bad
+
+
+def test_rotary_abi_checks(lib):
+    p = PTR(256)
+
+    def call(q=p, qh=2, k=p, kh=2, dt=0, tokens=4, dim=8, pos=p, axes=1, inv=p, axis=p, pairs=4):
+        return lib.pkv_rotary(q, I64(16), I64(8), INT(qh), p, I64(16), I64(8), k, I64(16), I64(8),
+                              INT(kh), p, I64(16), I64(8), INT(dt), I64(tokens), INT(dim), pos,
+                              INT(axes), inv, axis, INT(pairs), INT(0), FLT(1.0), INT(0), None)
+    for bad in (dict(q=None), dict(k=None), dict(qh=-1), dict(dt=3), dict(tokens=-1), dict(dim=0),
+                dict(pairs=5), dict(pairs=-1), dict(axes=0), dict(axes=5), dict(pos=None),
+                dict(inv=None), dict(axes=2, axis=None)):
+        assert call(**bad) == EINVAL, bad
+    assert call(dim=8192, pairs=2049) == EUNSUPPORTED
+    assert call(tokens=0) == 0 and call(qh=0, kh=0) == 0
