@@ -30,7 +30,8 @@ CU_SOURCES = ["pkv_update.cu", "pkv_merge.cu", "pkv_plan.cu", "pkv_pack.cu", "pk
               "pkv_attend.cu", "pkv_legacy.cu", "pkv_rope.cu", "pkv_exchange.cu", "pkv_norm.cu",
               "pkv_rotary.cu"]
 BIND_SOURCES = ["adahead_bind.cpp", "token_bind.cpp"]
-HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh", "pkv_vec.cuh"]
+HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh", "pkv_vec.cuh",
+           "pkv_tc.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
            "--ptxas-options=-v"] + ARCH
