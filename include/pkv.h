@@ -267,6 +267,51 @@ int pkv_attention_ws(const uint16_t *q, int64_t q_row_stride, int64_t q_head_str
                      int64_t o_row_stride, int64_t o_head_stride, void *workspace,
                      int64_t workspace_bytes, pkv_stream_t stream);
 
+/* ---- block-sparse attention over the ragged layout ---------------------------
+ * The keys of every (chunk, head) segment of pkv_attention's layout are cut
+ * into blocks of `block` keys (64 or 128; a segment's last block may be
+ * shorter).  Every group of query_block (1-128) consecutive rows of a chunk
+ * (a chunk's last group may be shorter) selects top_k (1-1024) blocks and
+ * attends their keys.  head_dim 64 or 128.  No counterparts in the reference,
+ * which attends the whole packed cache.
+ *
+ * pkv_block_means: the mean key of every block, fp32: block j of segment s at
+ * row cu[s] / block + s + j of `means` [means_rows, head_dim];
+ * pkv_block_rows rows hold any segmentation of kv_rows keys.  Rows that no
+ * block has are zeroed when zero_rest, else left as they were.
+ */
+int64_t pkv_block_rows(int64_t kv_rows, int segments, int block);
+int pkv_block_means(const uint16_t *k, int64_t kv_rows, int head_dim,
+                    const int32_t *cu_seqlens_k, int segments, int block, float *means,
+                    int64_t means_rows, int zero_rest, pkv_stream_t stream);
+
+/*
+ * For every (segment, group): the top_k blocks of highest score (the group's
+ * queries summed, times the block's mean, in float64), equal scores by index,
+ * NaN last; listed ascending, -1 behind the last.  blocks: int32
+ * [num_chunks * num_heads, ceil(rows_per_chunk / query_block), top_k].
+ * q as in pkv_attention (16-byte aligned, strides multiples of 8).
+ */
+int pkv_select_blocks(const uint16_t *q, int64_t q_row_stride, int64_t q_head_stride,
+                      const float *means, int64_t means_rows, const int32_t *cu_seqlens_k,
+                      int64_t kv_rows, int num_chunks, int num_heads, int rows_per_chunk,
+                      int head_dim, int query_block, int block, int top_k, int32_t *blocks,
+                      pkv_stream_t stream);
+
+/*
+ * pkv_attention over the listed blocks only (a caller may list any: entries
+ * outside the segment are skipped, a block listed twice counts twice, a row
+ * with no keys gives zeros).  softmax_scale > 0.  status (nullable):
+ * PKV_ST_TIMEOUT when a bounded device wait expired.
+ */
+int pkv_block_attention(const uint16_t *q, int64_t q_row_stride, int64_t q_head_stride,
+                        const uint16_t *k, const uint16_t *v, int64_t kv_rows,
+                        const int32_t *cu_seqlens_k, int num_chunks, int num_heads,
+                        int rows_per_chunk, int head_dim, float softmax_scale,
+                        const int32_t *blocks, int query_block, int block, int top_k,
+                        uint16_t *out, int64_t o_row_stride, int64_t o_head_stride,
+                        int32_t *status, pkv_stream_t stream);
+
 /*
  * One layer's MegaCache.update on the device: restore the committed
  * valid_count / recent pool, route each head's frames to sink or recent (FIFO

@@ -28,7 +28,7 @@ NVCC = os.path.join(CUDA, "bin", "nvcc")
 
 CU_SOURCES = ["pkv_update.cu", "pkv_merge.cu", "pkv_plan.cu", "pkv_pack.cu", "pkv_attn.cu",
               "pkv_attend.cu", "pkv_legacy.cu", "pkv_rope.cu", "pkv_exchange.cu", "pkv_norm.cu",
-              "pkv_rotary.cu"]
+              "pkv_rotary.cu", "pkv_sparse.cu"]
 BIND_SOURCES = ["adahead_bind.cpp", "token_bind.cpp"]
 HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh", "pkv_vec.cuh",
            "pkv_tc.cuh"]

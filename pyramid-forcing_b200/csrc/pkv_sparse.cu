@@ -1,0 +1,1135 @@
+// Block-sparse attention over the ragged K/V layout: the keys of every
+// (chunk, head) segment are cut into blocks of `block` keys, every group of
+// `query_block` consecutive query rows of a chunk keeps the top_k blocks whose
+// mean key scores highest against the group's summed query, and attends the
+// keys of those blocks only.
+//
+//   mean_j   = sum of the block's keys / their number        (fp32, rounded once)
+//   score_gj = (sum over the group's rows of q) . mean_j     (float64)
+//   sel_g    = top_k highest scores, equal ones by index, listed ascending, -1 behind
+//   out_r    = softmax(scale * q_r . k) v over the keys of sel_g
+//
+// Three kernels:
+//  * block_means_kernel -- one pass over K, bound by HBM.  Segment s's block j
+//    has row cu[s] / block + s + j of the table: a closed form, so the table
+//    needs no offsets of its own (ceil(n / B) <= floor((a + n) / B) - floor(a / B) + 1).
+//  * select_blocks_kernel -- a CTA a group.  Which block comes last is decided
+//    by the order of two scores, so sums are float64 (of bf16 terms: exact)
+//    and products of the fp32 means are exact before their float64 sum: the
+//    choice does not depend on the order of summation.
+//  * attention over the listed blocks, by the rows of a group:
+//    up to 16 rows (a decoded token, a small group): warps each take 16 keys,
+//    K and V go from memory straight into mma fragments, a thread-block
+//    cluster splits the list and joins the parts through distributed shared
+//    memory -- bound by latency and by the bytes of the listed blocks;
+//    more rows: tcgen05 tiles of 128 rows (see sparse_tc_kernel).
+#include <mutex>
+
+#include "pkv_internal.h"
+#include "pkv_tc.cuh"
+
+namespace pkv {
+namespace {
+
+constexpr int kMaxTopK = 1024;
+constexpr int kFewRows = 16;  // rows of a group served by the mma kernel
+
+struct SegView {
+  int start, len;
+};
+
+// Segment s clipped to the K/V rows that exist: a corrupt cu_seqlens reads
+// nothing out of range.
+__device__ __forceinline__ SegView segment(const int32_t* cu, int s, int64_t kv_rows) {
+  const int64_t a = max(cu[s], 0), b = min(int64_t(cu[s + 1]), kv_rows);
+  return {int(min(a, kv_rows)), b > a ? int(b - a) : 0};
+}
+
+// ---------------------------------------------------------------------------
+// Block means
+// ---------------------------------------------------------------------------
+// A warp a table row: 16 (D = 128) or 8 lanes a key, 8 elements each.  Four
+// keys are added in fp32 (exact unless their exponents differ by 14) before a
+// float64 add, which keeps the conversions off the critical pipe.
+template <int D>
+__global__ void __launch_bounds__(256)
+    block_means_kernel(const uint16_t* __restrict__ k, int64_t kv_rows,
+                       const int32_t* __restrict__ cu, int n_seg, int block,
+                       float* __restrict__ means, int64_t rows, int zero_rest) {
+  constexpr int kLanes = D / 8, kKeys = 32 / kLanes;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / kLanes, d0 = (lane % kLanes) * 8;
+  const int64_t step = int64_t(gridDim.x) * (blockDim.x >> 5);
+  const int64_t used = int64_t(cu[n_seg]) / block + n_seg;
+  for (int64_t row = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5); row < rows;
+       row += step) {
+    if (row >= used && !zero_rest) break;
+    // last segment whose first row is <= row
+    int lo = 0, hi = n_seg - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (int64_t(cu[mid]) / block + mid <= row)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    const SegView sg = segment(cu, lo, kv_rows);
+    const int64_t j = row - (int64_t(cu[lo]) / block + lo);
+    const int64_t first = j * block;
+    float* out = means + row * D;
+    if (j < 0 || first >= sg.len) {  // no block has this row
+      if (zero_rest)
+        for (int d = lane * 4; d < D; d += 128)
+          *reinterpret_cast<float4*>(out + d) = make_float4(0.f, 0.f, 0.f, 0.f);
+      continue;
+    }
+    const int n = min(int64_t(block), sg.len - first);
+    const uint16_t* p = k + (sg.start + first) * D + d0;
+    double acc[8] = {};
+    for (int r = sub; r < n; r += 4 * kKeys) {
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = r + i * kKeys < n
+                   ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kKeys) * D))
+                   : make_uint4(0, 0, 0, 0);
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float lo4[4], hi4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
+          hi4[i] = __uint_as_float(u & 0xffff0000u);
+        }
+        f[2 * e] = (lo4[0] + lo4[1]) + (lo4[2] + lo4[3]);
+        f[2 * e + 1] = (hi4[0] + hi4[1]) + (hi4[2] + hi4[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += double(f[e]);
+    }
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+    if (sub == 0) {
+      const double inv = 1.0 / double(n);
+      const bool pow2 = (n & (n - 1)) == 0;  // then the product is exact
+      float m[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[e] = float(pow2 ? acc[e] * inv : acc[e] / double(n));
+      *reinterpret_cast<float4*>(out + d0) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(out + d0 + 4) = make_float4(m[4], m[5], m[6], m[7]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Selection
+// ---------------------------------------------------------------------------
+constexpr int kSelThreads = 256;
+constexpr int kSelChunk = 2048;  // scores added per round
+
+struct SelectArgs {
+  const uint16_t* q;
+  int64_t q_rs, q_hs, kv_rows, means_rows;
+  const float* means;
+  const int32_t* cu;
+  int32_t* blocks;
+  int H, rows_per_chunk, groups, query_block, block, top_k;
+};
+
+struct SelectSmem {
+  union {
+    double red[kSelThreads / 8][128];  // partial query sums (D = 64: two rows' worth used)
+    struct {
+      uint64_t key[kMaxTopK + kSelChunk];
+      int id[kMaxTopK + kSelChunk];
+    } c;
+  };
+  double q[128];
+  int hist[256];
+  int wsum[2][kSelThreads / 32];
+  uint64_t prefix;
+  uint64_t lo, hi;
+  int need, done;
+};
+
+// Scores as integers in the same order; NaN below all, -0 as 0.
+__device__ __forceinline__ uint64_t order_key(double s) {
+  if (s != s) return 0;
+  if (s == 0.0) s = 0.0;
+  const int64_t b = __double_as_longlong(s);
+  return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  SelectSmem& sm = *reinterpret_cast<SelectSmem*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int s = blockIdx.x / a.groups, g = blockIdx.x - s * a.groups;
+  const int c = s / a.H, h = s - c * a.H;
+  const SegView sg = segment(a.cu, s, a.kv_rows);
+  const int nblk = (sg.len + a.block - 1) / a.block;
+  int32_t* out = a.blocks + (int64_t(s) * a.groups + g) * a.top_k;
+  if (nblk <= a.top_k) {  // every block is kept
+    for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
+    return;
+  }
+  // ---- sum of the group's queries, float64 (exact for bf16 of like size) ----
+  const int r0 = g * a.query_block;
+  const int nr = min(a.query_block, a.rows_per_chunk - r0);
+  {
+    constexpr int kLanes = D / 8, kRows = kSelThreads / kLanes;
+    const int sub = tid / kLanes, d0 = (tid % kLanes) * 8;
+    const uint16_t* p =
+        a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
+    double acc[8] = {};
+    for (int r = sub; r < nr; r += kRows) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p + r * a.q_rs));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[2 * e] += double(bf16_bits_to_f32(u[e] & 0xffffu));
+        acc[2 * e + 1] += double(__uint_as_float(u[e] & 0xffff0000u));
+      }
+    }
+    double* red = &sm.red[0][0];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[sub * D + d0 + e] = acc[e];
+    __syncthreads();
+    if (tid < D) {
+      double t = 0.0;
+      for (int i = 0; i < min(kRows, nr); ++i) t += red[i * D + tid];
+      sm.q[tid] = t;
+    }
+    __syncthreads();
+  }
+  // ---- scores: 8 lanes a block, D / 8 products each ----
+  constexpr int kPer = D / 8;
+  const int l8 = tid & 7;
+  double q[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) q[i] = sm.q[(i / 4) * 32 + l8 * 4 + (i & 3)];
+  const int64_t base = int64_t(a.cu[s]) / a.block + s;
+  int kept = 0;
+  for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
+    const int m = min(kSelChunk, nblk - b0);
+    uint64_t mn = ~uint64_t(0), mx = 0;
+    for (int i = tid >> 3; i < (m + 31) / 32 * 32; i += kSelThreads / 8) {
+      double t = 0.0;
+      const int64_t row = base + b0 + i;
+      if (i < m && row >= 0 && row < a.means_rows) {
+        const float* p = a.means + row * D + l8 * 4;
+        float4 f[kPer / 4];
+#pragma unroll
+        for (int e = 0; e < kPer / 4; ++e) f[e] = __ldg(reinterpret_cast<const float4*>(p + e * 32));
+#pragma unroll
+        for (int e = 0; e < kPer / 4; ++e) {
+          t = fma(double(f[e].x), q[4 * e], t);
+          t = fma(double(f[e].y), q[4 * e + 1], t);
+          t = fma(double(f[e].z), q[4 * e + 2], t);
+          t = fma(double(f[e].w), q[4 * e + 3], t);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (i < m && l8 == 0) {
+        const uint64_t key = order_key(t);
+        sm.c.key[kept + i] = key;
+        sm.c.id[kept + i] = b0 + i;
+      }
+    }
+    __syncthreads();
+    const int total = kept + m;
+    const bool last = b0 + m == nblk;
+    if (total <= a.top_k) {  // (not the last round: nblk > top_k)
+      kept = total;
+      continue;
+    }
+    // ---- the top_k-th key: digits of 8 bits from the highest that differs ----
+    for (int i = tid; i < total; i += kSelThreads) {
+      mn = min(mn, sm.c.key[i]);
+      mx = max(mx, sm.c.key[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (tid == 0) {
+      sm.lo = ~uint64_t(0);
+      sm.hi = 0;
+    }
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), mn);
+      atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), mx);
+    }
+    __syncthreads();
+    mn = sm.lo;
+    mx = sm.hi;
+    int shift = mn == mx ? 0 : 64 - __clzll(mn ^ mx);  // bits below `shift` differ
+    uint64_t prefix = shift == 64 ? 0 : mx >> shift;
+    int need = a.top_k;
+    bool exact = false;  // every key with the prefix is kept
+    while (shift > 0 && !exact) {
+      const int bits = min(8, shift);
+      shift -= bits;
+      for (int i = tid; i < 256; i += kSelThreads) sm.hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < total; i += kSelThreads) {
+        const uint64_t key = sm.c.key[i];
+        const uint64_t up = shift + bits == 64 ? 0 : key >> (shift + bits);
+        if (up == prefix) atomicAdd(&sm.hist[int(key >> shift) & ((1 << bits) - 1)], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // lane owns bins 255 - 8 lane .. 248 - 8 lane: a scan from the top
+        int cnt[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += cnt[i] = sm.hist[255 - 8 * lane - i];
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        before -= sum;
+        if (before < need && before + sum >= need) {
+          int acc = before;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (acc < need && acc + cnt[i] >= need) {
+              sm.prefix = (prefix << bits) | uint64_t(255 - 8 * lane - i);
+              sm.need = need - acc;
+              sm.done = cnt[i] == need - acc;
+            }
+            acc += cnt[i];
+          }
+        }
+      }
+      __syncthreads();
+      prefix = sm.prefix;
+      need = sm.need;
+      exact = sm.done != 0;
+      __syncthreads();
+    }
+    // ---- keep: above the prefix, and the first `need` at it, in index order ----
+    int eq_seen = 0, written = 0;
+    for (int t0 = 0; t0 < total; t0 += kSelThreads) {
+      const int i = t0 + tid;
+      const uint64_t key = i < total ? sm.c.key[i] : 0;
+      const int id = i < total ? sm.c.id[i] : 0;
+      const uint64_t up = shift == 64 ? 0 : key >> shift;
+      const bool gt = i < total && up > prefix, eq = i < total && up == prefix;
+      const uint32_t be = __ballot_sync(0xffffffffu, eq);
+      if (lane == 0) sm.wsum[0][warp] = __popc(be);
+      __syncthreads();
+      int er = eq_seen + __popc(be & ((1u << lane) - 1));
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        if (w < warp) er += sm.wsum[0][w];
+        eq_seen += sm.wsum[0][w];
+      }
+      const bool keep = gt || (eq && er < need);
+      const uint32_t bk = __ballot_sync(0xffffffffu, keep);
+      if (lane == 0) sm.wsum[1][warp] = __popc(bk);
+      __syncthreads();
+      int at = written + __popc(bk & ((1u << lane) - 1));
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        if (w < warp) at += sm.wsum[1][w];
+        written += sm.wsum[1][w];
+      }
+      // at <= i, and every key of this tile is in registers: in place
+      if (keep && at < a.top_k) {
+        if (last)
+          out[at] = id;
+        else {
+          sm.c.key[at] = key;
+          sm.c.id[at] = id;
+        }
+      }
+      __syncthreads();
+    }
+    kept = a.top_k;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention of up to 16 rows
+// ---------------------------------------------------------------------------
+struct SparseArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_rs, q_hs, kv_rows, o_rs, o_hs;
+  const int32_t* cu;
+  const int32_t* blocks;
+  uint16_t* out;
+  int32_t* status;
+  int H, rows_per_chunk, groups, query_block, block, top_k;
+  float scale_log2;
+};
+
+constexpr int kFewWarps = 8;
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& w, int i) {
+  return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
+  uint32_t addr;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(su32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Partial results of the warps and of the CTA: unnormalised O, maximum, sum.
+template <int D>
+struct FewSmem {
+  float o[kFewWarps][kFewRows][D];
+  float m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
+  float co[kFewRows][D];
+  float cm[kFewRows], cl[kFewRows];
+  int list[kMaxTopK];
+  int count;
+};
+
+// A cluster a (segment, group); its warps take chunks of 16 keys of the listed
+// blocks in turn.  With the fragment layout of mma.m16n8k16 a lane (g, c) =
+// (lane / 4, lane % 4) holds, of a tile of 8 keys, key g and two dim pairs per
+// k-step.  The order of the contraction is free, so k-steps 2i, 2i + 1 take
+// dims 32 i + 8 c .. + 7: one 16-byte load a key and 32 dims, for Q alike.  For
+// P V, lane (g, c) holds keys 2c, 2c + 1, 2c + 8, 2c + 9 of column g of an
+// output tile; columns are free too, so tile t takes dim 8 g + t: four
+// 16-byte loads of V rows serve 8 tiles after pairing the halves of two keys.
+template <int D>
+__global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  FewSmem<D>& sm = *reinterpret_cast<FewSmem<D>*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int X = int(cluster_size()), rank = int(cluster_rank());
+  const int unit = blockIdx.x / X;
+  const int s = unit / a.groups, grp = unit - s * a.groups;
+  const int ch = s / a.H, h = s - ch * a.H;
+  const int r0 = grp * a.query_block;
+  const int nr = min(a.query_block, a.rows_per_chunk - r0);
+  const SegView sg = segment(a.cu, s, a.kv_rows);
+  const int nblk = (sg.len + a.block - 1) / a.block;
+  const int g = lane >> 2, c = lane & 3;
+  // ---- the listed blocks that exist, in order ----
+  if (warp == 0) {
+    const int32_t* lst = a.blocks + int64_t(unit) * a.top_k;
+    int n = 0;
+    for (int b = 0; b < a.top_k; b += 32) {
+      const int e = b + lane < a.top_k ? lst[b + lane] : -1;
+      const bool ok = e >= 0 && e < nblk;
+      const uint32_t m = __ballot_sync(0xffffffffu, ok);
+      if (ok) sm.list[n + __popc(m & ((1u << lane) - 1))] = e;
+      n += __popc(m);
+    }
+    if (lane == 0) sm.count = n;
+  }
+  // ---- queries as A fragments ----
+  const uint16_t* qp =
+      a.q + (int64_t(ch) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs;
+  uint4 q0[D / 32], q1[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    q0[i] = g < nr ? *reinterpret_cast<const uint4*>(qp + g * a.q_rs + 32 * i + 8 * c)
+                   : make_uint4(0, 0, 0, 0);
+    q1[i] = g + 8 < nr ? *reinterpret_cast<const uint4*>(qp + (g + 8) * a.q_rs + 32 * i + 8 * c)
+                       : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  const int per = a.block / 16;
+  const int chunks = sm.count * per;
+  float o[D / 8][4];
+#pragma unroll
+  for (int t = 0; t < D / 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  for (int i = rank * kFewWarps + warp; i < chunks; i += X * kFewWarps) {
+    const int key0 = sm.list[i / per] * a.block + (i % per) * 16;
+    const int valid = sg.len - key0;  // keys of this chunk inside the segment
+    if (valid <= 0) continue;
+    const uint16_t* kp = a.k + (int64_t(sg.start) + key0) * D;
+    const uint16_t* vp = a.v + (int64_t(sg.start) + key0) * D;
+    uint4 kw[2][D / 32], vw[4][D / 64];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e)
+        kw[t][e] = t * 8 + g < valid
+                       ? __ldg(reinterpret_cast<const uint4*>(kp + (t * 8 + g) * D + 32 * e + 8 * c))
+                       : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int key = 2 * c + (t & 1) + (t >> 1) * 8;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e)
+        vw[t][e] = key < valid
+                       ? __ldg(reinterpret_cast<const uint4*>(vp + key * D + 64 * e + 8 * g))
+                       : make_uint4(0, 0, 0, 0);
+    }
+    float sc[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        mma_16816(sc[t], q0[e].x, q1[e].x, q0[e].y, q1[e].y, kw[t][e].x, kw[t][e].y);
+        mma_16816(sc[t], q0[e].z, q1[e].z, q0[e].w, q1[e].w, kw[t][e].z, kw[t][e].w);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sc[t][e] = t * 8 + 2 * c + (e & 1) < valid ? sc[t][e] * a.scale_log2 : -INFINITY;
+    }
+    float n0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+    float n1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+    }
+    n0 = fmaxf(n0, m0);
+    n1 = fmaxf(n1, m1);
+    // a row whose scores are all -inf keeps a reference of 0
+    const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
+    const float f0 = fast_exp2(m0 - u0), f1 = fast_exp2(m1 - u1);
+    m0 = n0;
+    m1 = n1;
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      p[t][0] = fast_exp2(sc[t][0] - u0);
+      p[t][1] = fast_exp2(sc[t][1] - u0);
+      p[t][2] = fast_exp2(sc[t][2] - u1);
+      p[t][3] = fast_exp2(sc[t][3] - u1);
+    }
+    l0 = l0 * f0 + ((p[0][0] + p[0][1]) + (p[1][0] + p[1][1]));
+    l1 = l1 * f1 + ((p[0][2] + p[0][3]) + (p[1][2] + p[1][3]));
+#pragma unroll
+    for (int t = 0; t < D / 8; ++t) {
+      o[t][0] *= f0;
+      o[t][1] *= f0;
+      o[t][2] *= f1;
+      o[t][3] *= f1;
+    }
+    // P is rounded to bf16 for the product, as the tile kernel's is: half a
+    // step of 2^-8 a weight, averaged over the keys
+    const uint32_t a0 = pack_bf16x2(p[0][0], p[0][1]), a1 = pack_bf16x2(p[0][2], p[0][3]);
+    const uint32_t a2 = pack_bf16x2(p[1][0], p[1][1]), a3 = pack_bf16x2(p[1][2], p[1][3]);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const uint32_t sel = (t & 1) ? 0x7632u : 0x5410u;
+        const uint32_t b0 = __byte_perm(word(vw[0][e], t >> 1), word(vw[1][e], t >> 1), sel);
+        const uint32_t b1 = __byte_perm(word(vw[2][e], t >> 1), word(vw[3][e], t >> 1), sel);
+        mma_16816(o[e * 8 + t], a0, a1, a2, a3, b0, b1);
+      }
+  }
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+  // ---- join the warps ----
+  if (c == 0) {
+    sm.m[warp][g] = m0;
+    sm.m[warp][g + 8] = m1;
+    sm.l[warp][g] = l0;
+    sm.l[warp][g + 8] = l1;
+  }
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int d = 64 * e + 16 * c + t;
+      if (g < nr) {
+        sm.o[warp][g][d] = o[e * 8 + t][0];
+        sm.o[warp][g][d + 8] = o[e * 8 + t][1];
+      }
+      if (g + 8 < nr) {
+        sm.o[warp][g + 8][d] = o[e * 8 + t][2];
+        sm.o[warp][g + 8][d + 8] = o[e * 8 + t][3];
+      }
+    }
+  __syncthreads();
+  for (int i = tid; i < nr * D; i += kFewWarps * 32) {
+    const int r = i / D, d = i - r * D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, sm.m[w][r]);
+    const float U = M == -INFINITY ? 0.0f : M;
+    float acc = 0.0f, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float f = fast_exp2(sm.m[w][r] - U);
+      acc = fmaf(f, sm.o[w][r][d], acc);
+      L = fmaf(f, sm.l[w][r], L);
+    }
+    sm.co[r][d] = acc;
+    if (d == 0) {
+      sm.cm[r] = M;
+      sm.cl[r] = L;
+    }
+  }
+  // ---- join the CTAs: each takes its share of the columns ----
+  if (X > 1)
+    cluster_barrier();
+  else
+    __syncthreads();
+  const int cols = D / X;
+  for (int i = tid; i < nr * cols / 2; i += kFewWarps * 32) {
+    const int r = i / (cols / 2), d = rank * cols + (i - r * (cols / 2)) * 2;
+    float M = -INFINITY;
+    for (int x = 0; x < X; ++x) M = fmaxf(M, ld_peer(&sm.cm[r], x));
+    const float U = M == -INFINITY ? 0.0f : M;
+    float y0 = 0.0f, y1 = 0.0f, L = 0.0f;
+    for (int x = 0; x < X; ++x) {
+      const float f = fast_exp2(ld_peer(&sm.cm[r], x) - U);
+      y0 = fmaf(f, ld_peer(&sm.co[r][d], x), y0);
+      y1 = fmaf(f, ld_peer(&sm.co[r][d + 1], x), y1);
+      L = fmaf(f, ld_peer(&sm.cl[r], x), L);
+    }
+    const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
+    uint16_t* dst = a.out + (int64_t(ch) * a.rows_per_chunk + r0 + r) * a.o_rs +
+                    int64_t(h) * a.o_hs + d;
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(y0 * inv, y1 * inv);
+  }
+  if (X > 1) cluster_barrier();  // no CTA leaves while another reads its memory
+}
+
+// ---------------------------------------------------------------------------
+// Attention of 128-row tiles on tcgen05
+// ---------------------------------------------------------------------------
+// One CTA a (segment, group): Q tile, one K and one V buffer of 128 keys (two
+// listed 64-key halves a step), S / P and O in TMEM; two CTAs share an SM, so
+// one's softmax runs while the tensor pipe works for the other.  Warp 0 loads
+// (TMA), warp 1 issues the MMAs, warps 2-5 are the softmax (thread = row).
+//   K(j+1) loads once Q.K(j) has committed (during softmax j), V(j+1) once
+//   P.V(j) has; both have a whole softmax to arrive in, so one buffer of each
+//   suffices and two CTAs fit an SM.
+// The tensor pipe runs a CTA's MMAs in issue order, so Q.K(j+1), which
+// overwrites P(j), follows P.V(j), and S(j+1) seen means O is complete.
+// Rows of V behind a segment's end (or of a half that is not there) are
+// zeroed in shared memory: their weights are 0, but 0 * inf would not be.
+constexpr int kTcThreads = 192;
+constexpr int kMaxHalves = 2 * kMaxTopK;
+
+template <int D>
+struct __align__(1024) SparseTcSmem {
+  uint8_t q[kBM * D * 2];
+  uint8_t k[kBN * D * 2];
+  uint8_t v[kBN * D * 2];
+  uint64_t q_full, k_full, v_full, s_full, p_full, pv_done, drain;
+  uint32_t tmem_base;
+  int abort, halves;
+  int list[kMaxHalves];
+};
+
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 2)
+    sparse_tc_kernel(const __grid_constant__ CUtensorMap tm_q,
+                     const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, SparseArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  SparseTcSmem<D>& sm = *reinterpret_cast<SparseTcSmem<D>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kCols = D / 64;                  // 64-column halves of a row
+  constexpr uint32_t kColBytes = kBM * 64 * 2;   // one of them, 128 rows
+  constexpr uint32_t kHalfKeys = 64 * 64 * 2;    // 64 keys of one of them
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &sm.abort;
+  const int unit = blockIdx.x;
+  const int s = unit / a.groups, grp = unit - s * a.groups;
+  const int ch = s / a.H, h = s - ch * a.H;
+  const int r0 = grp * a.query_block;
+  const int nr = min(a.query_block, a.rows_per_chunk - r0);
+  const SegView sg = segment(a.cu, s, a.kv_rows);
+
+  if (threadIdx.x == 0) {
+    sm.abort = 0;
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.k_full, 1);
+    mbar_init(&sm.v_full, 1);
+    mbar_init(&sm.s_full, 1);
+    mbar_init(&sm.p_full, 4);
+    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {  // the listed 64-key halves that hold keys, in order
+    const int nblk = (sg.len + a.block - 1) / a.block, per = a.block / 64;
+    const int32_t* lst = a.blocks + int64_t(unit) * a.top_k;
+    int n = 0;
+    for (int b = 0; b < a.top_k; b += 32) {
+      const int e = b + lane < a.top_k ? lst[b + lane] : -1;
+      int mine = e >= 0 && e < nblk ? per : 0;
+      if (mine == 2 && int64_t(e) * 128 + 64 >= sg.len) mine = 1;
+      int at = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += y;
+      }
+      const int total = __shfl_sync(0xffffffffu, at, 31);
+      at += n - mine;
+      for (int i = 0; i < mine; ++i) sm.list[at + i] = e * per + i;
+      n += total;
+    }
+    if (lane == 0) sm.halves = n;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     su32(&sm.tmem_base)),
+                 "r"(256));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  const int nh = sm.halves, steps = (nh + 1) >> 1;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0 && steps > 0) {
+      mbar_expect_tx(&sm.q_full, kBM * D * 2);
+      const int row0 = ch * a.rows_per_chunk + r0;
+#pragma unroll
+      for (int x = 0; x < kCols; ++x)
+        tma_load_3d(sm.q + x * kColBytes, &tm_q, &sm.q_full, 64 * x, h, row0);
+      int kj = 0, vj = 0;  // loads issued
+      for (int j = 0; j < steps; ++j) {
+        const int here = 2 * j + 1 < nh ? 2 : 1;
+        const int y0 = sg.start + sm.list[2 * j] * 64;
+        const int y1 = here == 2 ? sg.start + sm.list[2 * j + 1] * 64 : 0;
+        if (j > 0 && !mbar_wait(&sm.s_full, (j - 1) & 1, abort, a.status)) break;
+        mbar_expect_tx(&sm.k_full, here * kHalfKeys * kCols);
+#pragma unroll
+        for (int x = 0; x < kCols; ++x) {
+          tma_load_2d(sm.k + x * kColBytes, &tm_k, &sm.k_full, 64 * x, y0);
+          if (here == 2) tma_load_2d(sm.k + x * kColBytes + kHalfKeys, &tm_k, &sm.k_full, 64 * x, y1);
+        }
+        ++kj;
+        if (j > 0 && !mbar_wait(&sm.pv_done, (j - 1) & 1, abort, a.status)) break;
+        mbar_expect_tx(&sm.v_full, here * kHalfKeys * kCols);
+#pragma unroll
+        for (int x = 0; x < kCols; ++x) {
+          tma_load_2d(sm.v + x * kColBytes, &tm_v, &sm.v_full, 64 * x, y0);
+          if (here == 2) tma_load_2d(sm.v + x * kColBytes + kHalfKeys, &tm_v, &sm.v_full, 64 * x, y1);
+        }
+        ++vj;
+      }
+      if (*abort) {  // this CTA's own copies land before its memory goes away
+        const uint64_t t0 = now_ns();
+        while (!mbar_try(&sm.q_full, 0) && now_ns() - t0 < kTimeoutNs) {
+        }
+        while (kj > 0 && !mbar_try(&sm.k_full, (kj - 1) & 1) && now_ns() - t0 < kTimeoutNs) {
+        }
+        while (vj > 0 && !mbar_try(&sm.v_full, (vj - 1) & 1) && now_ns() - t0 < kTimeoutNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0 && steps > 0) {
+      constexpr uint32_t id_qk = idesc_bf16(false);
+      constexpr uint32_t id_pv =
+          (idesc_bf16(true) & ~(uint32_t(kBN >> 3) << 17)) | (uint32_t(D >> 3) << 17);
+      const uint64_t dq = sdesc_sw128(su32(sm.q), 16, 1024);
+      const uint64_t dk = sdesc_sw128(su32(sm.k), 16, 1024);
+      const uint64_t dv = sdesc_sw128(su32(sm.v), kColBytes, 1024);
+      const uint32_t d_hi = uint32_t(dq >> 32), v_hi = uint32_t(dv >> 32);
+      const uint32_t q_lo = uint32_t(dq), k_lo = uint32_t(dk), v_lo = uint32_t(dv);
+      auto issue_qk = [&]() {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kColBytes + (kk & 3) * 32) >> 4;
+          mma_ss(tmem, (uint64_t(d_hi) << 32) | (q_lo + off), (uint64_t(d_hi) << 32) | (k_lo + off),
+                 id_qk, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&sm.s_full);
+      };
+      bool ok = mbar_wait(&sm.q_full, 0, abort, a.status) &&
+                mbar_wait(&sm.k_full, 0, abort, a.status);
+      if (ok) {
+        tc_fence_after();
+        issue_qk();
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        ok = mbar_wait(&sm.v_full, j & 1, abort, a.status) &&
+             mbar_wait(&sm.p_full, j & 1, abort, a.status);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_ts(tmem + 128, tmem + kk * 8, (uint64_t(v_hi) << 32) | (v_lo + ((kk * 2048) >> 4)),
+                 id_pv, (kk > 0 || j > 0) ? 1u : 0u);
+        tc_commit(&sm.pv_done);
+        if (j + 1 < steps) {
+          ok = mbar_wait(&sm.k_full, (j + 1) & 1, abort, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk();
+        }
+      }
+      // every MMA issued here completes before the CTA frees TMEM
+      tc_commit(&sm.drain);
+      const uint64_t t0 = now_ns();
+      while (!mbar_try(&sm.drain, 0) && now_ns() - t0 < kTimeoutNs) {
+      }
+    }
+  } else {
+    // ---------------- softmax, correction, output ----------------
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_off = uint32_t(quad * 32) << 16;
+    const uint32_t s_tm = tmem + lane_off, o_tm = tmem + 128 + lane_off;
+    const float sc = a.scale_log2;
+    float m_ref = -INFINITY, l_sum = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      const int v0 = min(64, sg.len - sm.list[2 * j] * 64);  // keys of the halves
+      const int v1 = 2 * j + 1 < nh ? min(64, sg.len - sm.list[2 * j + 1] * 64) : 0;
+      const bool partial = v0 < 64 || v1 < 64;
+      if (!mbar_wait(&sm.s_full, j & 1, abort, a.status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld32(s_tm + q * 32, sr[q]);
+      tmem_wait_ld();
+      if (partial) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((q & 1) * 32 + e >= (q < 2 ? v0 : v1)) sr[q][e] = __float_as_uint(-INFINITY);
+        // zero this thread's row of V when it holds no key
+        if (!mbar_wait(&sm.v_full, j & 1, abort, a.status)) {
+          ok = false;
+          break;
+        }
+        if ((row & 63) >= (row < 64 ? v0 : v1)) {
+#pragma unroll
+          for (int x = 0; x < kCols; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(sm.v + x * kColBytes + row * 128 + e * 16) =
+                  make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+      }
+      const float m_new = fmaxf(m_ref, row_max128(sr) * sc);
+      const bool grow = m_new > m_ref + kRescaleThreshold || j == 0;
+      float alpha = 1.0f;
+      if (grow) {
+        alpha = (j == 0 || m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
+        m_ref = m_new;
+      }
+      const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
+      const f2 scale2 = mk2(sc, sc), negm2 = mk2(-m_use, -m_use);
+      f2 acc[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = mk2(0.0f, 0.0f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t pr[16];
+        if (partial)
+          softmax_chunk<false>(sr[q], scale2, negm2, acc[2 * q], acc[2 * q + 1], pr);
+        else
+          softmax_chunk<true>(sr[q], scale2, negm2, acc[2 * q], acc[2 * q + 1], pr);
+        tmem_st16(s_tm + q * 16, pr);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], acc[i + 4]);
+      acc[0] = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
+      float e0, e1;
+      un2(acc[0], e0, e1);
+      l_sum = l_sum * alpha + (e0 + e1);
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t orr[32];
+          tmem_ld32(o_tm + q * 32, orr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * alpha);
+          tmem_st32(o_tm + q * 32, orr);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full);
+    }
+    uint16_t* dst = a.out + (int64_t(ch) * a.rows_per_chunk + r0 + row) * a.o_rs +
+                    int64_t(h) * a.o_hs;
+    if (steps == 0) {
+      if (row < nr)
+        for (int e = 0; e < D; e += 8)
+          *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
+    } else if (ok && mbar_wait(&sm.pv_done, (steps - 1) & 1, abort, a.status)) {
+      tc_fence_after();
+      const float inv = l_sum > 0.0f ? 1.0f / l_sum : (l_sum == 0.0f ? 0.0f : l_sum);
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t orr[32];
+        tmem_ld32(o_tm + q * 32, orr);
+        tmem_wait_ld();
+        if (row < nr) store_row32(dst + q * 32, orr, inv);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+bool shape_ok(int num_chunks, int H, int rows_per_chunk, int query_block, int block, int top_k) {
+  return num_chunks >= 0 && H >= 0 && rows_per_chunk >= 0 && query_block >= 1 &&
+         query_block <= kBM && (block == 64 || block == 128) && top_k >= 1;
+}
+
+template <typename F>
+int opt_in_smem(int (&done)[kMaxDevices], std::mutex& mu, F* fn, size_t bytes) {
+  return per_device_once(done, mu, [fn, bytes] {
+    return cudaFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                int(bytes)) == cudaSuccess
+               ? 1
+               : 0;
+  });
+}
+
+template <int D>
+int launch_few(const SparseArgs& a, int64_t units, cudaStream_t stream) {
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  const size_t smem = sizeof(FewSmem<D>);
+  if (opt_in_smem(done, mu, sparse_few_kernel<D>, smem) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  // the cluster: a warp gets a chunk at least, and the grid stays within a
+  // few CTAs an SM
+  const int chunks = a.top_k * (a.block / 16);
+  int X = 1;
+  while (X < 8 && X * kFewWarps < chunks && units * X < int64_t(sm_count()) * 2) X *= 2;
+  if (units * X >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(units * X));
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = X;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, sparse_few_kernel<D>, a) != cudaSuccess) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  return PKV_OK;
+}
+
+template <int D>
+int launch_tc(const SparseArgs& a, int num_chunks, int64_t units, cudaStream_t stream) {
+  CUtensorMap mq, mk, mv;
+  // (no keys at all: every list is empty and no K/V tile is loaded; the maps
+  // then only have to be well formed)
+  const void* kb = a.kv_rows > 0 ? a.k : a.q;
+  const void* vb = a.kv_rows > 0 ? a.v : a.q;
+  const cuuint64_t kv_dims[2] = {cuuint64_t(D), cuuint64_t(a.kv_rows > 0 ? a.kv_rows : 1)};
+  const cuuint64_t kv_str[1] = {cuuint64_t(D) * 2};
+  const cuuint32_t kv_box[2] = {64, 64};
+  const cuuint64_t q_dims[3] = {cuuint64_t(D), cuuint64_t(a.H),
+                                cuuint64_t(num_chunks) * a.rows_per_chunk};
+  const cuuint64_t q_str[2] = {cuuint64_t(a.q_hs > 0 ? a.q_hs : D) * 2, cuuint64_t(a.q_rs) * 2};
+  const cuuint32_t q_box[3] = {64, 1, kBM};
+  if (!make_map(&mk, kb, 2, kv_dims, kv_str, kv_box) ||
+      !make_map(&mv, vb, 2, kv_dims, kv_str, kv_box) ||
+      !make_map(&mq, a.q, 3, q_dims, q_str, q_box))
+    return PKV_EUNSUPPORTED;
+  // at least 100 KB, so that no third CTA comes to an SM (TMEM holds two)
+  size_t smem = sizeof(SparseTcSmem<D>) + 1024;
+  if (smem < 100 * 1024) smem = 100 * 1024;
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  if (opt_in_smem(done, mu, sparse_tc_kernel<D>, smem) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  sparse_tc_kernel<D><<<int(units), kTcThreads, smem, stream>>>(mq, mk, mv, a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int64_t pkv_block_rows(int64_t kv_rows, int segments, int block) {
+  if (kv_rows < 0 || segments < 0 || (block != 64 && block != 128)) return 0;
+  return kv_rows / block + segments;
+}
+
+extern "C" int pkv_block_means(const uint16_t* k, int64_t kv_rows, int head_dim,
+                               const int32_t* cu_seqlens_k, int segments, int block, float* means,
+                               int64_t means_rows, int zero_rest, pkv_stream_t stream) {
+  if (kv_rows < 0 || segments < 0 || means_rows < 0 || (block != 64 && block != 128))
+    return PKV_EINVAL;
+  if (segments == 0 || means_rows == 0) return PKV_OK;
+  if ((kv_rows > 0 && !k) || !cu_seqlens_k || !means) return PKV_EINVAL;
+  if ((head_dim != 64 && head_dim != 128) || kv_rows >= (int64_t(1) << 31) ||
+      reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(means) % 16)
+    return PKV_EUNSUPPORTED;
+  int64_t grid = (means_rows + 7) / 8;
+  const int64_t cap = int64_t(sm_count()) * 8;
+  if (grid > cap) grid = cap;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128)
+    block_means_kernel<128><<<int(grid), 256, 0, s>>>(k, kv_rows, cu_seqlens_k, segments, block,
+                                                      means, means_rows, zero_rest);
+  else
+    block_means_kernel<64><<<int(grid), 256, 0, s>>>(k, kv_rows, cu_seqlens_k, segments, block,
+                                                     means, means_rows, zero_rest);
+  return launch_status();
+}
+
+extern "C" int pkv_select_blocks(const uint16_t* q, int64_t q_row_stride, int64_t q_head_stride,
+                                 const float* means, int64_t means_rows,
+                                 const int32_t* cu_seqlens_k, int64_t kv_rows, int num_chunks,
+                                 int num_heads, int rows_per_chunk, int head_dim, int query_block,
+                                 int block, int top_k, int32_t* blocks, pkv_stream_t stream) {
+  if (!shape_ok(num_chunks, num_heads, rows_per_chunk, query_block, block, top_k) ||
+      means_rows < 0 || kv_rows < 0)
+    return PKV_EINVAL;
+  if (num_chunks == 0 || num_heads == 0 || rows_per_chunk == 0) return PKV_OK;
+  if (!q || (means_rows > 0 && !means) || !cu_seqlens_k || !blocks) return PKV_EINVAL;
+  if (top_k > kMaxTopK) return PKV_ECAPACITY;
+  if ((head_dim != 64 && head_dim != 128) || reinterpret_cast<uintptr_t>(q) % 16 ||
+      q_row_stride % 8 || q_head_stride % 8 || reinterpret_cast<uintptr_t>(means) % 16)
+    return PKV_EUNSUPPORTED;
+  SelectArgs a{};
+  a.q = q;
+  a.q_rs = q_row_stride;
+  a.q_hs = q_head_stride;
+  a.kv_rows = kv_rows;
+  a.means_rows = means_rows;
+  a.means = means;
+  a.cu = cu_seqlens_k;
+  a.blocks = blocks;
+  a.H = num_heads;
+  a.rows_per_chunk = rows_per_chunk;
+  a.groups = (rows_per_chunk + query_block - 1) / query_block;
+  a.query_block = query_block;
+  a.block = block;
+  a.top_k = top_k;
+  const int64_t grid = int64_t(num_chunks) * num_heads * a.groups;
+  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  auto s = static_cast<cudaStream_t>(stream);
+  const size_t smem = sizeof(SelectSmem);
+  static std::mutex mu;
+  static int done128[kMaxDevices] = {}, done64[kMaxDevices] = {};
+  const int ok = head_dim == 128 ? opt_in_smem(done128, mu, select_blocks_kernel<128>, smem)
+                                 : opt_in_smem(done64, mu, select_blocks_kernel<64>, smem);
+  if (ok <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  if (head_dim == 128)
+    select_blocks_kernel<128><<<int(grid), kSelThreads, smem, s>>>(a);
+  else
+    select_blocks_kernel<64><<<int(grid), kSelThreads, smem, s>>>(a);
+  return launch_status();
+}
+
+extern "C" int pkv_block_attention(const uint16_t* q, int64_t q_row_stride, int64_t q_head_stride,
+                                   const uint16_t* k, const uint16_t* v, int64_t kv_rows,
+                                   const int32_t* cu_seqlens_k, int num_chunks, int num_heads,
+                                   int rows_per_chunk, int head_dim, float softmax_scale,
+                                   const int32_t* blocks, int query_block, int block, int top_k,
+                                   uint16_t* out, int64_t o_row_stride, int64_t o_head_stride,
+                                   int32_t* status, pkv_stream_t stream) {
+  if (!shape_ok(num_chunks, num_heads, rows_per_chunk, query_block, block, top_k) || kv_rows < 0)
+    return PKV_EINVAL;
+  if (num_chunks == 0 || num_heads == 0 || rows_per_chunk == 0) return PKV_OK;
+  if (!q || (kv_rows > 0 && (!k || !v)) || !cu_seqlens_k || !blocks || !out) return PKV_EINVAL;
+  if (!(softmax_scale > 0.0f)) return PKV_EINVAL;
+  if (top_k > kMaxTopK) return PKV_ECAPACITY;
+  const int64_t q_rows = int64_t(num_chunks) * rows_per_chunk;
+  if ((head_dim != 64 && head_dim != 128) || kv_rows >= (int64_t(1) << 31) ||
+      q_rows >= (int64_t(1) << 31) || reinterpret_cast<uintptr_t>(q) % 16 ||
+      reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16 ||
+      reinterpret_cast<uintptr_t>(out) % 16 || q_row_stride % 8 || q_head_stride % 8 ||
+      o_row_stride % 8 || o_head_stride % 8 || q_row_stride <= 0 ||
+      (q_head_stride <= 0 && num_heads > 1))
+    return PKV_EUNSUPPORTED;
+  SparseArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_rs = q_row_stride;
+  a.q_hs = q_head_stride;
+  a.kv_rows = kv_rows;
+  a.o_rs = o_row_stride;
+  a.o_hs = o_head_stride;
+  a.cu = cu_seqlens_k;
+  a.blocks = blocks;
+  a.out = out;
+  a.status = status;
+  a.H = num_heads;
+  a.rows_per_chunk = rows_per_chunk;
+  a.groups = (rows_per_chunk + query_block - 1) / query_block;
+  a.query_block = query_block;
+  a.block = block;
+  a.top_k = top_k;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  const int64_t units = int64_t(num_chunks) * num_heads * a.groups;
+  if (units >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  auto s = static_cast<cudaStream_t>(stream);
+  const int rows = query_block < rows_per_chunk ? query_block : rows_per_chunk;
+  if (rows <= kFewRows)
+    return head_dim == 128 ? launch_few<128>(a, units, s) : launch_few<64>(a, units, s);
+  return head_dim == 128 ? launch_tc<128>(a, num_chunks, units, s)
+                         : launch_tc<64>(a, num_chunks, units, s);
+}

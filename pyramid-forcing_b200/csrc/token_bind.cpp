@@ -1,4 +1,5 @@
-// torch glue of the token-path ops (layer norm, rotary positions): checks the
+// torch glue of the token-path ops (layer norm, rotary positions, block-sparse
+// attention): checks the
 // tensors and calls one extern "C" entry point of libpkv.so on the current
 // CUDA stream.  A fragment of the `adahead` library registered in
 // adahead_bind.cpp.
@@ -196,6 +197,133 @@ std::tuple<Tensor, Tensor> op_rotary(Tensor q, std::optional<Tensor> k, Tensor p
   return {qo, ko};
 }
 
+// ---- block-sparse attention ----------------------------------------------------
+struct SparseCall {
+  Tensor q, k, v, cu;
+  int64_t C, H, R, D, groups;
+};
+
+const uint16_t* u16(const Tensor& t) { return static_cast<const uint16_t*>(ptr(t)); }
+
+// q [C * R, H, D], k / v [rows, D] (or anything that views so), cu int32.
+SparseCall sparse_call(const char* op, const Tensor& q, const Tensor* k, const Tensor* v,
+                       const Tensor& cu, int64_t num_chunks, int64_t rows, int64_t query_block,
+                       int64_t block, int64_t top_k) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16, op,
+              ": q must be a bf16 [num_chunks * rows, H, D] CUDA tensor");
+  SparseCall c;
+  c.C = num_chunks;
+  c.R = rows;
+  c.H = q.size(1);
+  c.D = q.size(2);
+  TORCH_CHECK(num_chunks >= 0 && rows >= 0 && q.size(0) == num_chunks * rows, op,
+              ": q has ", q.size(0), " rows, not ", num_chunks, " x ", rows);
+  TORCH_CHECK(c.D == 64 || c.D == 128, op, ": head size must be 64 or 128");
+  TORCH_CHECK(block == 64 || block == 128, op, ": block must be 64 or 128");
+  TORCH_CHECK(query_block >= 1 && query_block <= 128, op, ": query_block must be 1 to 128");
+  TORCH_CHECK(top_k >= 1 && top_k <= 1024, op, ": top_k must be 1 to 1024");
+  TORCH_CHECK(num_chunks * c.H < (int64_t(1) << 31), op, ": too many segments");
+  TORCH_CHECK(cu.device() == q.device() && cu.scalar_type() == at::kInt && cu.dim() == 1 &&
+                  cu.numel() >= num_chunks * c.H + 1,
+              op, ": cu_seqlens_k must be int32 [num_chunks * H + 1] on q's device");
+  c.cu = cu.contiguous();
+  for (const Tensor* t : {k, v}) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kBFloat16 &&
+                    t->numel() % c.D == 0,
+                op, ": k / v must be bf16 rows of q's head size on its device");
+    Tensor f = t->reshape({t->numel() / c.D, c.D}).contiguous();
+    // a view at an odd offset is copied: rows are read 16 bytes at a time
+    if (reinterpret_cast<uintptr_t>(f.data_ptr()) % 16) f = f.clone();
+    (t == k ? c.k : c.v) = f;
+  }
+  if (v != nullptr) TORCH_CHECK(c.k.size(0) == c.v.size(0), op, ": k and v rows differ");
+  c.q = q;
+  if (c.q.stride(2) != 1 || c.q.stride(0) % 8 || c.q.stride(1) % 8 || c.q.stride(0) <= 0 ||
+      (c.q.stride(1) <= 0 && c.H > 1) || reinterpret_cast<uintptr_t>(c.q.data_ptr()) % 16)
+    c.q = c.q.clone(at::MemoryFormat::Contiguous);
+  c.groups = (rows + query_block - 1) / query_block;
+  return c;
+}
+
+Tensor op_block_means(Tensor k, Tensor cu, int64_t block, bool zero_rest) {
+  const char* op = "pkv_block_means";
+  TORCH_CHECK(k.is_cuda() && k.dim() >= 2 && k.scalar_type() == at::kBFloat16, op,
+              ": k must be a bf16 [rows, D] CUDA tensor");
+  const int64_t D = k.size(-1);
+  TORCH_CHECK(D == 64 || D == 128, op, ": head size must be 64 or 128");
+  TORCH_CHECK(block == 64 || block == 128, op, ": block must be 64 or 128");
+  TORCH_CHECK(cu.device() == k.device() && cu.scalar_type() == at::kInt && cu.dim() == 1 &&
+                  cu.numel() >= 1 && cu.numel() < (int64_t(1) << 31),
+              op, ": cu_seqlens_k must be int32 [segments + 1] on k's device");
+  const c10::cuda::CUDAGuard g(k.device());
+  Tensor kk = k.reshape({k.numel() / D, D}).contiguous();
+  if (reinterpret_cast<uintptr_t>(kk.data_ptr()) % 16) kk = kk.clone();
+  const Tensor cc = cu.contiguous();
+  const int segs = int(cc.numel() - 1);
+  const int64_t rows = pkv_block_rows(kk.size(0), segs, int(block));
+  const Tensor means = at::empty({rows, D}, k.options().dtype(at::kFloat));
+  check_rc(pkv_block_means(u16(kk), kk.size(0), int(D), cc.data_ptr<int32_t>(), segs, int(block),
+                           static_cast<float*>(mut(means)), rows, zero_rest, stream_of(k)),
+           op);
+  return means;
+}
+
+Tensor op_select_blocks(Tensor q, Tensor means, Tensor cu, int64_t kv_rows, int64_t num_chunks,
+                        int64_t rows, int64_t top_k, int64_t query_block, int64_t block) {
+  const char* op = "pkv_select_blocks";
+  const c10::cuda::OptionalCUDAGuard g(q.is_cuda() ? std::optional<c10::Device>(q.device())
+                                                   : std::nullopt);
+  const SparseCall c =
+      sparse_call(op, q, nullptr, nullptr, cu, num_chunks, rows, query_block, block, top_k);
+  TORCH_CHECK(means.device() == q.device() && means.scalar_type() == at::kFloat &&
+                  means.dim() == 2 && means.size(1) == c.D && kv_rows >= 0 &&
+                  means.size(0) >= pkv_block_rows(kv_rows, int(c.C * c.H), int(block)),
+              op, ": means must be the fp32 table pkv_block_means gives for these keys");
+  Tensor mm = means.contiguous();
+  if (reinterpret_cast<uintptr_t>(mm.data_ptr()) % 16) mm = mm.clone();
+  const Tensor blocks = at::empty({c.C * c.H, c.groups, top_k}, c.cu.options());
+  check_rc(pkv_select_blocks(u16(c.q), c.q.stride(0), c.q.stride(1),
+                             static_cast<const float*>(ptr(mm)), mm.size(0),
+                             c.cu.data_ptr<int32_t>(), kv_rows, int(c.C), int(c.H), int(c.R),
+                             int(c.D), int(query_block), int(block), int(top_k),
+                             static_cast<int32_t*>(mut(blocks)), stream_of(q)),
+           op);
+  return blocks;
+}
+
+Tensor op_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu, int64_t num_chunks,
+                          int64_t rows, Tensor blocks, int64_t query_block, int64_t block,
+                          double scale, std::optional<Tensor> status) {
+  const char* op = "pkv_block_attention";
+  TORCH_CHECK(blocks.dim() == 3, op, ": blocks must be [num_chunks * H, groups, top_k]");
+  const c10::cuda::OptionalCUDAGuard g(q.is_cuda() ? std::optional<c10::Device>(q.device())
+                                                   : std::nullopt);
+  const SparseCall c =
+      sparse_call(op, q, &k, &v, cu, num_chunks, rows, query_block, block, blocks.size(2));
+  TORCH_CHECK(blocks.device() == q.device() && blocks.scalar_type() == at::kInt &&
+                  blocks.size(0) == c.C * c.H && blocks.size(1) == c.groups,
+              op, ": blocks must be int32 [", c.C * c.H, ", ", c.groups, ", top_k] on q's device");
+  TORCH_CHECK(scale > 0.0, op, ": softmax_scale must be positive");
+  const Tensor bb = blocks.contiguous();
+  int32_t* st = nullptr;
+  if (status.has_value() && status->defined()) {
+    TORCH_CHECK(status->device() == q.device() && status->scalar_type() == at::kInt &&
+                    status->numel() >= 1,
+                op, ": status must be int32 on q's device");
+    st = status->data_ptr<int32_t>();
+  }
+  const Tensor out = at::empty(q.sizes(), q.options());
+  check_rc(pkv_block_attention(u16(c.q), c.q.stride(0), c.q.stride(1), u16(c.k), u16(c.v),
+                               c.k.size(0), c.cu.data_ptr<int32_t>(), int(c.C), int(c.H),
+                               int(c.R), int(c.D), float(scale),
+                               static_cast<const int32_t*>(ptr(bb)), int(query_block), int(block),
+                               int(blocks.size(2)), static_cast<uint16_t*>(mut(out)),
+                               out.stride(0), out.stride(1), st, stream_of(q)),
+           op);
+  return out;
+}
+
 }  // namespace
 }  // namespace pkv_torch
 
@@ -209,10 +337,19 @@ TORCH_LIBRARY_FRAGMENT(adahead, m) {
         "-> (Tensor, Tensor, Tensor)");
   m.def("pkv_rotary(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, Tensor? axis, "
         "bool half, float scale, bool inverse) -> (Tensor, Tensor)");
+  m.def("pkv_block_means(Tensor k, Tensor cu_seqlens_k, int block, bool zero_rest) -> Tensor");
+  m.def("pkv_select_blocks(Tensor q, Tensor means, Tensor cu_seqlens_k, int kv_rows, "
+        "int num_chunks, int rows_per_chunk, int top_k, int query_block, int block) -> Tensor");
+  m.def("pkv_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_k, int num_chunks, "
+        "int rows_per_chunk, Tensor blocks, int query_block, int block, float softmax_scale, "
+        "Tensor(a!)? status) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
   m.impl("pkv_layer_norm", op_layer_norm);
   m.impl("pkv_layer_norm_backward", op_layer_norm_backward);
   m.impl("pkv_rotary", op_rotary);
+  m.impl("pkv_block_means", op_block_means);
+  m.impl("pkv_select_blocks", op_select_blocks);
+  m.impl("pkv_block_attention", op_block_attention);
 }

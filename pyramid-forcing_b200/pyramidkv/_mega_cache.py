@@ -30,6 +30,7 @@ import torch
 from . import _mega_state_ops
 from . import _mega_state_ref as ref
 from . import _ops
+from . import sparse
 
 _STRATEGY_NAME_TO_KIND = {
     "RecentStrategy": ref.SK_RECENT,
@@ -145,8 +146,13 @@ class MegaCache:
             bool(ctx.has_merge_head))
 
     def attend(self, q: torch.Tensor, current_start: int, *, freqs=None, softmax_scale=None,
-               causal: bool = False, max_seqlen_k=None) -> torch.Tensor:
-        """Attention output [B, L_q, H, D] from the current cache (reference :419-569)."""
+               causal: bool = False, max_seqlen_k=None, top_blocks: int | None = None,
+               query_block: int = 128, key_block: int = 64) -> torch.Tensor:
+        """Attention output [B, L_q, H, D] from the current cache (reference :419-569).
+
+        ``top_blocks`` (not in the reference) attends, for every group of
+        ``query_block`` rows of a frame, only the ``top_blocks`` blocks of
+        ``key_block`` packed keys that score highest (``pyramidkv.sparse``)."""
         ctx = self.ctx
         FSEQ = int(ctx.frame_seqlen)
         B, L_q, H, D = q.shape
@@ -171,7 +177,10 @@ class MegaCache:
                 int(ctx.sink_time_clamp_min), int(ctx.sink_time_clamp_max),
                 int(ctx.decoupled_sink_time_lag), ft, fy, fx)
         ops = _ops.ops()
-        if ctx.on_stage is None:
+        if top_blocks is not None:
+            out = self._attend_sparse(q, args, float(softmax_scale), counter, int(top_blocks),
+                                      int(query_block), int(key_block))
+        elif ctx.on_stage is None:
             out = ops.pkv_attend(ctx.mgr, self.states_bytes_for_layer, int(self.layer_idx), q,
                                  *args, float(softmax_scale), counter)
         else:
@@ -180,6 +189,26 @@ class MegaCache:
             ctx.on_stage("packed")
             out = ops.pkv_attend_attention(ctx.mgr, q, float(softmax_scale))
         return out if out.dtype == q.dtype else out.to(q.dtype)
+
+    def _attend_sparse(self, q, args, scale, counter, top_blocks, query_block, key_block):
+        """Plan + pack as attend, then block-sparse attention over the packed cache."""
+        ctx, mgr, ops = self.ctx, self.ctx.mgr, _ops.ops()
+        _, L_q, H, D = q.shape
+        C = L_q // int(ctx.frame_seqlen)
+        ops.pkv_attend_pack(mgr, self.states_bytes_for_layer, int(self.layer_idx), int(L_q),
+                            *args, counter)
+        if ctx.on_stage is not None:
+            ctx.on_stage("packed")
+        # the rows that C chunks can fill bound the table of block means
+        slots = int(mgr.max_total()) + int(mgr.max_merge_blocks())
+        rows = C * H * slots * max(int(ctx.frame_seqlen), int(mgr.max_merge_tokens_per_anchor()))
+        k = mgr.k_flat_out().view(-1, D)[:rows]
+        v = mgr.v_flat_out().view(-1, D)[:rows]
+        qq = q[0] if q.dtype == torch.bfloat16 else q[0].to(torch.bfloat16)
+        out, _ = sparse.sparse_attention(qq, k, v, mgr.cu_seqlens_k(), C, int(ctx.frame_seqlen),
+                                         top_blocks, query_block=query_block, block=key_block,
+                                         softmax_scale=scale, status=mgr.status_word())
+        return out.view(q.shape)
 
 
 _EMPTY: dict = {}

@@ -97,3 +97,47 @@ def test_rotary_abi_checks(lib):
         assert call(**bad) == EINVAL, bad
     assert call(dim=8192, pairs=2049) == EUNSUPPORTED
     assert call(tokens=0) == 0 and call(qh=0, kh=0) == 0
+
+
+def test_sparse_abi_checks(lib):
+    p = PTR(256)
+    lib.pkv_block_rows.restype = I64
+    assert lib.pkv_block_rows(I64(1000), INT(3), INT(64)) == 18
+    assert lib.pkv_block_rows(I64(1000), INT(3), INT(32)) == 0
+
+    def means(k=p, rows=100, dim=128, cu=p, segs=2, block=64, out=p, n=4):
+        return lib.pkv_block_means(k, I64(rows), INT(dim), cu, INT(segs), INT(block), out, I64(n),
+                                   INT(1), None)
+    for bad in (dict(k=None), dict(rows=-1), dict(cu=None), dict(segs=-1), dict(block=96),
+                dict(out=None), dict(n=-1)):
+        assert means(**bad) == EINVAL, bad
+    for bad in (dict(dim=96), dict(rows=1 << 31), dict(k=PTR(258)), dict(out=PTR(264))):
+        assert means(**bad) == EUNSUPPORTED, bad
+    assert means(segs=0) == 0 and means(n=0) == 0
+
+    def select(q=p, qs=256, mean=p, cu=p, C=1, H=2, R=3, dim=128, gr=128, block=64, top=4, out=p):
+        return lib.pkv_select_blocks(q, I64(qs), I64(128), mean, I64(4), cu, I64(100), INT(C),
+                                     INT(H), INT(R), INT(dim), INT(gr), INT(block), INT(top), out,
+                                     None)
+    for bad in (dict(q=None), dict(mean=None), dict(cu=None), dict(out=None), dict(C=-1),
+                dict(H=-1), dict(R=-1), dict(gr=0), dict(gr=129), dict(block=16), dict(top=0)):
+        assert select(**bad) == EINVAL, bad
+    assert select(top=1025) == 3   # PKV_ECAPACITY
+    for bad in (dict(dim=80), dict(q=PTR(264)), dict(qs=257), dict(mean=PTR(260))):
+        assert select(**bad) == EUNSUPPORTED, bad
+    assert select(R=0) == 0 and select(C=0) == 0
+
+    def attend(q=p, qs=256, hs=128, k=p, v=p, rows=100, R=3, dim=128, scale=0.1, lst=p, gr=128,
+               block=64, top=4, out=p, os_=256):
+        return lib.pkv_block_attention(q, I64(qs), I64(hs), k, v, I64(rows), p, INT(1), INT(2),
+                                       INT(R), INT(dim), FLT(scale), lst, INT(gr), INT(block),
+                                       INT(top), out, I64(os_), I64(128), None, None)
+    for bad in (dict(q=None), dict(k=None), dict(v=None), dict(lst=None), dict(out=None),
+                dict(scale=0.0), dict(scale=float("nan")), dict(rows=-1), dict(gr=0),
+                dict(block=1), dict(top=0)):
+        assert attend(**bad) == EINVAL, bad
+    assert attend(top=1025) == 3
+    for bad in (dict(dim=96), dict(rows=1 << 31), dict(q=PTR(258)), dict(k=PTR(258)),
+                dict(qs=12), dict(hs=0), dict(qs=0), dict(os_=4), dict(out=PTR(264))):
+        assert attend(**bad) == EUNSUPPORTED, bad
+    assert attend(R=0) == 0
