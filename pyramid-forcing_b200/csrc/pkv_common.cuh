@@ -123,6 +123,19 @@ inline int per_device_once(int (&cache)[kMaxDevices], std::mutex& mu, Fn fn) {
   return v;
 }
 
+// Opt a kernel in to `bytes` of dynamic shared memory on the current device;
+// > 0 on success.
+template <typename F>
+inline int smem_opt_in(int (&done)[kMaxDevices], std::mutex& mu, F* fn, size_t bytes) {
+  return per_device_once(done, mu, [fn, bytes] {
+    return cudaFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                int(bytes)) == cudaSuccess
+               ? 1
+               : 0;
+  });
+}
+
 // Streaming multiprocessors of the current device.
 inline int sm_count() {
   static std::mutex mu;

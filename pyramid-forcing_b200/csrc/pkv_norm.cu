@@ -51,48 +51,11 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return s;
 }
 
-// One row per warp (kWarpRow) or per block; V elements a vector, NV vectors
-// a thread in registers.
-template <typename TX, typename TW, int V, int NV, bool kWarpRow>
-__global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(NormArgs a) {
-  __shared__ float red[2][32];
-  const int tpr = kWarpRow ? 32 : blockDim.x;
-  const int tid = kWarpRow ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t row = kWarpRow ? blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5)
-                               : int64_t(blockIdx.x);
-  if (row >= a.rows) return;  // whole warps (kWarpRow) or whole blocks
-  const int nvec = a.C / V;
-  const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
-  float f[NV][V];
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int j = tid + i * tpr;
-    if (j < nvec) {
-      const Vec<TX, V> t = ld_vec<TX, V>(x + j * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e) s += f[i][e] = to_f32(t.v[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
-    }
-  }
-  const float inv_c = 1.0f / float(a.C);
-  const float mu = (kWarpRow ? warp_sum(s) : block_sum(s, red[0])) * inv_c;
-  float q = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (tid + i * tpr < nvec)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        f[i][e] -= mu;
-        q = fmaf(f[i][e], f[i][e], q);
-      }
-  const float rstd = rsqrtf((kWarpRow ? warp_sum(q) : block_sum(q, red[1])) * inv_c + a.eps);
-  if (tid == 0) {
-    if (a.mean) a.mean[row] = mu;
-    if (a.rstd) a.rstd[row] = rstd;
-  }
+// What a thread does with its vectors of a row once they are in f: centre,
+// normalise, modulate, round, store.
+template <typename TX, typename TW, int V, int NV>
+__device__ __forceinline__ void norm_store(const NormArgs& a, int64_t row, int tid, int tpr,
+                                           int nvec, const float (&f)[NV][V], float rstd) {
   const int64_t g = row / a.rows_per_group;
   const TW* w = a.w ? static_cast<const TW*>(a.w) + g * a.C : nullptr;
   const TW* b = a.b ? static_cast<const TW*>(a.b) + g * a.C : nullptr;
@@ -101,10 +64,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(NormArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int j = tid + i * tpr;
     if (j < nvec) {
-      float r[V];
+      float r[V], t2[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) r[e] = f[i][e] * rstd;
-      float t2[V];
       if (w) {
         ld_f32<TW, V>(w + j * V, t2);
 #pragma unroll
@@ -120,6 +82,115 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(NormArgs a) {
       for (int e = 0; e < V; ++e) t.v[e] = from_f32<TX>(r[e]);
       st_vec<TX, V>(y + j * V, t);
     }
+  }
+}
+
+// A block a row: V elements a vector, NV vectors a thread in registers.
+template <typename TX, typename TW, int V, int NV>
+__global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
+  __shared__ float red[2][32];
+  const int tid = threadIdx.x, tpr = blockDim.x;
+  const int64_t row = blockIdx.x;
+  const int nvec = a.C / V;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
+  float f[NV][V];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = tid + i * tpr;
+    if (j < nvec) {
+      const Vec<TX, V> t = ld_vec<TX, V>(x + j * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[i][e] = to_f32(t.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += f[i][e];
+  const float inv_c = 1.0f / float(a.C);
+  const float mu = block_sum(s, red[0]) * inv_c;
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (tid + i * tpr < nvec)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[i][e] -= mu;
+        q = fmaf(f[i][e], f[i][e], q);
+      }
+  const float rstd = rsqrtf(block_sum(q, red[1]) * inv_c + a.eps);
+  if (tid == 0) {
+    if (a.mean) a.mean[row] = mu;
+    if (a.rstd) a.rstd[row] = rstd;
+  }
+  norm_store<TX, TW, V, NV>(a, row, tid, tpr, nvec, f, rstd);
+}
+
+// A warp a row, many rows a warp: the next kStages - 1 rows are on their way
+// into shared memory while one is in registers, so HBM stays busy through the
+// reductions.  Each lane copies exactly what it will read: no barriers.
+constexpr int kFwdStages = 4;
+
+template <typename TX, typename TW, int V, int NV>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_stream_kernel(NormArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Vec<TX, V>* ring = reinterpret_cast<Vec<TX, V>*>(raw) + warp * (kFwdStages * NV * 32) + lane;
+  const int64_t step = int64_t(gridDim.x) * (kNormThreads / 32);
+  const int64_t first = blockIdx.x * int64_t(kNormThreads / 32) + warp;
+  const int nvec = a.C / V;
+  const float inv_c = 1.0f / float(a.C);
+  auto fetch = [&](int64_t row, int st) {
+    if (row < a.rows) {
+      const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = lane + i * 32;
+        if (j < nvec) cp_async<TX, V>(ring + (st * NV + i) * 32, x + j * V);
+      }
+    }
+    cp_commit();  // an empty group counts too
+  };
+  for (int i = 0; i < kFwdStages - 1; ++i) fetch(first + i * step, i);
+  int st = 0;
+  for (int64_t row = first; row < a.rows; row += step) {
+    cp_wait<kFwdStages - 2>();
+    float f[NV][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (lane + i * 32 < nvec) {
+        const Vec<TX, V> t = ring[(st * NV + i) * 32];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += f[i][e] = to_f32(t.v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
+      }
+    }
+    // the slot read one row ago is free: its values are in registers
+    fetch(row + (kFwdStages - 1) * step, st == 0 ? kFwdStages - 1 : st - 1);
+    st = st + 1 == kFwdStages ? 0 : st + 1;
+    const float mu = warp_sum(s) * inv_c;
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + i * 32 < nvec)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          f[i][e] -= mu;
+          q = fmaf(f[i][e], f[i][e], q);
+        }
+    const float rstd = rsqrtf(warp_sum(q) * inv_c + a.eps);
+    if (lane == 0) {
+      if (a.mean) a.mean[row] = mu;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    norm_store<TX, TW, V, NV>(a, row, lane, 32, nvec, f, rstd);
   }
 }
 
@@ -168,13 +239,24 @@ struct NormBwdArgs {
   float plus;
 };
 
-constexpr int kBwdRows = 2;  // rows of one reduction round
+// Rows of one reduction round, and rounds of x and dy on their way into
+// shared memory.
+__host__ __device__ constexpr int bwd_stages(int stage_bytes) { return stage_bytes < 128 ? 4 : 3; }
+__host__ __device__ constexpr int bwd_rows(int elems) { return elems <= 8 ? 2 : 1; }
 
-// CTA (group, part): its rows, every column.
-template <typename TX, typename TW, int V, int NV>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(NormBwdArgs a) {
-  __shared__ float red[2][2 * kBwdRows][8];
+// CTA (group, part): its rows, every column; V * NV columns a thread.
+// 16-bit single elements (V = 1) are too small for asynchronous copies and
+// are loaded directly.
+template <typename TX, typename TW, int V, int NV, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads <= 256 && V * NV <= 8 ? 3 : 1)
+    norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int R = bwd_rows(V * NV);
+  constexpr bool kRing = V * sizeof(TX) >= 4;
+  constexpr int kStages = bwd_stages(R * 2 * NV * V * sizeof(TX));
+  __shared__ float red[2][2 * R][kThreads / 32];
+  extern __shared__ __align__(16) uint8_t raw[];
   const int tid = threadIdx.x, nthr = blockDim.x, nw = nthr >> 5;
+  Vec<TX, V>* ring = reinterpret_cast<Vec<TX, V>*>(raw) + tid;  // [stage][row][x, dy][NV][nthr]
   const int64_t grp = blockIdx.x / a.parts;
   const int p = int(blockIdx.x - grp * a.parts);
   const int64_t r0 = grp * a.rows_per_group + a.rows_per_group * p / a.parts;
@@ -182,6 +264,28 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(NormBwdArgs a) {
   const int nvec = a.C / V;
   const float inv_c = 1.0f / float(a.C);
   const TW* wp = a.w ? static_cast<const TW*>(a.w) + grp * a.C : nullptr;
+  auto fetch = [&](int64_t r, int st) {
+    if constexpr (kRing) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (r + k < r1) {
+          const TX* x = static_cast<const TX*>(a.x) + (r + k) * a.x_rs;
+          const TX* d = static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int j = tid + i * nthr;
+            if (j < nvec) {
+              Vec<TX, V>* slot = ring + int64_t(((st * R + k) * 2) * NV + i) * nthr;
+              cp_async<TX, V>(slot, x + j * V);
+              cp_async<TX, V>(slot + NV * nthr, d + j * V);
+            }
+          }
+        }
+      }
+      cp_commit();
+    }
+  };
+  for (int i = 0; i < kStages - 1; ++i) fetch(r0 + i * R, i);
   float w[NV][V], aw[NV][V], ab[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -194,64 +298,71 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(NormBwdArgs a) {
       aw[i][e] = ab[i][e] = 0.0f;
     }
   }
-  int round = 0;
-  for (int64_t r = r0; r < r1; r += kBwdRows, ++round) {
-    Vec<TX, V> vx[kBwdRows][NV], vd[kBwdRows][NV];
-    float mu[kBwdRows], rs[kBwdRows], c1[kBwdRows], c2[kBwdRows];
+  int round = 0, st = 0;
+  for (int64_t r = r0; r < r1; r += R, ++round) {
+    Vec<TX, V> vx[R][NV], vd[R][NV];
+    float mu[R], rs[R], c1[R], c2[R];
 #pragma unroll
-    for (int k = 0; k < kBwdRows; ++k) {
+    for (int k = 0; k < R; ++k) {
+      mu[k] = r + k < r1 ? a.mean[r + k] : 0.0f;
+      rs[k] = r + k < r1 ? a.rstd[r + k] : 0.0f;
+    }
+    if constexpr (kRing) cp_wait<kStages - 2>();
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
       const bool live = r + k < r1;
-      const TX* x = static_cast<const TX*>(a.x) + (r + k) * a.x_rs;
-      const TX* d = static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs;
-      mu[k] = live ? a.mean[r + k] : 0.0f;
-      rs[k] = live ? a.rstd[r + k] : 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int j = tid + i * nthr;
         if (live && j < nvec) {
-          vx[k][i] = ld_vec<TX, V>(x + j * V);
-          vd[k][i] = ld_vec<TX, V>(d + j * V);
+          if constexpr (kRing) {
+            const Vec<TX, V>* slot = ring + int64_t(((st * R + k) * 2) * NV + i) * nthr;
+            vx[k][i] = slot[0];
+            vd[k][i] = slot[NV * nthr];
+          } else {
+            vx[k][i] = ld_vec<TX, V>(static_cast<const TX*>(a.x) + (r + k) * a.x_rs + j * V);
+            vd[k][i] = ld_vec<TX, V>(static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs + j * V);
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            vx[k][i].v[e] = from_f32<TX>(0.0f);
-            vd[k][i].v[e] = from_f32<TX>(0.0f);
-          }
+          for (int e = 0; e < V; ++e) vx[k][i].v[e] = vd[k][i].v[e] = from_f32<TX>(0.0f);
         }
       }
     }
+    // the slot read one round ago is free: its values were in registers
+    fetch(r + int64_t(kStages - 1) * R, st == 0 ? kStages - 1 : st - 1);
+    st = st + 1 == kStages ? 0 : st + 1;
 #pragma unroll
-    for (int k = 0; k < kBwdRows; ++k) {
+    for (int k = 0; k < R; ++k) {
       c1[k] = c2[k] = 0.0f;
-      const bool live = r + k < r1;
+      // (columns and rows that are not there have dy = 0, and mean and rstd 0)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (live && tid + i * nthr < nvec)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float d = to_f32(vd[k][i].v[e]);
-            const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
-            const float g = d * w[i][e];
-            c1[k] += g;
-            c2[k] = fmaf(g, xh, c2[k]);
-            aw[i][e] = fmaf(d, xh, aw[i][e]);
-            ab[i][e] += d;
-          }
+        for (int e = 0; e < V; ++e) {
+          const float d = to_f32(vd[k][i].v[e]);
+          const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
+          const float g = d * w[i][e];
+          c1[k] += g;
+          c2[k] = fmaf(g, xh, c2[k]);
+          aw[i][e] = fmaf(d, xh, aw[i][e]);
+          ab[i][e] += d;
+        }
       c1[k] = warp_sum(c1[k]);
       c2[k] = warp_sum(c2[k]);
     }
     // two buffers in turn: a warp may write the next round's while another
     // still reads this one's
-    float(*buf)[8] = red[round & 1];
+    auto& buf = red[round & 1];
     if ((tid & 31) == 0)
 #pragma unroll
-      for (int k = 0; k < kBwdRows; ++k) {
+      for (int k = 0; k < R; ++k) {
         buf[2 * k][tid >> 5] = c1[k];
         buf[2 * k + 1][tid >> 5] = c2[k];
       }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kBwdRows; ++k) {
+    for (int k = 0; k < R; ++k) {
       c1[k] = c2[k] = 0.0f;
       for (int i = 0; i < nw; ++i) {
         c1[k] += buf[2 * k][i];
@@ -262,7 +373,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(NormBwdArgs a) {
     }
     if (a.dx != nullptr) {
 #pragma unroll
-      for (int k = 0; k < kBwdRows; ++k) {
+      for (int k = 0; k < R; ++k) {
         if (r + k >= r1) break;
         TX* dx = static_cast<TX*>(a.dx) + (r + k) * a.dx_rs;
 #pragma unroll
@@ -370,49 +481,79 @@ __global__ void __launch_bounds__(256)
   if (db) db[grp * C + c] = from_f32<TW>(sb);
 }
 
-// Parts of a group in the backward pass: about two CTAs an SM over all
-// groups, at least kBwdRows rows each.
+// Parts of a group in the backward pass: about three CTAs an SM over all
+// groups, at least two rows each.
 int64_t bwd_parts(int64_t rows_per_group, int64_t groups) {
-  const int64_t want = (int64_t(sm_count()) * 2 + groups - 1) / groups;
-  const int64_t most = (rows_per_group + kBwdRows - 1) / kBwdRows;
+  const int64_t want = (int64_t(sm_count()) * 3 + groups - 1) / groups;
+  const int64_t most = (rows_per_group + 1) / 2;
   const int64_t p = want < most ? want : most;
   return p < 1 ? 1 : p;
 }
 
 constexpr int round_warp(int n) { return (n + 31) / 32 * 32; }
 
+template <typename TX, typename TW, int V, int NV>
+int stream_fwd(const NormArgs& a, cudaStream_t s) {
+  constexpr size_t smem = size_t(kNormThreads) * kFwdStages * NV * V * sizeof(TX);
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  if (smem_opt_in(done, mu, norm_stream_kernel<TX, TW, V, NV>, smem) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  const int64_t need = (a.rows + kNormThreads / 32 - 1) / (kNormThreads / 32);
+  const int64_t most = int64_t(sm_count()) * 2;
+  norm_stream_kernel<TX, TW, V, NV>
+      <<<int(need < most ? need : most), kNormThreads, smem, s>>>(a);
+  return launch_status();
+}
+
 template <typename TX, typename TW, int V>
 int launch_fwd(const NormArgs& a, cudaStream_t s) {
   const int nvec = a.C / V;
-  // a warp a row while its lanes hold the row (V * 6 elements each) and the
-  // rows fill the GPU; else a block a row
-  if (nvec <= 32 * 6 && a.rows >= int64_t(sm_count()) * 4) {
-    const int per = kNormThreads / 32;
-    const int64_t grid = (a.rows + per - 1) / per;
-    if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
-    if (nvec <= 32)
-      norm_fwd_kernel<TX, TW, V, 1, true><<<int(grid), kNormThreads, 0, s>>>(a);
-    else if (nvec <= 64)
-      norm_fwd_kernel<TX, TW, V, 2, true><<<int(grid), kNormThreads, 0, s>>>(a);
-    else if (nvec <= 128)
-      norm_fwd_kernel<TX, TW, V, 4, true><<<int(grid), kNormThreads, 0, s>>>(a);
-    else
-      norm_fwd_kernel<TX, TW, V, 6, true><<<int(grid), kNormThreads, 0, s>>>(a);
-    return launch_status();
+  if constexpr (V * sizeof(TX) >= 4) {
+    // rows for two warps of every scheduler and a row that fits a warp's
+    // registers: stream
+    if (nvec <= 32 * 8 && a.rows >= int64_t(sm_count()) * 16) {
+      if (nvec <= 32) return stream_fwd<TX, TW, V, 1>(a, s);
+      if (nvec <= 64) return stream_fwd<TX, TW, V, 2>(a, s);
+      if (nvec <= 128) return stream_fwd<TX, TW, V, 4>(a, s);
+      if (nvec <= 192) return stream_fwd<TX, TW, V, 6>(a, s);
+      return stream_fwd<TX, TW, V, 8>(a, s);
+    }
   }
   if (a.rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   const int grid = int(a.rows);
-  const int thr = nvec < kNormThreads ? round_warp(nvec) : kNormThreads;
-  if (nvec <= kNormThreads)
-    norm_fwd_kernel<TX, TW, V, 1, false><<<grid, thr, 0, s>>>(a);
-  else if (nvec <= 2 * kNormThreads)
-    norm_fwd_kernel<TX, TW, V, 2, false><<<grid, thr, 0, s>>>(a);
-  else if (nvec <= 4 * kNormThreads)
-    norm_fwd_kernel<TX, TW, V, 4, false><<<grid, thr, 0, s>>>(a);
-  else if (nvec <= 8 * kNormThreads)
-    norm_fwd_kernel<TX, TW, V, 8, false><<<grid, thr, 0, s>>>(a);
+  auto threads = [nvec](int nv) { return round_warp((nvec + nv - 1) / nv); };
+  // about 256 threads a row; up to 1024 where the row is longer than NV = 8
+  // vectors (or 16 elements) a thread
+  constexpr int kMost = V >= 8 ? 2 : V >= 4 ? 4 : 8;
+  if (nvec <= 256)
+    norm_fwd_kernel<TX, TW, V, 1><<<grid, threads(1), 0, s>>>(a);
+  else if (nvec <= 512)
+    norm_fwd_kernel<TX, TW, V, 2><<<grid, threads(2), 0, s>>>(a);
+  else if (kMost >= 4 && nvec <= 1024)
+    norm_fwd_kernel<TX, TW, V, kMost >= 4 ? 4 : 2><<<grid, threads(4), 0, s>>>(a);
+  else if (nvec <= 1024 * kMost)
+    norm_fwd_kernel<TX, TW, V, kMost><<<grid, threads(kMost), 0, s>>>(a);
   else
     norm_fwd_long_kernel<TX, TW><<<grid, 1024, 0, s>>>(a);
+  return launch_status();
+}
+
+template <typename TX, typename TW, int V, int NV, int kThreads>
+int row_bwd(const NormBwdArgs& a, int64_t grid, cudaStream_t s) {
+  const int thr = round_warp((a.C / V + NV - 1) / NV);
+  constexpr size_t stage = size_t(bwd_rows(V * NV)) * 2 * NV * V * sizeof(TX);
+  constexpr size_t per = V * sizeof(TX) >= 4 ? bwd_stages(stage) * stage : 0;
+  static_assert(per * kThreads <= 200 * 1024, "the rounds of a block fit its shared memory");
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  if (smem_opt_in(done, mu, norm_bwd_kernel<TX, TW, V, NV, kThreads>, per * kThreads) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  norm_bwd_kernel<TX, TW, V, NV, kThreads><<<int(grid), thr, per * thr, s>>>(a);
   return launch_status();
 }
 
@@ -420,41 +561,56 @@ template <typename TX, typename TW, int V>
 int launch_bwd(const NormBwdArgs& a, int64_t groups, cudaStream_t s) {
   const int nvec = a.C / V;
   const int64_t grid = groups * a.parts;
-  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
-  const int thr = nvec < kNormThreads ? round_warp(nvec) : kNormThreads;
-  if (nvec <= kNormThreads)
-    norm_bwd_kernel<TX, TW, V, 1><<<int(grid), thr, 0, s>>>(a);
-  else if (nvec <= 2 * kNormThreads)
-    norm_bwd_kernel<TX, TW, V, 2><<<int(grid), thr, 0, s>>>(a);
-  else if (nvec <= 4 * kNormThreads)
-    norm_bwd_kernel<TX, TW, V, 4><<<int(grid), thr, 0, s>>>(a);
-  else {
-    const int64_t rows = groups * a.rows_per_group;
-    if (rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
-    if (a.dx) norm_bwd_long_kernel<TX, TW><<<int(rows), 1024, 0, s>>>(a);
-    const dim3 cols(unsigned(grid), unsigned((a.C + kNormThreads - 1) / kNormThreads));
-    if (a.part) norm_cols_kernel<TX><<<cols, kNormThreads, 0, s>>>(a);
+  const int64_t rows = groups * a.rows_per_group;
+  if (grid >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  if (nvec <= 256) return row_bwd<TX, TW, V, 1, 256>(a, grid, s);
+  if (nvec <= 512) return row_bwd<TX, TW, V, 2, 256>(a, grid, s);
+  if constexpr (V >= 8) {
+    if (nvec <= 1024) return row_bwd<TX, TW, V, 2, 512>(a, grid, s);
+  } else {
+    if (nvec <= 1024) return row_bwd<TX, TW, V, 4, 256>(a, grid, s);
+    if constexpr (V >= 4) {
+      if (nvec <= 2048) return row_bwd<TX, TW, V, 4, 512>(a, grid, s);
+    } else {
+      if (nvec <= 4096) return row_bwd<TX, TW, V, 8, 512>(a, grid, s);
+      if constexpr (V == 1)
+        if (nvec <= 8192) return row_bwd<TX, TW, V, 16, 512>(a, grid, s);
+    }
   }
+  if (a.dx) norm_bwd_long_kernel<TX, TW><<<int(rows), 1024, 0, s>>>(a);
+  const dim3 cols(unsigned(grid), unsigned((a.C + kNormThreads - 1) / kNormThreads));
+  if (a.part) norm_cols_kernel<TX><<<cols, kNormThreads, 0, s>>>(a);
   return launch_status();
 }
 
+// Access width: 16 bytes, 4 bytes (16-bit types with even rows), one element.
 template <typename TX, typename TW>
 int run_fwd(const NormArgs& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(TX);
-  if (a.C % V == 0 && vec_ok(a.x, a.x_rs, V, sizeof(TX)) &&
-      vec_ok(a.y, a.y_rs, V, sizeof(TX)) && vec_ok(a.w, 0, 16, 1) && vec_ok(a.b, 0, 16, 1))
-    return launch_fwd<TX, TW, V>(a, s);
+  auto fits = [&a](int v) {
+    const int sx = sizeof(TX), sw = int(sizeof(TW)) * v < 16 ? int(sizeof(TW)) * v : 16;
+    return a.C % v == 0 && vec_ok(a.x, a.x_rs, v, sx) && vec_ok(a.y, a.y_rs, v, sx) &&
+           vec_ok(a.w, 0, sw, 1) && vec_ok(a.b, 0, sw, 1);
+  };
+  if (fits(V)) return launch_fwd<TX, TW, V>(a, s);
+  if constexpr (sizeof(TX) == 2)
+    if (fits(2)) return launch_fwd<TX, TW, 2>(a, s);
   return launch_fwd<TX, TW, 1>(a, s);
 }
 
 template <typename TX, typename TW>
 int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream_t s) {
   constexpr int V = 16 / sizeof(TX);
-  int rc;
-  if (a.C % V == 0 && vec_ok(a.x, a.x_rs, V, sizeof(TX)) &&
-      vec_ok(a.dy, a.dy_rs, V, sizeof(TX)) && vec_ok(a.dx, a.dx_rs, V, sizeof(TX)) &&
-      vec_ok(a.w, 0, 16, 1))
+  auto fits = [&a](int v) {
+    const int sx = sizeof(TX), sw = int(sizeof(TW)) * v < 16 ? int(sizeof(TW)) * v : 16;
+    return a.C % v == 0 && vec_ok(a.x, a.x_rs, v, sx) && vec_ok(a.dy, a.dy_rs, v, sx) &&
+           vec_ok(a.dx, a.dx_rs, v, sx) && vec_ok(a.w, 0, sw, 1);
+  };
+  int rc = PKV_OK;
+  if (fits(V))
     rc = launch_bwd<TX, TW, V>(a, groups, s);
+  else if (sizeof(TX) == 2 && fits(2))
+    rc = launch_bwd<TX, TW, sizeof(TX) == 2 ? 2 : 1>(a, groups, s);
   else
     rc = launch_bwd<TX, TW, 1>(a, groups, s);
   if (rc != PKV_OK || a.part == nullptr) return rc;

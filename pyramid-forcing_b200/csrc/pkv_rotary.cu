@@ -33,8 +33,25 @@ struct RotSide {
   int heads;
 };
 
+constexpr int kUnroll = 4;
+
+// n / d for n < 2^31 by a multiplication (d >= 1): with s = ceil(log2 d) and
+// mul = ceil(2^(31 + s) / d) the product's error stays below 1 / d.
+struct Div {
+  uint32_t mul, shift;
+  explicit Div(uint32_t d = 1) {
+    shift = 0;
+    while ((uint64_t(1) << shift) < d) ++shift;
+    mul = uint32_t(((uint64_t(1) << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return uint32_t((uint64_t(n) * mul) >> (31 + shift));
+  }
+};
+
 struct RotArgs {
   RotSide s[2];
+  Div by_heads, by_turn, by_rest;
   int64_t tokens;
   const int64_t* pos;
   const double* inv_freq;
@@ -61,59 +78,98 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
     tab[i] = make_float2(fmaf(-lo, s, c) * a.scale, fmaf(lo, c, s) * a.scale * a.sign);
   }
   __syncthreads();
-  const int turn = a.P / V;                 // units of V pairs of a head
-  const int units = turn + (a.D - 2 * a.P) / V;  // and of V copied elements
+  // turned units of V pairs, kUnroll at a time: their loads are on their way
+  // together
   const int h0 = a.s[0].heads, heads = h0 + a.s[1].heads;
-  const int n = nt * heads * units;
-  for (int i = threadIdx.x; i < n; i += kRotThreads) {
-    const int u = i % units, th = i / units;
-    const int t = th / heads;
-    int h = th - t * heads;
+  auto rows = [&](uint32_t th, const T*& x, T*& o, int& t) {
+    t = int(a.by_heads.div(th));
+    int h = int(th) - t * heads;
     const bool second = h >= h0;
     if (second) h -= h0;
     const RotSide& sd = a.s[second ? 1 : 0];
-    const T* x = static_cast<const T*>(sd.x) + (t0 + t) * sd.x_tok + h * sd.x_head;
-    T* o = static_cast<T*>(sd.out) + (t0 + t) * sd.o_tok + h * sd.o_head;
-    if (u >= turn) {
-      const int e = 2 * a.P + (u - turn) * V;
-      st_vec<T, V>(o + e, ld_vec<T, V>(x + e));
-      continue;
-    }
-    const float2* cs = tab + t * a.P + u * V;
-    const int e0 = a.half ? u * V : 2 * u * V;
-    const int e1 = a.half ? a.P + u * V : 2 * u * V + V;
-    const Vec<T, V> x0 = ld_vec<T, V>(x + e0), x1 = ld_vec<T, V>(x + e1);
-    Vec<T, V> y0, y1;
-    if (a.half) {
+    x = static_cast<const T*>(sd.x) + (t0 + t) * sd.x_tok + h * sd.x_head;
+    o = static_cast<T*>(sd.out) + (t0 + t) * sd.o_tok + h * sd.o_head;
+  };
+  const int turn = a.P / V;
+  const int n = nt * heads * turn;
+  for (int i0 = threadIdx.x; i0 < n; i0 += kRotThreads * kUnroll) {
+    Vec<T, V> x0[kUnroll], x1[kUnroll];
+    T* o[kUnroll];
+    int at[kUnroll], e0[kUnroll];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float p = to_f32(x0.v[j]), q = to_f32(x1.v[j]);
-        const float2 w = cs[j];
-        y0.v[j] = from_f32<T>(p * w.x - q * w.y);
-        y1.v[j] = from_f32<T>(p * w.y + q * w.x);
-      }
-    } else {
-      T in[2 * V], r[2 * V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        in[j] = x0.v[j];
-        in[V + j] = x1.v[j];
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float p = to_f32(in[2 * j]), q = to_f32(in[2 * j + 1]);
-        const float2 w = cs[j];
-        r[2 * j] = from_f32<T>(p * w.x - q * w.y);
-        r[2 * j + 1] = from_f32<T>(p * w.y + q * w.x);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        y0.v[j] = r[j];
-        y1.v[j] = r[V + j];
+    for (int k = 0; k < kUnroll; ++k) {
+      const int i = i0 + k * kRotThreads;
+      if (i < n) {
+        const uint32_t th = a.by_turn.div(i);
+        const int u = i - int(th) * turn;
+        const T* x;
+        int t;
+        rows(th, x, o[k], t);
+        at[k] = t * a.P + u * V;
+        e0[k] = a.half ? u * V : 2 * u * V;
+        x0[k] = ld_vec<T, V>(x + e0[k]);
+        x1[k] = ld_vec<T, V>(x + e0[k] + (a.half ? a.P : V));
       }
     }
-    st_vec<T, V>(o + e0, y0);
-    st_vec<T, V>(o + e1, y1);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      if (i0 + k * kRotThreads >= n) break;
+      const float2* cs = tab + at[k];
+      Vec<T, V> y0, y1;
+      if (a.half) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float p = to_f32(x0[k].v[j]), q = to_f32(x1[k].v[j]);
+          const float2 w = cs[j];
+          y0.v[j] = from_f32<T>(p * w.x - q * w.y);
+          y1.v[j] = from_f32<T>(p * w.y + q * w.x);
+        }
+      } else {
+        T in[2 * V], r[2 * V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          in[j] = x0[k].v[j];
+          in[V + j] = x1[k].v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float p = to_f32(in[2 * j]), q = to_f32(in[2 * j + 1]);
+          const float2 w = cs[j];
+          r[2 * j] = from_f32<T>(p * w.x - q * w.y);
+          r[2 * j + 1] = from_f32<T>(p * w.y + q * w.x);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          y0.v[j] = r[j];
+          y1.v[j] = r[V + j];
+        }
+      }
+      st_vec<T, V>(o[k] + e0[k], y0);
+      st_vec<T, V>(o[k] + e0[k] + (a.half ? a.P : V), y1);
+    }
+  }
+  // copied units of V elements
+  const int rest = (a.D - 2 * a.P) / V;
+  const int m = nt * heads * rest;
+  for (int i0 = threadIdx.x; i0 < m; i0 += kRotThreads * 2 * kUnroll) {
+    Vec<T, V> v[2 * kUnroll];
+    T* o[2 * kUnroll];
+#pragma unroll
+    for (int k = 0; k < 2 * kUnroll; ++k) {
+      const int i = i0 + k * kRotThreads;
+      if (i < m) {
+        const uint32_t th = a.by_rest.div(i);
+        const T* x;
+        int t;
+        rows(th, x, o[k], t);
+        const int e = 2 * a.P + (i - int(th) * rest) * V;
+        o[k] += e;
+        v[k] = ld_vec<T, V>(x + e);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * kUnroll; ++k)
+      if (i0 + k * kRotThreads < m) st_vec<T, V>(o[k], v[k]);
   }
 }
 
@@ -129,19 +185,27 @@ bool rot_fits(const RotArgs& a) {
   return true;
 }
 
+template <typename T, int V>
+void launch_rotary(RotArgs a, int64_t grid, cudaStream_t s) {
+  a.by_heads = Div(uint32_t(a.s[0].heads + a.s[1].heads));
+  if (a.P >= V) a.by_turn = Div(uint32_t(a.P / V));
+  if (a.D - 2 * a.P >= V) a.by_rest = Div(uint32_t((a.D - 2 * a.P) / V));
+  rotary_kernel<T, V><<<int(grid), kRotThreads, 0, s>>>(a);
+}
+
 template <typename T>
 int run_rotary(const RotArgs& a, int64_t grid, cudaStream_t s) {
   // the widest access that divides the pairs, the head, the strides and the
   // addresses
   constexpr int kWide = 16 / sizeof(T);
   if (rot_fits<T, kWide>(a))
-    rotary_kernel<T, kWide><<<int(grid), kRotThreads, 0, s>>>(a);
+    launch_rotary<T, kWide>(a, grid, s);
   else if (kWide > 4 && rot_fits<T, 4>(a))
-    rotary_kernel<T, 4><<<int(grid), kRotThreads, 0, s>>>(a);
+    launch_rotary<T, 4>(a, grid, s);
   else if (rot_fits<T, 2>(a))
-    rotary_kernel<T, 2><<<int(grid), kRotThreads, 0, s>>>(a);
+    launch_rotary<T, 2>(a, grid, s);
   else
-    rotary_kernel<T, 1><<<int(grid), kRotThreads, 0, s>>>(a);
+    launch_rotary<T, 1>(a, grid, s);
   return launch_status();
 }
 

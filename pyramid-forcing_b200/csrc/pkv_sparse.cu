@@ -45,6 +45,10 @@ __device__ __forceinline__ SegView segment(const int32_t* cu, int s, int64_t kv_
   return {int(min(a, kv_rows)), b > a ? int(b - a) : 0};
 }
 
+__device__ __forceinline__ uint32_t word(const uint4& w, int i) {
+  return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+}
+
 // ---------------------------------------------------------------------------
 // Block means
 // ---------------------------------------------------------------------------
@@ -86,28 +90,27 @@ __global__ void __launch_bounds__(256)
     const int n = min(int64_t(block), sg.len - first);
     const uint16_t* p = k + (sg.start + first) * D + d0;
     double acc[8] = {};
-    for (int r = sub; r < n; r += 4 * kKeys) {
-      uint4 w[4];
+    for (int r = sub; r < n; r += 8 * kKeys) {
+      uint4 w[8];  // 8 loads a lane on their way: 4 KB a warp
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 8; ++i)
         w[i] = r + i * kKeys < n
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kKeys) * D))
                    : make_uint4(0, 0, 0, 0);
-      float f[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float lo4[4], hi4[4];
+      for (int i = 0; i < 8; i += 4)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
-          hi4[i] = __uint_as_float(u & 0xffff0000u);
+        for (int e = 0; e < 4; ++e) {
+          float lo4[4], hi4[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t u = word(w[i + x], e);
+            lo4[x] = bf16_bits_to_f32(u & 0xffffu);
+            hi4[x] = __uint_as_float(u & 0xffff0000u);
+          }
+          acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
+          acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
         }
-        f[2 * e] = (lo4[0] + lo4[1]) + (lo4[2] + lo4[3]);
-        f[2 * e + 1] = (hi4[0] + hi4[1]) + (hi4[2] + hi4[3]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += double(f[e]);
     }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1)
@@ -125,11 +128,40 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
+  uint32_t addr;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(su32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Into the first CTA of the cluster.
+__device__ __forceinline__ void st_peer(uint64_t* p, uint64_t v) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(addr) : "r"(su32(p)));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // Selection
 // ---------------------------------------------------------------------------
 constexpr int kSelThreads = 256;
-constexpr int kSelChunk = 2048;  // scores added per round
+constexpr int kSelChunk = 1024;  // scores added per round
+constexpr int kSelCluster = 8;   // most CTAs a group
 
 struct SelectArgs {
   const uint16_t* q;
@@ -141,19 +173,15 @@ struct SelectArgs {
 };
 
 struct SelectSmem {
-  union {
-    double red[kSelThreads / 8][128];  // partial query sums (D = 64: two rows' worth used)
-    struct {
-      uint64_t key[kMaxTopK + kSelChunk];
-      int id[kMaxTopK + kSelChunk];
-    } c;
-  };
+  double red[kSelThreads / 32][128];  // the warps' query sums
   double q[128];
   int hist[256];
   int wsum[2][kSelThreads / 32];
-  uint64_t prefix;
-  uint64_t lo, hi;
+  uint64_t prefix, lo, hi;
   int need, done;
+  // [top_k + kSelChunk] keys, then as many ids: the kept blocks of earlier
+  // rounds, then this round's
+  uint64_t key[1];
 };
 
 // Scores as integers in the same order; NaN below all, -0 as 0.
@@ -164,21 +192,30 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
+// A CTA a group, or a cluster whose CTAs share the scores and whose first
+// picks: with few groups (single tokens) the table of means is then read by
+// many SMs.
 template <int D>
-__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) select_blocks_kernel(SelectArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(raw);
+  uint64_t* skey = sm.key;
+  int* sid = reinterpret_cast<int*>(skey + a.top_k + kSelChunk);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int s = blockIdx.x / a.groups, g = blockIdx.x - s * a.groups;
+  const int X = int(cluster_size()), rank = int(cluster_rank());
+  const int unit = blockIdx.x / X;
+  const int s = unit / a.groups, g = unit - s * a.groups;
   const int c = s / a.H, h = s - c * a.H;
   const SegView sg = segment(a.cu, s, a.kv_rows);
   const int nblk = (sg.len + a.block - 1) / a.block;
-  int32_t* out = a.blocks + (int64_t(s) * a.groups + g) * a.top_k;
-  if (nblk <= a.top_k) {  // every block is kept
-    for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
+  int32_t* out = a.blocks + int64_t(unit) * a.top_k;
+  if (nblk <= a.top_k) {  // every block is kept (the whole cluster leaves)
+    if (rank == 0)
+      for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
     return;
   }
-  // ---- sum of the group's queries, float64 (exact for bf16 of like size) ----
+  // ---- sum of the group's queries, float64 (exact for bf16 of like size;
+  // four rows are added in fp32 first, as block_means_kernel does) ----
   const int r0 = g * a.query_block;
   const int nr = min(a.query_block, a.rows_per_chunk - r0);
   {
@@ -187,72 +224,109 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
     const uint16_t* p =
         a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
     double acc[8] = {};
-    for (int r = sub; r < nr; r += kRows) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p + r * a.q_rs));
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int r = sub; r < nr; r += 4 * kRows) {
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = r + i * kRows < nr
+                   ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs))
+                   : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        acc[2 * e] += double(bf16_bits_to_f32(u[e] & 0xffffu));
-        acc[2 * e + 1] += double(__uint_as_float(u[e] & 0xffff0000u));
+        float lo4[4], hi4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = word(w[i], e);
+          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
+          hi4[i] = __uint_as_float(u & 0xffff0000u);
+        }
+        acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
+        acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
       }
     }
-    double* red = &sm.red[0][0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) red[sub * D + d0 + e] = acc[e];
+    for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+    if (lane < kLanes)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sm.red[warp][d0 + e] = acc[e];
     __syncthreads();
     if (tid < D) {
       double t = 0.0;
-      for (int i = 0; i < min(kRows, nr); ++i) t += red[i * D + tid];
+#pragma unroll
+      for (int i = 0; i < kSelThreads / 32; ++i) t += sm.red[i][tid];
       sm.q[tid] = t;
     }
     __syncthreads();
   }
-  // ---- scores: 8 lanes a block, D / 8 products each ----
-  constexpr int kPer = D / 8;
-  const int l8 = tid & 7;
+  // ---- scores: 16 lanes a block, D / 16 products each; 4 blocks on their way ----
+  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = 4;
+  const int l16 = tid & 15;
   double q[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) q[i] = sm.q[(i / 4) * 32 + l8 * 4 + (i & 3)];
+  for (int i = 0; i < kPer; ++i) q[i] = sm.q[(i / 4) * 64 + l16 * 4 + (i & 3)];
   const int64_t base = int64_t(a.cu[s]) / a.block + s;
+  const int stride = X * (kSelThreads / 16);
   int kept = 0;
+  if (X > 1) cluster_barrier();  // the first CTA runs: its memory may be written
   for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
     const int m = min(kSelChunk, nblk - b0);
     uint64_t mn = ~uint64_t(0), mx = 0;
-    for (int i = tid >> 3; i < (m + 31) / 32 * 32; i += kSelThreads / 8) {
-      double t = 0.0;
-      const int64_t row = base + b0 + i;
-      if (i < m && row >= 0 && row < a.means_rows) {
-        const float* p = a.means + row * D + l8 * 4;
-        float4 f[kPer / 4];
+    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kSelChunk; i0 += stride * kBatch) {
+      if (i0 - (lane >> 4) >= m) break;  // (the whole warp)
+      float4 f[kBatch][kVec];
 #pragma unroll
-        for (int e = 0; e < kPer / 4; ++e) f[e] = __ldg(reinterpret_cast<const float4*>(p + e * 32));
+      for (int x = 0; x < kBatch; ++x) {
+        const int64_t row = base + b0 + i0 + x * stride;
+        const bool ok = i0 + x * stride < m && row >= 0 && row < a.means_rows;
+        const float* p = a.means + row * D + l16 * 4;
 #pragma unroll
-        for (int e = 0; e < kPer / 4; ++e) {
-          t = fma(double(f[e].x), q[4 * e], t);
-          t = fma(double(f[e].y), q[4 * e + 1], t);
-          t = fma(double(f[e].z), q[4 * e + 2], t);
-          t = fma(double(f[e].w), q[4 * e + 3], t);
+        for (int e = 0; e < kVec; ++e)
+          f[x][e] = ok ? __ldg(reinterpret_cast<const float4*>(p + e * 64))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        double t = 0.0;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          t = fma(double(f[x][e].x), q[4 * e], t);
+          t = fma(double(f[x][e].y), q[4 * e + 1], t);
+          t = fma(double(f[x][e].z), q[4 * e + 2], t);
+          t = fma(double(f[x][e].w), q[4 * e + 3], t);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        const int i = i0 + x * stride;
+        if (i < m && l16 == 0) {
+          st_peer(&skey[kept + i], order_key(t));
         }
       }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (i < m && l8 == 0) {
-        const uint64_t key = order_key(t);
-        sm.c.key[kept + i] = key;
-        sm.c.id[kept + i] = b0 + i;
-      }
     }
-    __syncthreads();
+    if (rank == 0)
+      for (int i = tid; i < m; i += kSelThreads) sid[kept + i] = b0 + i;
+    if (X > 1)
+      cluster_barrier();  // every score is in the first CTA's memory
+    else
+      __syncthreads();
     const int total = kept + m;
     const bool last = b0 + m == nblk;
+    if (rank != 0) {
+      if (last) return;
+      kept = min(total, a.top_k);
+      cluster_barrier();  // the first CTA has picked: its memory may be written
+      continue;
+    }
     if (total <= a.top_k) {  // (not the last round: nblk > top_k)
       kept = total;
+      if (X > 1) cluster_barrier();
       continue;
     }
     // ---- the top_k-th key: digits of 8 bits from the highest that differs ----
     for (int i = tid; i < total; i += kSelThreads) {
-      mn = min(mn, sm.c.key[i]);
-      mx = max(mx, sm.c.key[i]);
+      mn = min(mn, skey[i]);
+      mx = max(mx, skey[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -281,7 +355,7 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
       for (int i = tid; i < 256; i += kSelThreads) sm.hist[i] = 0;
       __syncthreads();
       for (int i = tid; i < total; i += kSelThreads) {
-        const uint64_t key = sm.c.key[i];
+        const uint64_t key = skey[i];
         const uint64_t up = shift + bits == 64 ? 0 : key >> (shift + bits);
         if (up == prefix) atomicAdd(&sm.hist[int(key >> shift) & ((1 << bits) - 1)], 1);
       }
@@ -321,8 +395,8 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
     int eq_seen = 0, written = 0;
     for (int t0 = 0; t0 < total; t0 += kSelThreads) {
       const int i = t0 + tid;
-      const uint64_t key = i < total ? sm.c.key[i] : 0;
-      const int id = i < total ? sm.c.id[i] : 0;
+      const uint64_t key = i < total ? skey[i] : 0;
+      const int id = i < total ? sid[i] : 0;
       const uint64_t up = shift == 64 ? 0 : key >> shift;
       const bool gt = i < total && up > prefix, eq = i < total && up == prefix;
       const uint32_t be = __ballot_sync(0xffffffffu, eq);
@@ -347,13 +421,14 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
         if (last)
           out[at] = id;
         else {
-          sm.c.key[at] = key;
-          sm.c.id[at] = id;
+          skey[at] = key;
+          sid[at] = id;
         }
       }
       __syncthreads();
     }
     kept = a.top_k;
+    if (X > 1 && !last) cluster_barrier();
   }
 }
 
@@ -382,31 +457,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t word(const uint4& w, int i) {
-  return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
-  uint32_t addr;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(su32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 
 // Partial results of the warps and of the CTA: unnormalised O, maximum, sum.
@@ -642,6 +692,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 // zeroed in shared memory: their weights are 0, but 0 * inf would not be.
 constexpr int kTcThreads = 192;
 constexpr int kMaxHalves = 2 * kMaxTopK;
+constexpr int kAhead = 2;  // steps whose keys are pulled into L2 ahead of their loads
 
 template <int D>
 struct __align__(1024) SparseTcSmem {
@@ -726,6 +777,18 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
       for (int x = 0; x < kCols; ++x)
         tma_load_3d(sm.q + x * kColBytes, &tm_q, &sm.q_full, 64 * x, h, row0);
+      // keys of the next steps go to L2 while this one's are in use: a list
+      // jumps about, so its loads would each wait for HBM
+      auto pull = [&](int i) {
+        if (i >= nh) return;
+        const int y = sg.start + sm.list[i] * 64;
+#pragma unroll
+        for (int x = 0; x < kCols; ++x) {
+          tma_prefetch_2d(&tm_k, 64 * x, y);
+          tma_prefetch_2d(&tm_v, 64 * x, y);
+        }
+      };
+      for (int i = 0; i < 2 * kAhead; ++i) pull(2 + i);
       int kj = 0, vj = 0;  // loads issued
       for (int j = 0; j < steps; ++j) {
         const int here = 2 * j + 1 < nh ? 2 : 1;
@@ -747,6 +810,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           if (here == 2) tma_load_2d(sm.v + x * kColBytes + kHalfKeys, &tm_v, &sm.v_full, 64 * x, y1);
         }
         ++vj;
+        pull(2 * (j + 1 + kAhead));
+        pull(2 * (j + 1 + kAhead) + 1);
       }
       if (*abort) {  // this CTA's own copies land before its memory goes away
         const uint64_t t0 = now_ns();
@@ -927,15 +992,45 @@ bool shape_ok(int num_chunks, int H, int rows_per_chunk, int query_block, int bl
          query_block <= kBM && (block == 64 || block == 128) && top_k >= 1;
 }
 
-template <typename F>
-int opt_in_smem(int (&done)[kMaxDevices], std::mutex& mu, F* fn, size_t bytes) {
-  return per_device_once(done, mu, [fn, bytes] {
-    return cudaFuncSetAttribute(reinterpret_cast<const void*>(fn),
-                                cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(bytes)) == cudaSuccess
-               ? 1
-               : 0;
-  });
+// One-dimensional grid in clusters of X.
+template <typename A>
+int launch_cluster(void (*kernel)(A), const A& a, int64_t units, int X, int threads, size_t smem,
+                   cudaStream_t stream) {
+  if (units * X >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(units * X));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = unsigned(X);
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  return PKV_OK;
+}
+
+template <int D>
+int launch_select(const SelectArgs& a, int64_t units, cudaStream_t stream) {
+  const size_t most = sizeof(SelectSmem) + size_t(kMaxTopK + kSelChunk) * 12;
+  const size_t smem = sizeof(SelectSmem) + size_t(a.top_k + kSelChunk) * 12;
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  if (smem_opt_in(done, mu, select_blocks_kernel<D>, most) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  // a cluster while the groups leave SMs idle and the keys could make blocks
+  // enough to share (16 a round and CTA)
+  int X = 1;
+  const int64_t blocks = a.kv_rows / a.block;
+  while (X < kSelCluster && units * X * 2 <= sm_count() && blocks >= int64_t(X) * 64) X *= 2;
+  return launch_cluster(select_blocks_kernel<D>, a, units, X, kSelThreads, smem, stream);
 }
 
 template <int D>
@@ -943,7 +1038,7 @@ int launch_few(const SparseArgs& a, int64_t units, cudaStream_t stream) {
   static std::mutex mu;
   static int done[kMaxDevices] = {};
   const size_t smem = sizeof(FewSmem<D>);
-  if (opt_in_smem(done, mu, sparse_few_kernel<D>, smem) <= 0) {
+  if (smem_opt_in(done, mu, sparse_few_kernel<D>, smem) <= 0) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
@@ -952,23 +1047,7 @@ int launch_few(const SparseArgs& a, int64_t units, cudaStream_t stream) {
   const int chunks = a.top_k * (a.block / 16);
   int X = 1;
   while (X < 8 && X * kFewWarps < chunks && units * X < int64_t(sm_count()) * 2) X *= 2;
-  if (units * X >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(units * X));
-  cfg.blockDim = dim3(kFewWarps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = X;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, sparse_few_kernel<D>, a) != cudaSuccess) {
-    cudaGetLastError();
-    return PKV_ELAUNCH;
-  }
-  return PKV_OK;
+  return launch_cluster(sparse_few_kernel<D>, a, units, X, kFewWarps * 32, smem, stream);
 }
 
 template <int D>
@@ -994,7 +1073,7 @@ int launch_tc(const SparseArgs& a, int num_chunks, int64_t units, cudaStream_t s
   if (smem < 100 * 1024) smem = 100 * 1024;
   static std::mutex mu;
   static int done[kMaxDevices] = {};
-  if (opt_in_smem(done, mu, sparse_tc_kernel<D>, smem) <= 0) {
+  if (smem_opt_in(done, mu, sparse_tc_kernel<D>, smem) <= 0) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
@@ -1067,20 +1146,8 @@ extern "C" int pkv_select_blocks(const uint16_t* q, int64_t q_row_stride, int64_
   const int64_t grid = int64_t(num_chunks) * num_heads * a.groups;
   if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   auto s = static_cast<cudaStream_t>(stream);
-  const size_t smem = sizeof(SelectSmem);
-  static std::mutex mu;
-  static int done128[kMaxDevices] = {}, done64[kMaxDevices] = {};
-  const int ok = head_dim == 128 ? opt_in_smem(done128, mu, select_blocks_kernel<128>, smem)
-                                 : opt_in_smem(done64, mu, select_blocks_kernel<64>, smem);
-  if (ok <= 0) {
-    cudaGetLastError();
-    return PKV_ELAUNCH;
-  }
-  if (head_dim == 128)
-    select_blocks_kernel<128><<<int(grid), kSelThreads, smem, s>>>(a);
-  else
-    select_blocks_kernel<64><<<int(grid), kSelThreads, smem, s>>>(a);
-  return launch_status();
+  const int rc = head_dim == 128 ? launch_select<128>(a, grid, s) : launch_select<64>(a, grid, s);
+  return rc;
 }
 
 extern "C" int pkv_block_attention(const uint16_t* q, int64_t q_row_stride, int64_t q_head_stride,

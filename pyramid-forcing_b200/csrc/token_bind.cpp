@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -145,6 +146,62 @@ std::tuple<Tensor, Tensor, Tensor> op_layer_norm_backward(
   return {dx, dw, db};
 }
 
+bool wants_grad(const std::optional<Tensor>& t) {
+  return t.has_value() && t->defined() && t->requires_grad();
+}
+
+// Layer norm over the last dimension of any x, with its gradient.
+Tensor norm_rows(const Tensor& x) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "pkv_layer_norm: x has no channels");
+  return x.reshape({x.numel() / x.size(-1), x.size(-1)});
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void refuse_twice(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op,
+              ": the gradient is not differentiable (no create_graph)");
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, std::optional<Tensor> weight,
+                        std::optional<Tensor> bias, double eps, bool one_plus) {
+    const Tensor rows = norm_rows(x);
+    auto [y, mean, rstd] = op_layer_norm(rows, weight, bias, eps, one_plus, true);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), mean, rstd});
+    ctx->saved_data["one_plus"] = one_plus;
+    return y.view(x.sizes());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_twice("pkv_norm");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+    const bool need_w = w.defined() && ctx->needs_input_grad(1);
+    const bool need_b = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
+    auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    auto [dx, dw, db] = op_layer_norm_backward(
+        norm_rows(grads[0]), norm_rows(x), opt(w), opt(b), saved[3], saved[4],
+        ctx->saved_data["one_plus"].toBool(), ctx->needs_input_grad(0), need_w, need_b);
+    if (dx.defined()) dx = dx.view(x.sizes());
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Tensor op_norm(Tensor x, std::optional<Tensor> weight, std::optional<Tensor> bias, double eps,
+               bool one_plus) {
+  return std::get<0>(op_layer_norm(norm_rows(x), weight, bias, eps, one_plus, false))
+      .view(x.sizes());
+}
+
+Tensor op_norm_autograd(Tensor x, std::optional<Tensor> weight, std::optional<Tensor> bias,
+                        double eps, bool one_plus) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
+    return LayerNormFn::apply(x, weight, bias, eps, one_plus);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op_norm(x, weight, bias, eps, one_plus);
+}
+
 // ---- rotary positions --------------------------------------------------------
 Tensor dense_heads(const Tensor& x) { return x.stride(2) == 1 || x.size(2) == 1 ? x : x.contiguous(); }
 
@@ -195,6 +252,71 @@ std::tuple<Tensor, Tensor> op_rotary(Tensor q, std::optional<Tensor> k, Tensor p
                       int(inv_freq.size(0)), half, float(scale), inverse, stream_of(q)),
            op);
   return {qo, ko};
+}
+
+// Rotary positions of q and k [..., heads, D], with their gradients.
+Tensor rot_rows(const Tensor& x) {
+  TORCH_CHECK(x.dim() >= 3, "pkv_rotary: q and k must be [..., heads, dim]");
+  int64_t n = 1;
+  for (int64_t i = 0; i < x.dim() - 2; ++i) n *= x.size(i);
+  return x.dim() == 3 ? x : x.reshape({n, x.size(-2), x.size(-1)});
+}
+
+std::tuple<Tensor, Tensor> op_rotary_apply(Tensor q, std::optional<Tensor> k, Tensor positions,
+                                           Tensor inv_freq, std::optional<Tensor> axis, bool half,
+                                           double scale) {
+  const bool two = k.has_value() && k->defined();
+  auto [qo, ko] = op_rotary(rot_rows(q), two ? std::optional<Tensor>(rot_rows(*k)) : std::nullopt,
+                            positions, inv_freq, axis, half, scale, false);
+  return {qo.view(q.sizes()), two ? ko.view(k->sizes()) : ko};
+}
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, Tensor q, std::optional<Tensor> k,
+                               Tensor positions, Tensor inv_freq, std::optional<Tensor> axis,
+                               bool half, double scale) {
+    auto [qo, ko] = op_rotary_apply(q, k, positions, inv_freq, axis, half, scale);
+    ctx->save_for_backward({positions, inv_freq, axis.value_or(Tensor())});
+    ctx->saved_data["half"] = half;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["k"] = ko.defined();
+    ctx->set_materialize_grads(false);
+    if (!ko.defined()) return {qo};
+    return {qo, ko};
+  }
+  // the transpose of a rotation: the same turn the other way
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_twice("pkv_rotary_apply");
+    const auto saved = ctx->get_saved_variables();
+    const bool two = ctx->saved_data["k"].toBool();
+    Tensor dq = grads[0], dk = two ? grads[1] : Tensor();
+    if (!ctx->needs_input_grad(0)) dq = Tensor();
+    if (two && !ctx->needs_input_grad(1)) dk = Tensor();
+    variable_list out(7);
+    const Tensor first = dq.defined() ? dq : dk;
+    if (!first.defined()) return out;
+    const bool both = dq.defined() && dk.defined();
+    auto [g0, g1] = op_rotary(
+        rot_rows(first), both ? std::optional<Tensor>(rot_rows(dk)) : std::nullopt, saved[0],
+        saved[1], saved[2].defined() ? std::optional<Tensor>(saved[2]) : std::nullopt,
+        ctx->saved_data["half"].toBool(), ctx->saved_data["scale"].toDouble(), true);
+    out[dq.defined() ? 0 : 1] = g0.view(first.sizes());
+    if (both) out[1] = g1.view(dk.sizes());
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> op_rotary_autograd(Tensor q, std::optional<Tensor> k, Tensor positions,
+                                              Tensor inv_freq, std::optional<Tensor> axis,
+                                              bool half, double scale) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
+              "pkv_rotary_apply: inv_freq has no gradient here; detach it");
+  if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) {
+    const variable_list r = RotaryFn::apply(q, k, positions, inv_freq, axis, half, scale);
+    return {r[0], r.size() > 1 ? r[1] : Tensor()};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return op_rotary_apply(q, k, positions, inv_freq, axis, half, scale);
 }
 
 // ---- block-sparse attention ----------------------------------------------------
@@ -330,6 +452,9 @@ Tensor op_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu, int64_t num_c
 using namespace pkv_torch;
 
 TORCH_LIBRARY_FRAGMENT(adahead, m) {
+  m.def("pkv_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool one_plus) -> Tensor");
+  m.def("pkv_rotary_apply(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, Tensor? axis, "
+        "bool half, float scale) -> (Tensor, Tensor)");
   m.def("pkv_layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool one_plus, "
         "bool stats) -> (Tensor, Tensor, Tensor)");
   m.def("pkv_layer_norm_backward(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, "
@@ -352,4 +477,11 @@ TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
   m.impl("pkv_block_means", op_block_means);
   m.impl("pkv_select_blocks", op_select_blocks);
   m.impl("pkv_block_attention", op_block_attention);
+  m.impl("pkv_norm", op_norm);
+  m.impl("pkv_rotary_apply", op_rotary_apply);
+}
+
+TORCH_LIBRARY_IMPL(adahead, AutogradCUDA, m) {
+  m.impl("pkv_norm", op_norm_autograd);
+  m.impl("pkv_rotary_apply", op_rotary_autograd);
 }

@@ -3,35 +3,15 @@
 ``layer_norm`` normalises over the last dimension and applies a weight and a
 bias that may differ between groups of rows (frames, videos), optionally as
 ``1 + weight``: the ``LN(x) * (1 + scale) + shift`` of a DiT block is one
-launch.  Differentiable in ``x``, ``weight`` and ``bias``
-(``torch.ops.adahead.pkv_layer_norm`` / ``pkv_layer_norm_backward``).  The
-reference leaves this to torch (wan/modules/causal_model.py:335-360).
+launch.  Differentiable (once) in ``x``, ``weight`` and ``bias``
+(``torch.ops.adahead.pkv_norm`` over ``pkv_layer_norm`` and
+``pkv_layer_norm_backward``).  The reference leaves this to torch (wan/modules/causal_model.py:335-360).
 """
 from __future__ import annotations
 
 import torch
 
 from . import _ops
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, one_plus):
-        y, mean, rstd = _ops.ops().pkv_layer_norm(x, weight, bias, eps, one_plus,
-                                                  any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.one_plus = one_plus
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad[:3]
-        dx, dw, db = _ops.ops().pkv_layer_norm_backward(dy, x, weight, bias, mean, rstd,
-                                                        ctx.one_plus, *need)
-        return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None,
-                None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -47,17 +27,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     """
     if not x.is_cuda:
         raise ValueError("layer_norm: x must be a CUDA tensor")
-    if x.dim() == 0:
-        raise ValueError("layer_norm: x needs a last dimension to normalise")
     if weight is not None and bias is not None:
         if weight.dtype != bias.dtype:
             raise ValueError("layer_norm: weight and bias must have one type")
         if weight.shape != bias.shape:
             weight, bias = torch.broadcast_tensors(weight, bias)
-    rows = x.reshape(x.numel() // x.shape[-1], x.shape[-1]) if x.shape[-1] else x.view(0, 0)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
-        y = _LayerNorm.apply(rows, weight, bias, float(eps), bool(one_plus))
-    else:
-        y = _ops.ops().pkv_layer_norm(rows, weight, bias, float(eps), bool(one_plus), False)[0]
-    return y.view(x.shape)
+    return _ops.ops().pkv_norm(x, weight, bias, eps, one_plus)

@@ -57,31 +57,6 @@ def causal_rope_apply(x: torch.Tensor, grid_sizes, freqs: torch.Tensor, start_fr
 # ---- rotary positions of any axes, layout and frequencies ----------------------------
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, axis, half, scale):
-        ctx.save_for_backward(positions, inv_freq, axis)
-        ctx.half, ctx.scale, ctx.two = half, scale, k is not None
-        q_out, k_out = _ops.ops().pkv_rotary(q, k, positions, inv_freq, axis, half, scale, False)
-        return (q_out, k_out) if k is not None else q_out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk=None):
-        # the transpose of a rotation: the same turn the other way
-        positions, inv_freq, axis = ctx.saved_tensors
-        need_k = ctx.two and ctx.needs_input_grad[1]
-        ops = _ops.ops()
-        if not need_k:
-            g = ops.pkv_rotary(dq, None, positions, inv_freq, axis, ctx.half, ctx.scale, True)
-            return (g[0],) + (None,) * 6
-        if not ctx.needs_input_grad[0]:
-            g = ops.pkv_rotary(dk, None, positions, inv_freq, axis, ctx.half, ctx.scale, True)
-            return (None, g[0]) + (None,) * 5
-        g = ops.pkv_rotary(dq, dk, positions, inv_freq, axis, ctx.half, ctx.scale, True)
-        return (g[0], g[1]) + (None,) * 5
-
-
 def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: str = "none",
                        factor: float = 1.0, original_length: int = 8192, beta_fast: float = 32.0,
                        beta_slow: float = 1.0, device=None) -> tuple[torch.Tensor, float]:
@@ -135,7 +110,7 @@ def rotary_apply(x, positions: torch.Tensor, inv_freq: torch.Tensor,
     ``axis`` naming the axis of each pair (1 <= A <= 4).  Pair p turns by
     ``positions[..., axis[p]] * inv_freq[p]`` and is multiplied by ``scale``;
     pairs are elements (2p, 2p + 1) ("interleaved") or (p, p + P) ("half"),
-    P = len(inv_freq); elements from 2P on are copied.  Differentiable in x.
+    P = len(inv_freq); elements from 2P on are copied.  Differentiable (once) in x.
     """
     if layout not in ("interleaved", "half"):
         raise ValueError(f"rotary_apply: unknown layout {layout!r}")
@@ -154,14 +129,5 @@ def rotary_apply(x, positions: torch.Tensor, inv_freq: torch.Tensor,
     tokens = math.prod(lead)
     axes = 1 if positions.shape == lead else positions.shape[-1]
     pos = positions.reshape(tokens, axes).to(torch.int64).contiguous()
-    flat = [None if t is None else t.reshape(tokens, t.shape[-2], t.shape[-1]) for t in (q, k)]
-    args = (flat[0], flat[1], pos, inv_freq, axis, layout == "half", float(scale))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
-        out = _Rotary.apply(*args)
-        if k is None:
-            return out.view(q.shape)
-    else:
-        out = _ops.ops().pkv_rotary(*args, False)
-        if k is None:
-            return out[0].view(q.shape)
-    return out[0].view(q.shape), out[1].view(k.shape)
+    out = _ops.ops().pkv_rotary_apply(q, k, pos, inv_freq, axis, layout == "half", scale)
+    return out[0] if k is None else out

@@ -52,6 +52,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     rows_per_chunk, H, D], k / v bf16 [rows, D].  Entries of ``blocks`` outside
     a segment are skipped, a block listed twice counts twice, a row with no
     keys gives zeros."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise RuntimeError("pkv_block_attention has no gradient: call it under torch.no_grad()")
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     return _ops.ops().pkv_block_attention(q, k, v, cu_seqlens_k, int(num_chunks),
                                           int(rows_per_chunk), blocks, int(query_block),

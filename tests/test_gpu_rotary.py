@@ -195,6 +195,11 @@ def test_rotary_refusals(cuda):
                     (pos, inv.cpu(), axis), (pos[:, :1], torch.cat([inv, inv]), None)):
         with pytest.raises(RuntimeError, match="pkv_rotary"):
             rotary_apply(q, p, f, a)
+    with pytest.raises(RuntimeError, match="inv_freq"):
+        rotary_apply(q, pos, inv.clone().requires_grad_(True), axis)
+    x = torch.randn(4, 2, 64, device=cuda, requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(rotary_apply(x, pos, inv, axis).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="bf16, fp16 or fp32"):
         rotary_apply(q.double(), pos, inv, axis)
     assert math.isfinite(float(q.float().sum()))

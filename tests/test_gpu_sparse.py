@@ -350,6 +350,8 @@ def test_refusals(cuda):
     for bad in (lists.long(), lists[:1], lists[0], lists.expand(2, 2, 2)):
         with pytest.raises(RuntimeError, match="blocks"):
             block_attention(q, k, v, cu, 1, 3, bad)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        sparse_attention(q.clone().requires_grad_(True), k, v, cu, 1, 3, 2)
     with pytest.raises(RuntimeError, match="softmax_scale"):
         block_attention(q, k, v, cu, 1, 3, lists, softmax_scale=-1.0)
 
