@@ -420,7 +420,7 @@ int pkv_rope_q(const uint16_t *x, int64_t x_tok_stride, int64_t x_head_stride, u
  * weight / bias: [groups, cols] (either may be NULL), row r uses row
  * r / (rows / groups); groups divides rows.  dtype: x and y; wtype: weight and
  * bias (dtype or PKV_FP32).  Rows are x_row_stride / y_row_stride elements
- * apart, channels contiguous.  cols <= 2^20.  mean / rstd: fp32 [rows], saved for the backward pass
+ * apart, channels contiguous.  rows < 2^31, cols <= 2^20.  mean / rstd: fp32 [rows], saved for the backward pass
  * (nullable).
  */
 int pkv_layer_norm(const void *x, int64_t x_row_stride, const void *weight, const void *bias,

@@ -31,7 +31,7 @@ CU_SOURCES = ["pkv_update.cu", "pkv_merge.cu", "pkv_plan.cu", "pkv_pack.cu", "pk
               "pkv_rotary.cu", "pkv_sparse.cu"]
 BIND_SOURCES = ["adahead_bind.cpp", "token_bind.cpp"]
 HEADERS = ["pkv_common.cuh", "pkv_internal.h", "pkv_plan.cuh", "pkv_vec.cuh",
-           "pkv_tc.cuh"]
+           "pkv_tc.cuh", "pkv_f2.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
            "--ptxas-options=-v"] + ARCH

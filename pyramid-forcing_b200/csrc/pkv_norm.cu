@@ -18,6 +18,7 @@
 // (thread = fixed columns), keeps its column sums in registers over its rows
 // and writes them to a [parts, 2, C] workspace once; a second kernel adds the
 // parts in order.  No atomics: the result does not depend on timing.
+#include "pkv_f2.cuh"
 #include "pkv_vec.cuh"
 
 namespace pkv {
@@ -34,7 +35,7 @@ struct NormArgs {
   float* mean;
   float* rstd;
   int64_t x_rs, y_rs, rows, rows_per_group;
-  int C;
+  int C, parts;  // parts: blocks of a group (norm_cols_fwd_kernel)
   float eps, plus;
 };
 
@@ -49,6 +50,77 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   float s = 0.0f;
   for (int i = 0; i < nw; ++i) s += red[i];
   return s;
+}
+
+// Sums of N <= 4 values over a block, the same in every thread, with one
+// barrier.  A warp folds its values into one another on the way down the
+// butterfly (6 shuffles for 4 values), lanes 0, 8, 16, 24 are left with one
+// sum each.  `buf` ([warps][4]) must not be in use by an earlier call that a
+// slower warp still reads: callers alternate two.
+template <int N>
+__device__ __forceinline__ void block_sums(float (&v)[N], float (*buf)[4]) {
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  constexpr uint32_t kAll = 0xffffffffu;
+  float r;
+  if constexpr (N > 2) {
+    const bool up = lane & 16;
+    const float v3 = N > 3 ? v[N - 1] : 0.0f;
+    float a0 = up ? v[2] : v[0], a1 = up ? v3 : v[1];
+    a0 += __shfl_xor_sync(kAll, up ? v[0] : v[2], 16);
+    a1 += __shfl_xor_sync(kAll, up ? v[1] : v3, 16);
+    const bool up8 = lane & 8;
+    r = (up8 ? a1 : a0) + __shfl_xor_sync(kAll, up8 ? a0 : a1, 8);
+  } else if constexpr (N == 2) {
+    const bool up8 = lane & 8;
+    r = (up8 ? v[1] : v[0]) + __shfl_xor_sync(kAll, up8 ? v[0] : v[1], 8);
+    r += __shfl_xor_sync(kAll, r, 16);
+  } else {
+    r = v[0] + __shfl_xor_sync(kAll, v[0], 8);
+    r += __shfl_xor_sync(kAll, r, 16);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) r += __shfl_xor_sync(kAll, r, o);
+  if ((lane & 7) == 0) buf[threadIdx.x >> 5][lane >> 3] = r;
+  __syncthreads();
+  // lane 4 w + i adds value i of warps w, w + 8, ...; then across the lanes
+  const int w0 = lane >> 2;
+  r = w0 < nw ? buf[w0][lane & 3] : 0.0f;
+  for (int w = w0 + 8; w < nw; w += 8) r += buf[w][lane & 3];
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) r += __shfl_xor_sync(kAll, r, o);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kAll, r, i);
+}
+
+// E elements of a row's vectors as pairs (the last one padded with 0).
+template <int E>
+struct Pairs {
+  static constexpr int kN = (E + 1) / 2;
+  f2 p[kN];
+};
+template <typename T, int V, int NV>
+__device__ __forceinline__ Pairs<V * NV> to_pairs(const Vec<T, V> (&v)[NV]) {
+  Pairs<V * NV> r;
+  float f[2 * r.kN];
+  f[2 * r.kN - 1] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) widen<T, V>(v[i], f + i * V);
+#pragma unroll
+  for (int i = 0; i < r.kN; ++i) r.p[i] = mk2(f[2 * i], f[2 * i + 1]);
+  return r;
+}
+template <typename T, int V, int NV>
+__device__ __forceinline__ void from_pairs(const Pairs<V * NV>& r, Vec<T, V> (&v)[NV]) {
+  float f[2 * r.kN];
+#pragma unroll
+  for (int i = 0; i < r.kN; ++i) un2(r.p[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = narrow<T, V>(f + i * V);
+}
+__device__ __forceinline__ float fold(f2 a) {
+  float lo, hi;
+  un2(a, lo, hi);
+  return lo + hi;
 }
 
 // What a thread does with its vectors of a row once they are in f: centre,
@@ -77,10 +149,7 @@ __device__ __forceinline__ void norm_store(const NormArgs& a, int64_t row, int t
 #pragma unroll
         for (int e = 0; e < V; ++e) r[e] += t2[e];
       }
-      Vec<TX, V> t;
-#pragma unroll
-      for (int e = 0; e < V; ++e) t.v[e] = from_f32<TX>(r[e]);
-      st_vec<TX, V>(y + j * V, t);
+      st_vec<TX, V>(y + j * V, narrow<TX, V>(r));
     }
   }
 }
@@ -99,9 +168,7 @@ __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int j = tid + i * tpr;
     if (j < nvec) {
-      const Vec<TX, V> t = ld_vec<TX, V>(x + j * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[i][e] = to_f32(t.v[e]);
+      widen<TX, V>(ld_vec<TX, V>(x + j * V), f[i]);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
@@ -164,9 +231,9 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_stream_kernel(NormArgs a
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (lane + i * 32 < nvec) {
-        const Vec<TX, V> t = ring[(st * NV + i) * 32];
+        widen<TX, V>(ring[(st * NV + i) * 32], f[i]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += f[i][e] = to_f32(t.v[e]);
+        for (int e = 0; e < V; ++e) s += f[i][e];
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
@@ -191,6 +258,136 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_stream_kernel(NormArgs a
       if (a.rstd) a.rstd[row] = rstd;
     }
     norm_store<TX, TW, V, NV>(a, row, lane, 32, nvec, f, rstd);
+  }
+}
+
+// A block a range of a group's rows, every column (thread = fixed columns, as
+// the backward pass): weight and bias are read once and stay in registers,
+// kFwdRows rows share the two barriers of their statistics, and the next
+// rounds' rows are on their way into shared memory meanwhile.
+constexpr int kFwdRows = 4, kColStages = 3;
+
+template <typename TX, typename TW, int V, int NV, int kThreads>
+__global__ void __launch_bounds__(kThreads, 768 / kThreads) norm_cols_fwd_kernel(NormArgs a) {
+  constexpr int R = kFwdRows, E = V * NV;
+  __shared__ __align__(16) float red[2][kThreads / 32][4];
+  extern __shared__ __align__(16) uint8_t raw[];
+  const int tid = threadIdx.x, nthr = blockDim.x;
+  Vec<TX, V>* ring = reinterpret_cast<Vec<TX, V>*>(raw) + tid;  // [stage][row][NV][nthr]
+  const int64_t grp = blockIdx.x / a.parts;
+  const int p = int(blockIdx.x - grp * a.parts);
+  const int64_t r0 = grp * a.rows_per_group + a.rows_per_group * p / a.parts;
+  const int64_t r1 = grp * a.rows_per_group + a.rows_per_group * (p + 1) / a.parts;
+  const int nvec = a.C / V;
+  const float inv_c = 1.0f / float(a.C);
+  const int n = int(r1 - r0);  // rows of this block
+  const TX* xp = static_cast<const TX*>(a.x) + r0 * a.x_rs + tid * V;
+  TX* yp = static_cast<TX*>(a.y) + r0 * a.y_rs + tid * V;
+  int ahead = 0;  // rows asked for
+  auto fetch = [&](int st) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (ahead + k < n)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (tid + i * nthr < nvec)
+            cp_async<TX, V>(ring + ((st * R + k) * NV + i) * nthr, xp + i * nthr * V);
+      xp += a.x_rs;
+    }
+    ahead += R;
+    cp_commit();
+  };
+  for (int i = 0; i < kColStages - 1; ++i) fetch(i);
+  Pairs<E> w, b;
+  {
+    const TW* wp = a.w ? static_cast<const TW*>(a.w) + grp * a.C : nullptr;
+    const TW* bp = a.b ? static_cast<const TW*>(a.b) + grp * a.C : nullptr;
+    float fw[E], fb[E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = tid + i * nthr;
+      float tw[V], tb[V];
+      if (wp && j < nvec) ld_f32<TW, V>(wp + j * V, tw);
+      if (bp && j < nvec) ld_f32<TW, V>(bp + j * V, tb);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        fw[i * V + e] = wp && j < nvec ? tw[e] + a.plus : 1.0f;
+        fb[i * V + e] = bp && j < nvec ? tb[e] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < w.kN; ++i) {
+      w.p[i] = mk2(fw[2 * i], 2 * i + 1 < E ? fw[(2 * i + 1) % E] : 0.0f);
+      b.p[i] = mk2(fb[2 * i], 2 * i + 1 < E ? fb[(2 * i + 1) % E] : 0.0f);
+    }
+  }
+  int st = 0;
+  for (int r = 0; r < n; r += R) {
+    cp_wait<kColStages - 2>();
+    Pairs<E> f[R];
+    float s[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      Vec<TX, V> v[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (r + k < n && tid + i * nthr < nvec)
+          v[i] = ring[((st * R + k) * NV + i) * nthr];
+        else
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[i].v[e] = from_f32<TX>(0.0f);
+      }
+      f[k] = to_pairs<TX, V, NV>(v);
+      f2 t = f[k].p[0];
+#pragma unroll
+      for (int i = 1; i < f[k].kN; ++i) t = add2(t, f[k].p[i]);
+      s[k] = fold(t);
+    }
+    fetch(st == 0 ? kColStages - 1 : st - 1);
+    st = st + 1 == kColStages ? 0 : st + 1;
+    block_sums<R>(s, red[0]);
+    float mu[R], q[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      mu[k] = s[k] * inv_c;
+      const f2 m2 = mk2(mu[k], mu[k]);
+      f2 t = mk2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < f[k].kN; ++i) f[k].p[i] = sub2(f[k].p[i], m2);
+      // columns that are not there hold -mu now: leave them out
+#pragma unroll
+      for (int i = 0; i < f[k].kN; ++i) {
+        const int e0 = 2 * i, e1 = 2 * i + 1;
+        const bool in0 = tid + e0 / V * nthr < nvec;
+        const bool in1 = e1 < E && tid + e1 % E / V * nthr < nvec;
+        if (in0 && in1) {
+          t = fma2(f[k].p[i], f[k].p[i], t);
+        } else if (in0) {
+          float lo, hi, tl, th;
+          un2(f[k].p[i], lo, hi);
+          un2(t, tl, th);
+          t = mk2(fmaf(lo, lo, tl), th);
+        }
+      }
+      q[k] = fold(t);
+    }
+    block_sums<R>(q, red[1]);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (r + k >= n) break;
+      const float rstd = rsqrtf(q[k] * inv_c + a.eps);
+      if (tid == 0 && a.mean) a.mean[r0 + r + k] = mu[k];
+      if (tid == 0 && a.rstd) a.rstd[r0 + r + k] = rstd;
+      const f2 r2 = mk2(rstd, rstd);
+#pragma unroll
+      for (int i = 0; i < f[k].kN; ++i) f[k].p[i] = fma2(mul2(f[k].p[i], r2), w.p[i], b.p[i]);
+      Vec<TX, V> v[NV];
+      from_pairs<TX, V, NV>(f[k], v);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * nthr < nvec) st_vec<TX, V>(yp + i * nthr * V, v[i]);
+      yp += a.y_rs;
+    }
   }
 }
 
@@ -248,14 +445,14 @@ __host__ __device__ constexpr int bwd_rows(int elems) { return elems <= 8 ? 2 : 
 // 16-bit single elements (V = 1) are too small for asynchronous copies and
 // are loaded directly.
 template <typename TX, typename TW, int V, int NV, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads <= 256 && V * NV <= 8 ? 3 : 1)
+__global__ void __launch_bounds__(kThreads, kThreads <= 192 ? 3 : kThreads <= 256 && V * NV <= 8 ? 2 : 1)
     norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int R = bwd_rows(V * NV);
+  constexpr int R = bwd_rows(V * NV), E = V * NV;
   constexpr bool kRing = V * sizeof(TX) >= 4;
   constexpr int kStages = bwd_stages(R * 2 * NV * V * sizeof(TX));
-  __shared__ float red[2][2 * R][kThreads / 32];
+  __shared__ __align__(16) float red[2][kThreads / 32][4];
   extern __shared__ __align__(16) uint8_t raw[];
-  const int tid = threadIdx.x, nthr = blockDim.x, nw = nthr >> 5;
+  const int tid = threadIdx.x, nthr = blockDim.x;
   Vec<TX, V>* ring = reinterpret_cast<Vec<TX, V>*>(raw) + tid;  // [stage][row][x, dy][NV][nthr]
   const int64_t grp = blockIdx.x / a.parts;
   const int p = int(blockIdx.x - grp * a.parts);
@@ -264,145 +461,137 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 256 && V * NV <= 8 ? 3 :
   const int nvec = a.C / V;
   const float inv_c = 1.0f / float(a.C);
   const TW* wp = a.w ? static_cast<const TW*>(a.w) + grp * a.C : nullptr;
-  auto fetch = [&](int64_t r, int st) {
+  const int n = int(r1 - r0);  // rows of this block
+  const TX* xp = static_cast<const TX*>(a.x) + r0 * a.x_rs + tid * V;
+  const TX* dp = static_cast<const TX*>(a.dy) + r0 * a.dy_rs + tid * V;
+  TX* op = static_cast<TX*>(a.dx) + r0 * a.dx_rs + tid * V;
+  int ahead = 0;  // rows asked for
+  auto fetch = [&](int st) {
     if constexpr (kRing) {
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        if (r + k < r1) {
-          const TX* x = static_cast<const TX*>(a.x) + (r + k) * a.x_rs;
-          const TX* d = static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs;
+        if (ahead + k < n)
 #pragma unroll
-          for (int i = 0; i < NV; ++i) {
-            const int j = tid + i * nthr;
-            if (j < nvec) {
-              Vec<TX, V>* slot = ring + int64_t(((st * R + k) * 2) * NV + i) * nthr;
-              cp_async<TX, V>(slot, x + j * V);
-              cp_async<TX, V>(slot + NV * nthr, d + j * V);
+          for (int i = 0; i < NV; ++i)
+            if (tid + i * nthr < nvec) {
+              Vec<TX, V>* slot = ring + (((st * R + k) * 2) * NV + i) * nthr;
+              cp_async<TX, V>(slot, xp + i * nthr * V);
+              cp_async<TX, V>(slot + NV * nthr, dp + i * nthr * V);
             }
-          }
-        }
+        xp += a.x_rs;
+        dp += a.dy_rs;
       }
+      ahead += R;
       cp_commit();
     }
   };
-  for (int i = 0; i < kStages - 1; ++i) fetch(r0 + i * R, i);
-  float w[NV][V], aw[NV][V], ab[NV][V];
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  Pairs<E> w, aw, ab;
+  {
+    float fw[E];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int j = tid + i * nthr;
-    const bool have = wp && j < nvec;
-    if (have) ld_f32<TW, V>(wp + j * V, w[i]);
+    for (int i = 0; i < NV; ++i) {
+      const int j = tid + i * nthr;
+      float tw[V];
+      if (wp && j < nvec) ld_f32<TW, V>(wp + j * V, tw);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      w[i][e] = have ? w[i][e] + a.plus : 1.0f;
-      aw[i][e] = ab[i][e] = 0.0f;
+      for (int e = 0; e < V; ++e) fw[i * V + e] = wp && j < nvec ? tw[e] + a.plus : 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < w.kN; ++i) {
+      w.p[i] = mk2(fw[2 * i], 2 * i + 1 < E ? fw[(2 * i + 1) % E] : 0.0f);
+      aw.p[i] = ab.p[i] = mk2(0.0f, 0.0f);
     }
   }
   int round = 0, st = 0;
-  for (int64_t r = r0; r < r1; r += R, ++round) {
-    Vec<TX, V> vx[R][NV], vd[R][NV];
-    float mu[R], rs[R], c1[R], c2[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      mu[k] = r + k < r1 ? a.mean[r + k] : 0.0f;
-      rs[k] = r + k < r1 ? a.rstd[r + k] : 0.0f;
-    }
+  for (int r = 0; r < n; r += R, ++round) {
+    Pairs<E> xh[R], gr[R];
+    float rs[R], c[2 * R];
     if constexpr (kRing) cp_wait<kStages - 2>();
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      const bool live = r + k < r1;
+      const bool live = r + k < n;
+      const float mu = live ? a.mean[r0 + r + k] : 0.0f;
+      rs[k] = live ? a.rstd[r0 + r + k] : 0.0f;
+      Vec<TX, V> vx[NV], vd[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = tid + i * nthr;
-        if (live && j < nvec) {
+        if (live && tid + i * nthr < nvec) {
           if constexpr (kRing) {
-            const Vec<TX, V>* slot = ring + int64_t(((st * R + k) * 2) * NV + i) * nthr;
-            vx[k][i] = slot[0];
-            vd[k][i] = slot[NV * nthr];
+            const Vec<TX, V>* slot = ring + (((st * R + k) * 2) * NV + i) * nthr;
+            vx[i] = slot[0];
+            vd[i] = slot[NV * nthr];
           } else {
-            vx[k][i] = ld_vec<TX, V>(static_cast<const TX*>(a.x) + (r + k) * a.x_rs + j * V);
-            vd[k][i] = ld_vec<TX, V>(static_cast<const TX*>(a.dy) + (r + k) * a.dy_rs + j * V);
+            vx[i] = ld_vec<TX, V>(xp + i * nthr * V);
+            vd[i] = ld_vec<TX, V>(dp + i * nthr * V);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) vx[k][i].v[e] = vd[k][i].v[e] = from_f32<TX>(0.0f);
+          for (int e = 0; e < V; ++e) vx[i].v[e] = vd[i].v[e] = from_f32<TX>(0.0f);
         }
       }
+      if constexpr (!kRing) {
+        xp += a.x_rs;
+        dp += a.dy_rs;
+      }
+      // (columns and rows that are not there have dy = 0; such rows rstd = 0)
+      xh[k] = to_pairs<TX, V, NV>(vx);
+      gr[k] = to_pairs<TX, V, NV>(vd);
+      const f2 m2 = mk2(mu, mu), r2 = mk2(rs[k], rs[k]);
+      f2 s1 = mk2(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+      for (int i = 0; i < w.kN; ++i) {
+        const f2 d = gr[k].p[i];
+        xh[k].p[i] = mul2(sub2(xh[k].p[i], m2), r2);
+        gr[k].p[i] = mul2(d, w.p[i]);
+        s1 = add2(s1, gr[k].p[i]);
+        s2 = fma2(gr[k].p[i], xh[k].p[i], s2);
+        aw.p[i] = fma2(d, xh[k].p[i], aw.p[i]);
+        ab.p[i] = add2(ab.p[i], d);
+      }
+      c[2 * k] = fold(s1);
+      c[2 * k + 1] = fold(s2);
     }
     // the slot read one round ago is free: its values were in registers
-    fetch(r + int64_t(kStages - 1) * R, st == 0 ? kStages - 1 : st - 1);
+    fetch(st == 0 ? kStages - 1 : st - 1);
     st = st + 1 == kStages ? 0 : st + 1;
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      c1[k] = c2[k] = 0.0f;
-      // (columns and rows that are not there have dy = 0, and mean and rstd 0)
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = to_f32(vd[k][i].v[e]);
-          const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
-          const float g = d * w[i][e];
-          c1[k] += g;
-          c2[k] = fmaf(g, xh, c2[k]);
-          aw[i][e] = fmaf(d, xh, aw[i][e]);
-          ab[i][e] += d;
-        }
-      c1[k] = warp_sum(c1[k]);
-      c2[k] = warp_sum(c2[k]);
-    }
     // two buffers in turn: a warp may write the next round's while another
     // still reads this one's
-    auto& buf = red[round & 1];
-    if ((tid & 31) == 0)
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        buf[2 * k][tid >> 5] = c1[k];
-        buf[2 * k + 1][tid >> 5] = c2[k];
-      }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      c1[k] = c2[k] = 0.0f;
-      for (int i = 0; i < nw; ++i) {
-        c1[k] += buf[2 * k][i];
-        c2[k] += buf[2 * k + 1][i];
-      }
-      c1[k] *= inv_c;
-      c2[k] *= inv_c;
-    }
+    block_sums<2 * R>(c, red[round & 1]);
     if (a.dx != nullptr) {
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        if (r + k >= r1) break;
-        TX* dx = static_cast<TX*>(a.dx) + (r + k) * a.dx_rs;
+        if (r + k >= n) break;
+        const float n1 = -c[2 * k] * inv_c, n2 = -c[2 * k + 1] * inv_c;
+        const f2 c1 = mk2(n1, n1), c2 = mk2(n2, n2), r2 = mk2(rs[k], rs[k]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int j = tid + i * nthr;
-          if (j < nvec) {
-            Vec<TX, V> t;
+        for (int i = 0; i < w.kN; ++i)
+          gr[k].p[i] = mul2(fma2(xh[k].p[i], c2, add2(gr[k].p[i], c1)), r2);
+        Vec<TX, V> v[NV];
+        from_pairs<TX, V, NV>(gr[k], v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float xh = (to_f32(vx[k][i].v[e]) - mu[k]) * rs[k];
-              const float g = to_f32(vd[k][i].v[e]) * w[i][e];
-              t.v[e] = from_f32<TX>(rs[k] * (g - c1[k] - xh * c2[k]));
-            }
-            st_vec<TX, V>(dx + j * V, t);
-          }
-        }
+        for (int i = 0; i < NV; ++i)
+          if (tid + i * nthr < nvec) st_vec<TX, V>(op + i * nthr * V, v[i]);
+        op += a.dx_rs;
       }
     }
   }
   if (a.part != nullptr) {
     float* pw = a.part + int64_t(blockIdx.x) * 2 * a.C;
+    float sw[2 * w.kN], sb[2 * w.kN];
+#pragma unroll
+    for (int i = 0; i < w.kN; ++i) {
+      un2(aw.p[i], sw[2 * i], sw[2 * i + 1]);
+      un2(ab.p[i], sb[2 * i], sb[2 * i + 1]);
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = tid + i * nthr;
       if (j < nvec)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          pw[j * V + e] = aw[i][e];
-          pw[a.C + j * V + e] = ab[i][e];
+          pw[j * V + e] = sw[i * V + e];
+          pw[a.C + j * V + e] = sb[i * V + e];
         }
     }
   }
@@ -452,42 +641,54 @@ __global__ void __launch_bounds__(kNormThreads) norm_cols_kernel(NormBwdArgs a) 
   a.part[int64_t(blockIdx.x) * 2 * a.C + a.C + c] = sb;
 }
 
-// Column sums of a group's parts, in order, rounded to the weight's type.
-// 32 columns x 8 slices of the parts a block; the slices meet in shared memory.
+// Column sums of a group's parts, in a fixed order, rounded to the weight's
+// type.  32 columns x 32 slices of the parts a block, four parts of a slice on
+// their way at once; the slices meet in shared memory.
 template <typename TW>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     norm_parts_kernel(const float* part, int parts, int C, TW* dw, TW* db) {
-  __shared__ float sm[8][2][32];
+  __shared__ float sm[2][32][33];
   const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5;
   const int c = blockIdx.y * 32 + lane;
   const int64_t grp = blockIdx.x;
   float sw = 0.0f, sb = 0.0f;
-  if (c < C)
-    for (int p = sl; p < parts; p += 8) {
-      const float* q = part + (grp * parts + p) * 2 * int64_t(C);
-      sw += q[c];
-      sb += q[C + c];
+  if (c < C) {
+    const float* q = part + grp * parts * 2 * int64_t(C) + c;
+    for (int p = sl; p < parts; p += 128) {
+      float w[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = p + 32 * i < parts;
+        w[i] = in ? q[int64_t(p + 32 * i) * 2 * C] : 0.0f;
+        b[i] = in ? q[int64_t(p + 32 * i) * 2 * C + C] : 0.0f;
+      }
+      sw += (w[0] + w[1]) + (w[2] + w[3]);
+      sb += (b[0] + b[1]) + (b[2] + b[3]);
     }
-  sm[sl][0][lane] = sw;
-  sm[sl][1][lane] = sb;
-  __syncthreads();
-  if (sl != 0 || c >= C) return;
-  sw = sb = 0.0f;
-  for (int i = 0; i < 8; ++i) {
-    sw += sm[i][0][lane];
-    sb += sm[i][1][lane];
   }
-  if (dw) dw[grp * C + c] = from_f32<TW>(sw);
-  if (db) db[grp * C + c] = from_f32<TW>(sb);
+  sm[0][sl][lane] = sw;
+  sm[1][sl][lane] = sb;
+  __syncthreads();
+  // warp x adds column x: lanes are the slices
+  sw = warp_sum(sm[0][lane][sl]);
+  sb = warp_sum(sm[1][lane][sl]);
+  const int col = blockIdx.y * 32 + sl;
+  if (lane == 0 && col < C) {
+    if (dw) dw[grp * C + col] = from_f32<TW>(sw);
+    if (db) db[grp * C + col] = from_f32<TW>(sb);
+  }
 }
 
-// Parts of a group in the backward pass: about three CTAs an SM over all
-// groups, at least two rows each.
-int64_t bwd_parts(int64_t rows_per_group, int64_t groups) {
-  const int64_t want = (int64_t(sm_count()) * 3 + groups - 1) / groups;
-  const int64_t most = (rows_per_group + 1) / 2;
+// Blocks that share a group's rows: about `per_sm` an SM over all groups, at
+// least `least` rows each.
+int64_t row_parts(int64_t rows_per_group, int64_t groups, int per_sm, int least) {
+  const int64_t want = (int64_t(sm_count()) * per_sm + groups - 1) / groups;
+  const int64_t most = (rows_per_group + least - 1) / least;
   const int64_t p = want < most ? want : most;
   return p < 1 ? 1 : p;
+}
+int64_t bwd_parts(int64_t rows_per_group, int64_t groups) {
+  return row_parts(rows_per_group, groups, 3, 8);
 }
 
 constexpr int round_warp(int n) { return (n + 31) / 32 * 32; }
@@ -508,21 +709,40 @@ int stream_fwd(const NormArgs& a, cudaStream_t s) {
   return launch_status();
 }
 
+template <typename TX, typename TW, int V, int NV, int kThreads>
+int cols_fwd(NormArgs a, cudaStream_t s) {
+  const int thr = round_warp((a.C / V + NV - 1) / NV);
+  constexpr size_t per = size_t(kColStages) * kFwdRows * NV * V * sizeof(TX);
+  static_assert(per * kThreads <= 200 * 1024, "the rounds of a block fit its shared memory");
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  if (smem_opt_in(done, mu, norm_cols_fwd_kernel<TX, TW, V, NV, kThreads>, per * kThreads) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  const int64_t groups = a.rows / a.rows_per_group;
+  a.parts = int(row_parts(a.rows_per_group, groups, 1024 / kThreads, 2 * kFwdRows));
+  const int64_t grid = groups * a.parts;
+  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  norm_cols_fwd_kernel<TX, TW, V, NV, kThreads><<<int(grid), thr, per * thr, s>>>(a);
+  return launch_status();
+}
+
 template <typename TX, typename TW, int V>
 int launch_fwd(const NormArgs& a, cudaStream_t s) {
   const int nvec = a.C / V;
   if constexpr (V * sizeof(TX) >= 4) {
-    // rows for two warps of every scheduler and a row that fits a warp's
-    // registers: stream
-    if (nvec <= 32 * 8 && a.rows >= int64_t(sm_count()) * 16) {
+    if (a.rows >= int64_t(sm_count()) * 16) {
+      // short rows: a warp a row; longer ones, in groups that give a block
+      // rows to share its weights over: fixed columns
       if (nvec <= 32) return stream_fwd<TX, TW, V, 1>(a, s);
       if (nvec <= 64) return stream_fwd<TX, TW, V, 2>(a, s);
-      if (nvec <= 128) return stream_fwd<TX, TW, V, 4>(a, s);
-      if (nvec <= 192) return stream_fwd<TX, TW, V, 6>(a, s);
-      return stream_fwd<TX, TW, V, 8>(a, s);
+      if (a.rows_per_group >= 2 * kFwdRows) {
+        if (nvec <= 256) return cols_fwd<TX, TW, V, 1, 256>(a, s);
+        if (nvec <= 512) return cols_fwd<TX, TW, V, 2, 256>(a, s);
+      }
     }
   }
-  if (a.rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   const int grid = int(a.rows);
   auto threads = [nvec](int nv) { return round_warp((nvec + nv - 1) / nv); };
   // about 256 threads a row; up to 1024 where the row is longer than NV = 8
@@ -562,7 +782,8 @@ int launch_bwd(const NormBwdArgs& a, int64_t groups, cudaStream_t s) {
   const int nvec = a.C / V;
   const int64_t grid = groups * a.parts;
   const int64_t rows = groups * a.rows_per_group;
-  if (grid >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  if (nvec <= 192) return row_bwd<TX, TW, V, 1, 192>(a, grid, s);
   if (nvec <= 256) return row_bwd<TX, TW, V, 1, 256>(a, grid, s);
   if (nvec <= 512) return row_bwd<TX, TW, V, 2, 256>(a, grid, s);
   if constexpr (V >= 8) {
@@ -615,7 +836,7 @@ int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream
     rc = launch_bwd<TX, TW, 1>(a, groups, s);
   if (rc != PKV_OK || a.part == nullptr) return rc;
   const dim3 grid(unsigned(groups), unsigned((a.C + 31) / 32));
-  norm_parts_kernel<TW><<<grid, 256, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
+  norm_parts_kernel<TW><<<grid, 1024, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
                                              static_cast<TW*>(db));
   return launch_status();
 }
@@ -642,7 +863,7 @@ extern "C" int pkv_layer_norm(const void* x, int64_t x_row_stride, const void* w
   if (rows < 0 || cols <= 0 || groups <= 0 || !norm_types(dtype, wtype)) return PKV_EINVAL;
   if (rows == 0) return PKV_OK;
   if (!x || !y || rows % groups != 0 || !(eps >= 0.0f)) return PKV_EINVAL;
-  if (cols > kMaxCols) return PKV_EUNSUPPORTED;
+  if (cols > kMaxCols || rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   NormArgs a{};
   a.x = x;
   a.w = weight;
@@ -675,7 +896,7 @@ extern "C" int pkv_layer_norm_backward(const void* dy, int64_t dy_row_stride, co
                                        pkv_stream_t stream) {
   if (rows <= 0 || cols <= 0 || groups <= 0 || !norm_types(dtype, wtype)) return PKV_EINVAL;
   if (!dy || !x || !mean || !rstd || rows % groups != 0) return PKV_EINVAL;
-  if (cols > kMaxCols) return PKV_EUNSUPPORTED;
+  if (cols > kMaxCols || rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (!sums && !dx) return PKV_OK;
   if (sums && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||

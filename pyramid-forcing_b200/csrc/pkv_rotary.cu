@@ -33,8 +33,6 @@ struct RotSide {
   int heads;
 };
 
-constexpr int kUnroll = 4;
-
 // n / d for n < 2^31 by a multiplication (d >= 1): with s = ceil(log2 d) and
 // mul = ceil(2^(31 + s) / d) the product's error stays below 1 / d.
 struct Div {
@@ -60,11 +58,26 @@ struct RotArgs {
   float scale, sign;
 };
 
-template <typename T, int V>
+// kPair: a unit is V pairs out of two vectors (half layout, and interleaved
+// single elements); else it is one vector of V / 2 interleaved pairs.
+template <typename T, int V, bool kHalf>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
+  constexpr bool kPair = kHalf || V == 1;
   __shared__ float2 tab[kRotTable];
   const int64_t t0 = blockIdx.x * int64_t(a.tile);
   const int nt = int(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
+  const int h0 = a.s[0].heads, heads = h0 + a.s[1].heads;
+  auto rows = [&](uint32_t th, const T*& x, T*& o, int& t) {
+    t = int(a.by_heads.div(th));
+    int h = int(th) - t * heads;
+    const bool second = h >= h0;
+    if (second) h -= h0;
+    const RotSide& sd = a.s[second ? 1 : 0];
+    x = static_cast<const T*>(sd.x) + (t0 + t) * sd.x_tok + h * sd.x_head;
+    o = static_cast<T*>(sd.out) + (t0 + t) * sd.o_tok + h * sd.o_head;
+  };
+  const int turn = kPair ? a.P / V : 2 * a.P / V;
+  const int n = nt * heads * turn;
   for (int i = threadIdx.x; i < nt * a.P; i += kRotThreads) {
     const int t = i / a.P, p = i - t * a.P;
     int ax = a.axis ? a.axis[p] : 0;
@@ -78,104 +91,62 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
     tab[i] = make_float2(fmaf(-lo, s, c) * a.scale, fmaf(lo, c, s) * a.scale * a.sign);
   }
   __syncthreads();
-  // turned units of V pairs, kUnroll at a time: their loads are on their way
-  // together
-  const int h0 = a.s[0].heads, heads = h0 + a.s[1].heads;
-  auto rows = [&](uint32_t th, const T*& x, T*& o, int& t) {
-    t = int(a.by_heads.div(th));
-    int h = int(th) - t * heads;
-    const bool second = h >= h0;
-    if (second) h -= h0;
-    const RotSide& sd = a.s[second ? 1 : 0];
-    x = static_cast<const T*>(sd.x) + (t0 + t) * sd.x_tok + h * sd.x_head;
-    o = static_cast<T*>(sd.out) + (t0 + t) * sd.o_tok + h * sd.o_head;
-  };
-  const int turn = a.P / V;
-  const int n = nt * heads * turn;
-  for (int i0 = threadIdx.x; i0 < n; i0 += kRotThreads * kUnroll) {
-    Vec<T, V> x0[kUnroll], x1[kUnroll];
-    T* o[kUnroll];
-    int at[kUnroll], e0[kUnroll];
+  for (int i = threadIdx.x; i < n; i += kRotThreads) {
+    const uint32_t th = a.by_turn.div(i);
+    const int u = i - int(th) * turn;
+    const T* x;
+    T* o;
+    int t;
+    rows(th, x, o, t);
+    const float2* cs = tab + t * a.P + (kPair ? u * V : u * V / 2);
+    const int e = kHalf ? u * V : V == 1 ? 2 * u : u * V;
+    x += e;
+    o += e;
+    if constexpr (kPair) {
+      const int gap = kHalf ? a.P : 1;
+      float p[V], q[V];
+      const Vec<T, V> v0 = ld_vec<T, V>(x), v1 = ld_vec<T, V>(x + gap);
+      widen<T, V>(v0, p);
+      widen<T, V>(v1, q);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int i = i0 + k * kRotThreads;
-      if (i < n) {
-        const uint32_t th = a.by_turn.div(i);
-        const int u = i - int(th) * turn;
-        const T* x;
-        int t;
-        rows(th, x, o[k], t);
-        at[k] = t * a.P + u * V;
-        e0[k] = a.half ? u * V : 2 * u * V;
-        x0[k] = ld_vec<T, V>(x + e0[k]);
-        x1[k] = ld_vec<T, V>(x + e0[k] + (a.half ? a.P : V));
+      for (int j = 0; j < V; ++j) {
+        const float2 w = cs[j];
+        const float re = p[j] * w.x - q[j] * w.y;
+        q[j] = p[j] * w.y + q[j] * w.x;
+        p[j] = re;
       }
-    }
+      st_vec<T, V>(o, narrow<T, V>(p));
+      st_vec<T, V>(o + gap, narrow<T, V>(q));
+    } else {
+      float f[V];
+      widen<T, V>(ld_vec<T, V>(x), f);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (i0 + k * kRotThreads >= n) break;
-      const float2* cs = tab + at[k];
-      Vec<T, V> y0, y1;
-      if (a.half) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float p = to_f32(x0[k].v[j]), q = to_f32(x1[k].v[j]);
-          const float2 w = cs[j];
-          y0.v[j] = from_f32<T>(p * w.x - q * w.y);
-          y1.v[j] = from_f32<T>(p * w.y + q * w.x);
-        }
-      } else {
-        T in[2 * V], r[2 * V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          in[j] = x0[k].v[j];
-          in[V + j] = x1[k].v[j];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float p = to_f32(in[2 * j]), q = to_f32(in[2 * j + 1]);
-          const float2 w = cs[j];
-          r[2 * j] = from_f32<T>(p * w.x - q * w.y);
-          r[2 * j + 1] = from_f32<T>(p * w.y + q * w.x);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          y0.v[j] = r[j];
-          y1.v[j] = r[V + j];
-        }
+      for (int j = 0; j < V; j += 2) {
+        const float2 w = cs[j / 2];
+        const float re = f[j] * w.x - f[j + 1] * w.y;
+        f[j + 1] = f[j] * w.y + f[j + 1] * w.x;
+        f[j] = re;
       }
-      st_vec<T, V>(o[k] + e0[k], y0);
-      st_vec<T, V>(o[k] + e0[k] + (a.half ? a.P : V), y1);
+      st_vec<T, V>(o, narrow<T, V>(f));
     }
   }
   // copied units of V elements
   const int rest = (a.D - 2 * a.P) / V;
   const int m = nt * heads * rest;
-  for (int i0 = threadIdx.x; i0 < m; i0 += kRotThreads * 2 * kUnroll) {
-    Vec<T, V> v[2 * kUnroll];
-    T* o[2 * kUnroll];
-#pragma unroll
-    for (int k = 0; k < 2 * kUnroll; ++k) {
-      const int i = i0 + k * kRotThreads;
-      if (i < m) {
-        const uint32_t th = a.by_rest.div(i);
-        const T* x;
-        int t;
-        rows(th, x, o[k], t);
-        const int e = 2 * a.P + (i - int(th) * rest) * V;
-        o[k] += e;
-        v[k] = ld_vec<T, V>(x + e);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 2 * kUnroll; ++k)
-      if (i0 + k * kRotThreads < m) st_vec<T, V>(o[k], v[k]);
+  for (int i = threadIdx.x; i < m; i += kRotThreads) {
+    const uint32_t th = a.by_rest.div(i);
+    const T* x;
+    T* y;
+    int t;
+    rows(th, x, y, t);
+    const int e = 2 * a.P + (i - int(th) * rest) * V;
+    st_vec<T, V>(y + e, ld_vec<T, V>(x + e));
   }
 }
 
 template <typename T, int V>
 bool rot_fits(const RotArgs& a) {
-  if (a.P % V || a.D % V) return false;
+  if ((a.half || V == 1 ? a.P : 2 * a.P) % V || a.D % V) return false;
   for (const RotSide& s : a.s) {
     if (s.heads == 0) continue;
     if (!vec_ok(s.x, s.x_tok, V, sizeof(T)) || !vec_ok(s.out, s.o_tok, V, sizeof(T)) ||
@@ -188,9 +159,13 @@ bool rot_fits(const RotArgs& a) {
 template <typename T, int V>
 void launch_rotary(RotArgs a, int64_t grid, cudaStream_t s) {
   a.by_heads = Div(uint32_t(a.s[0].heads + a.s[1].heads));
-  if (a.P >= V) a.by_turn = Div(uint32_t(a.P / V));
+  const int turn = (a.half || V == 1 ? a.P : 2 * a.P) / V;
+  if (turn > 0) a.by_turn = Div(uint32_t(turn));
   if (a.D - 2 * a.P >= V) a.by_rest = Div(uint32_t((a.D - 2 * a.P) / V));
-  rotary_kernel<T, V><<<int(grid), kRotThreads, 0, s>>>(a);
+  if (a.half)
+    rotary_kernel<T, V, true><<<int(grid), kRotThreads, 0, s>>>(a);
+  else
+    rotary_kernel<T, V, false><<<int(grid), kRotThreads, 0, s>>>(a);
 }
 
 template <typename T>

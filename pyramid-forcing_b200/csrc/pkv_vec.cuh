@@ -55,19 +55,6 @@ __device__ __forceinline__ void st_vec(T* p, const Vec<T, N>& v) {
   *reinterpret_cast<Vec<T, N>*>(p) = v;
 }
 
-// N consecutive elements as fp32, in accesses of up to 16 bytes (aligned to
-// that where N > 1).
-template <typename T, int N>
-__device__ __forceinline__ void ld_f32(const T* p, float (&f)[N]) {
-  constexpr int M = N * sizeof(T) > 16 ? int(16 / sizeof(T)) : N;
-#pragma unroll
-  for (int i = 0; i < N; i += M) {
-    const Vec<T, M> t = ld_vec<T, M>(p + i);
-#pragma unroll
-    for (int e = 0; e < M; ++e) f[i + e] = to_f32(t.v[e]);
-  }
-}
-
 // Asynchronous copy of N elements (4, 8 or 16 bytes) into shared memory.  A
 // thread that copies only what it reads itself needs no barrier: its own
 // wait_group orders the copy before its loads.
@@ -88,6 +75,72 @@ __device__ __forceinline__ void cp_commit() {
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two 16-bit elements of a word: one instruction a value to widen them (bf16
+// is the upper half of fp32), one to round a pair.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi);
+template <>
+__device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void unpack2<__half>(uint32_t w, float& lo, float& hi) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  const float2 f = __half22float2(h);
+  lo = f.x;
+  hi = f.y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A vector's elements as fp32, and fp32 rounded into a vector.
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Vec<T, N>& v, float* f) {
+  if constexpr (sizeof(T) == 2 && N >= 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) unpack2<T>(w[i], f[2 * i], f[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f32(v.v[i]);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> narrow(const float* f) {
+  Vec<T, N> v;
+  if constexpr (sizeof(T) == 2 && N >= 2) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(f[i]);
+  }
+  return v;
+}
+
+// N consecutive elements as fp32, in accesses of up to 16 bytes (aligned to
+// that where N > 1).
+template <typename T, int N>
+__device__ __forceinline__ void ld_f32(const T* p, float (&f)[N]) {
+  constexpr int M = N * sizeof(T) > 16 ? int(16 / sizeof(T)) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += M) {
+    widen<T, M>(ld_vec<T, M>(p + i), f + i);
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
