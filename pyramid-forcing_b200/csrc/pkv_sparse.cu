@@ -13,10 +13,10 @@
 //  * block_means_kernel -- one pass over K, bound by HBM.  Segment s's block j
 //    has row cu[s] / block + s + j of the table: a closed form, so the table
 //    needs no offsets of its own (ceil(n / B) <= floor((a + n) / B) - floor(a / B) + 1).
-//  * select_blocks_kernel -- a CTA a group.  Which block comes last is decided
-//    by the order of two scores, so sums are float64 (of bf16 terms: exact)
-//    and products of the fp32 means are exact before their float64 sum: the
-//    choice does not depend on the order of summation.
+//  * select_blocks_kernel -- scores in fp32 with a bound on their error; only
+//    blocks within that bound of the last place are scored again in float64
+//    (queries summed in float64, products of fp32 means exact before their
+//    float64 sum), so the lists are those of the definition.
 //  * attention over the listed blocks, by the rows of a group:
 //    up to 16 rows (a decoded token, a small group): warps each take 16 keys,
 //    K and V go from memory straight into mma fragments, a thread-block
@@ -150,18 +150,18 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
 }
 
 // Into the first CTA of the cluster.
-__device__ __forceinline__ void st_peer(uint64_t* p, uint64_t v) {
+__device__ __forceinline__ void st_first(float* p, float v) {
   uint32_t addr;
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(addr) : "r"(su32(p)));
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // ---------------------------------------------------------------------------
 // Selection
 // ---------------------------------------------------------------------------
 constexpr int kSelThreads = 256;
-constexpr int kSelChunk = 1024;  // scores added per round
-constexpr int kSelCluster = 8;   // most CTAs a group
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelCluster = 8;  // most CTAs a group
 
 struct SelectArgs {
   const uint16_t* q;
@@ -169,19 +169,17 @@ struct SelectArgs {
   const float* means;
   const int32_t* cu;
   int32_t* blocks;
-  int H, rows_per_chunk, groups, query_block, block, top_k;
+  int H, rows_per_chunk, groups, packs, query_block, block, top_k;
 };
 
-struct SelectSmem {
-  double red[kSelThreads / 32][128];  // the warps' query sums
-  double q[128];
-  int hist[256];
-  int wsum[2][kSelThreads / 32];
-  uint64_t prefix, lo, hi;
-  int need, done;
-  // [top_k + kSelChunk] keys, then as many ids: the kept blocks of earlier
-  // rounds, then this round's
-  uint64_t key[1];
+// Groups of a CTA, blocks scored per round, bytes of shared memory for top_k.
+template <int D, int GQ>
+struct SelectShape {
+  static constexpr int kChunk = GQ == 1 ? 1024 : 512;
+  static size_t bytes(int top_k) {
+    const size_t cap = size_t(top_k) + kChunk;
+    return sizeof(double) * (GQ + kSelWarps) * D + GQ * cap * 12 + size_t(GQ) * top_k * 4;
+  }
 };
 
 // Scores as integers in the same order; NaN below all, -0 as 0.
@@ -192,88 +190,165 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
-// A CTA a group, or a cluster whose CTAs share the scores and whose first
-// picks: with few groups (single tokens) the table of means is then read by
-// many SMs.
-template <int D>
-__global__ void __launch_bounds__(kSelThreads, 4) select_blocks_kernel(SelectArgs a) {
+// fp32 scores as integers in the same order (not NaN), and back.
+__device__ __forceinline__ uint32_t order_f32(float s) {
+  const uint32_t b = __float_as_uint(s + 0.0f);  // -0 as 0
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unorder_f32(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+// The k-th largest of n > k scores, by a warp: the bits below the highest in
+// which the scores differ, from the top, by counting.
+__device__ __forceinline__ float kth_score(const float* s, int n, int k) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kRegs = 16;
+  const int lane = threadIdx.x & 31;
+  uint32_t r[kRegs];
+  uint32_t mn = 0xffffffffu, mx = 0;
+  const bool held = n <= 32 * kRegs;  // the keys fit the warp's registers
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      r[i] = 0;
+      if (i * 32 + lane < n) {
+        r[i] = order_f32(s[i * 32 + lane]);
+        mn = min(mn, r[i]);
+        mx = max(mx, r[i]);
+      }
+    }
+  } else {
+    for (int i = lane; i < n; i += 32) {
+      const uint32_t key = order_f32(s[i]);
+      mn = min(mn, key);
+      mx = max(mx, key);
+    }
+  }
+  mn = __reduce_min_sync(kAll, mn);
+  mx = __reduce_max_sync(kAll, mx);
+  if (mn == mx) return unorder_f32(mx);
+  uint32_t bit = 1u << (31 - __clz(int(mn ^ mx)));
+  uint32_t prefix = mx & ~(bit | (bit - 1));
+  for (; bit != 0; bit >>= 1) {
+    const uint32_t cand = prefix | bit;
+    int c = 0;
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) c += r[i] >= cand;
+    } else {
+      for (int i = lane; i < n; i += 32) c += order_f32(s[i]) >= cand;
+    }
+    if (int(__reduce_add_sync(kAll, c)) >= k) prefix = cand;
+  }
+  return unorder_f32(prefix);
+}
+
+// A CTA GQ groups of a segment, which share the loads of its means; with few
+// groups (GQ = 1, single tokens) a cluster a group, whose CTAs share the
+// scores and whose first picks: the table is then read by many SMs.
+//
+// An fp32 score differs from the exact one by at most e = 2^-20 |q| |mean|
+// (q rounded once, D / 16 products a lane in a chain, 4 levels of adds: 13
+// roundings of 2^-24).  With T the top_k-th fp32 score, a block above T + 2 e
+// is in the list for certain and one below T - 2 e is not; those between are
+// scored in float64 and ranked, unless all of them are in.  Infinite or NaN
+// queries or means make every block such a one.
+template <int D, int GQ>
+__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a) {
+  constexpr int kChunk = SelectShape<D, GQ>::kChunk;
+  constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(16) uint8_t raw[];
-  SelectSmem& sm = *reinterpret_cast<SelectSmem*>(raw);
-  uint64_t* skey = sm.key;
-  int* sid = reinterpret_cast<int*>(skey + a.top_k + kSelChunk);
+  __shared__ float nmax[kSelCluster * kSelWarps];
+  const int cap = a.top_k + kChunk;
+  double* qs = reinterpret_cast<double*>(raw);               // [GQ][D] summed queries
+  double* red = qs + GQ * D;                                 // [warps][D]
+  uint64_t* exact = reinterpret_cast<uint64_t*>(red + kSelWarps * D);  // [GQ][cap]
+  float* score = reinterpret_cast<float*>(exact + GQ * cap);           // [GQ][cap]
+  int* kid = reinterpret_cast<int*>(score + GQ * cap);       // [GQ][top_k] earlier rounds' ids
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int X = int(cluster_size()), rank = int(cluster_rank());
   const int unit = blockIdx.x / X;
-  const int s = unit / a.groups, g = unit - s * a.groups;
+  const int s = unit / a.packs, g0 = (unit - s * a.packs) * GQ;
+  const int ng = min(GQ, a.groups - g0);
   const int c = s / a.H, h = s - c * a.H;
   const SegView sg = segment(a.cu, s, a.kv_rows);
   const int nblk = (sg.len + a.block - 1) / a.block;
-  int32_t* out = a.blocks + int64_t(unit) * a.top_k;
+  int32_t* out = a.blocks + (int64_t(s) * a.groups + g0) * a.top_k;  // ng lists
   if (nblk <= a.top_k) {  // every block is kept (the whole cluster leaves)
     if (rank == 0)
-      for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
+      for (int i = tid; i < ng * a.top_k; i += kSelThreads) {
+        const int j = i % a.top_k;
+        out[i] = j < nblk ? j : -1;
+      }
     return;
   }
-  // ---- sum of the group's queries, float64 (exact for bf16 of like size;
+  // ---- sums of the groups' queries in float64 (exact for bf16 of like size;
   // four rows are added in fp32 first, as block_means_kernel does) ----
-  const int r0 = g * a.query_block;
-  const int nr = min(a.query_block, a.rows_per_chunk - r0);
   {
-    constexpr int kLanes = D / 8, kRows = kSelThreads / kLanes;
-    const int sub = tid / kLanes, d0 = (tid % kLanes) * 8;
+    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / GQ;
+    const int g = warp / kWarps, w = warp - g * kWarps;
+    const int sub = w * kPerWarp + lane / kLanes, d0 = (lane % kLanes) * 8;
+    constexpr int kRows = kWarps * kPerWarp;
+    const int r0 = (g0 + g) * a.query_block;
+    const int nr = g < ng ? min(a.query_block, a.rows_per_chunk - r0) : 0;
     const uint16_t* p =
         a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
     double acc[8] = {};
-    for (int r = sub; r < nr; r += 4 * kRows) {
-      uint4 w[4];
+    for (int r = sub; r < nr; r += 8 * kRows) {
+      uint4 v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = r + i * kRows < nr
+      for (int i = 0; i < 8; ++i)
+        v[i] = r + i * kRows < nr
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs))
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float lo4[4], hi4[4];
+      for (int i = 0; i < 8; i += 4)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u = word(w[i], e);
-          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
-          hi4[i] = __uint_as_float(u & 0xffff0000u);
+        for (int e = 0; e < 4; ++e) {
+          float lo4[4], hi4[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t u = word(v[i + x], e);
+            lo4[x] = bf16_bits_to_f32(u & 0xffffu);
+            hi4[x] = __uint_as_float(u & 0xffff0000u);
+          }
+          acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
+          acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
         }
-        acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
-        acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
-      }
     }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+      for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(kAll, acc[e], o);
     if (lane < kLanes)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sm.red[warp][d0 + e] = acc[e];
+      for (int e = 0; e < 8; ++e) red[warp * D + d0 + e] = acc[e];
     __syncthreads();
-    if (tid < D) {
+    for (int i = tid; i < GQ * D; i += kSelThreads) {
       double t = 0.0;
 #pragma unroll
-      for (int i = 0; i < kSelThreads / 32; ++i) t += sm.red[i][tid];
-      sm.q[tid] = t;
+      for (int x = 0; x < kWarps; ++x) t += red[(i / D * kWarps + x) * D + i % D];
+      qs[i] = t;
     }
     __syncthreads();
   }
-  // ---- scores: 16 lanes a block, D / 16 products each; 4 blocks on their way ----
-  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = 4;
+  // ---- rounds of scores: 16 lanes a block, D / 16 products a lane ----
+  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = GQ == 1 ? 4 : 2;
   const int l16 = tid & 15;
-  double q[kPer];
+  float q[GQ][kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) q[i] = sm.q[(i / 4) * 64 + l16 * 4 + (i & 3)];
+  for (int g = 0; g < GQ; ++g)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) q[g][i] = float(qs[g * D + (i / 4) * 64 + l16 * 4 + (i & 3)]);
   const int64_t base = int64_t(a.cu[s]) / a.block + s;
   const int stride = X * (kSelThreads / 16);
   int kept = 0;
+  float most = 0.0f;              // largest |mean|^2 that this warp has seen
   if (X > 1) cluster_barrier();  // the first CTA runs: its memory may be written
-  for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
-    const int m = min(kSelChunk, nblk - b0);
-    uint64_t mn = ~uint64_t(0), mx = 0;
-    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kSelChunk; i0 += stride * kBatch) {
+  for (int b0 = 0; b0 < nblk; b0 += kChunk) {
+    const int m = min(kChunk, nblk - b0);
+    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kChunk; i0 += stride * kBatch) {
       if (i0 - (lane >> 4) >= m) break;  // (the whole warp)
       float4 f[kBatch][kVec];
 #pragma unroll
@@ -288,147 +363,148 @@ __global__ void __launch_bounds__(kSelThreads, 4) select_blocks_kernel(SelectArg
       }
 #pragma unroll
       for (int x = 0; x < kBatch; ++x) {
-        double t = 0.0;
+        float t[GQ + 1];
+#pragma unroll
+        for (int g = 0; g <= GQ; ++g) t[g] = 0.0f;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          t = fma(double(f[x][e].x), q[4 * e], t);
-          t = fma(double(f[x][e].y), q[4 * e + 1], t);
-          t = fma(double(f[x][e].z), q[4 * e + 2], t);
-          t = fma(double(f[x][e].w), q[4 * e + 3], t);
+          const float v[4] = {f[x][e].x, f[x][e].y, f[x][e].z, f[x][e].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int g = 0; g < GQ; ++g) t[g] = fmaf(v[i], q[g][4 * e + i], t[g]);
+            t[GQ] = fmaf(v[i], v[i], t[GQ]);
+          }
         }
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+          for (int g = 0; g <= GQ; ++g) t[g] += __shfl_xor_sync(kAll, t[g], o);
+        most = t[GQ] < INFINITY ? fmaxf(most, t[GQ]) : INFINITY;
         const int i = i0 + x * stride;
-        if (i < m && l16 == 0) {
-          st_peer(&skey[kept + i], order_key(t));
+        if (i < m) {
+#pragma unroll
+          for (int g = 0; g < GQ; ++g)
+            if (l16 == g) st_first(&score[g * cap + kept + i], t[g]);
         }
       }
     }
-    if (rank == 0)
-      for (int i = tid; i < m; i += kSelThreads) sid[kept + i] = b0 + i;
+    const float both = fmaxf(most, __shfl_xor_sync(kAll, most, 16));
+    if (lane == 0) st_first(&nmax[rank * kSelWarps + warp], both);
     if (X > 1)
       cluster_barrier();  // every score is in the first CTA's memory
     else
       __syncthreads();
     const int total = kept + m;
     const bool last = b0 + m == nblk;
-    if (rank != 0) {
-      if (last) return;
-      kept = min(total, a.top_k);
-      cluster_barrier();  // the first CTA has picked: its memory may be written
-      continue;
-    }
-    if (total <= a.top_k) {  // (not the last round: nblk > top_k)
-      kept = total;
-      if (X > 1) cluster_barrier();
-      continue;
-    }
-    // ---- the top_k-th key: digits of 8 bits from the highest that differs ----
-    for (int i = tid; i < total; i += kSelThreads) {
-      mn = min(mn, skey[i]);
-      mx = max(mx, skey[i]);
-    }
+    if (rank != 0 && last) return;
+    if (rank == 0 && total > a.top_k && warp < ng) {
+      // ---- pick: a warp a group ----
+      const float* sc = score + warp * cap;
+      uint64_t* ex = exact + warp * cap;
+      int* kd = kid + warp * a.top_k;
+      const double* qg = qs + warp * D;
+      double qn = 0.0;
+      for (int d = lane; d < D; d += 32) qn = fma(qg[d], qg[d], qn);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    if (tid == 0) {
-      sm.lo = ~uint64_t(0);
-      sm.hi = 0;
-    }
-    __syncthreads();
-    if (lane == 0) {
-      atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), mn);
-      atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), mx);
-    }
-    __syncthreads();
-    mn = sm.lo;
-    mx = sm.hi;
-    int shift = mn == mx ? 0 : 64 - __clzll(mn ^ mx);  // bits below `shift` differ
-    uint64_t prefix = shift == 64 ? 0 : mx >> shift;
-    int need = a.top_k;
-    bool exact = false;  // every key with the prefix is kept
-    while (shift > 0 && !exact) {
-      const int bits = min(8, shift);
-      shift -= bits;
-      for (int i = tid; i < 256; i += kSelThreads) sm.hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < total; i += kSelThreads) {
-        const uint64_t key = skey[i];
-        const uint64_t up = shift + bits == 64 ? 0 : key >> (shift + bits);
-        if (up == prefix) atomicAdd(&sm.hist[int(key >> shift) & ((1 << bits) - 1)], 1);
+      for (int o = 16; o > 0; o >>= 1) qn += __shfl_xor_sync(kAll, qn, o);
+      float mm = 0.0f;
+      for (int i = lane; i < X * kSelWarps; i += 32) mm = fmaxf(mm, nmax[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
+      // 2.25 e, rounded up; the addend covers products that underflow
+      const float e2 = 2.25f * 9.5367431640625e-7f * 1.001f * float(sqrt(qn)) * sqrtf(mm) + 1e-36f;
+      const bool all = !(e2 < INFINITY);
+      float lo = 0.0f, hi = 0.0f;
+      if (!all) {
+        const float T = kth_score(sc, total, a.top_k);
+        lo = T - e2;
+        hi = T + e2;
       }
-      __syncthreads();
-      if (warp == 0) {
-        // lane owns bins 255 - 8 lane .. 248 - 8 lane: a scan from the top
-        int cnt[8], sum = 0;
+      int sure = 0, near = 0;
+      for (int i = lane; i < total; i += 32) {
+        sure += !all && sc[i] > hi;
+        near += all || (sc[i] >= lo && sc[i] <= hi);
+      }
+      sure = __reduce_add_sync(kAll, sure);
+      near = __reduce_add_sync(kAll, near);
+      const int need = a.top_k - sure;
+      if (near > need) {  // float64 scores of the near ones
+        for (int t0 = 0; t0 < total; t0 += 32) {
+          const int i = t0 + lane;
+          const bool is = i < total && (all || (sc[i] >= lo && sc[i] <= hi));
+          uint32_t todo = __ballot_sync(kAll, is);
+          while (todo) {
+            const int j = t0 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
+            double t = 0.0;
+            if (row >= 0 && row < a.means_rows)
+              for (int d = lane; d < D; d += 32)
+                t = fma(double(__ldg(a.means + row * D + d)), qg[d], t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += cnt[i] = sm.hist[255 - 8 * lane - i];
-        int before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += y;
-        }
-        before -= sum;
-        if (before < need && before + sum >= need) {
-          int acc = before;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (acc < need && acc + cnt[i] >= need) {
-              sm.prefix = (prefix << bits) | uint64_t(255 - 8 * lane - i);
-              sm.need = need - acc;
-              sm.done = cnt[i] == need - acc;
-            }
-            acc += cnt[i];
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kAll, t, o);
+            if (lane == 0) ex[j] = order_key(t);
           }
         }
+        __syncwarp();
       }
-      __syncthreads();
-      prefix = sm.prefix;
-      need = sm.need;
-      exact = sm.done != 0;
-      __syncthreads();
-    }
-    // ---- keep: above the prefix, and the first `need` at it, in index order ----
-    int eq_seen = 0, written = 0;
-    for (int t0 = 0; t0 < total; t0 += kSelThreads) {
-      const int i = t0 + tid;
-      const uint64_t key = i < total ? skey[i] : 0;
-      const int id = i < total ? sid[i] : 0;
-      const uint64_t up = shift == 64 ? 0 : key >> shift;
-      const bool gt = i < total && up > prefix, eq = i < total && up == prefix;
-      const uint32_t be = __ballot_sync(0xffffffffu, eq);
-      if (lane == 0) sm.wsum[0][warp] = __popc(be);
-      __syncthreads();
-      int er = eq_seen + __popc(be & ((1u << lane) - 1));
-      for (int w = 0; w < kSelThreads / 32; ++w) {
-        if (w < warp) er += sm.wsum[0][w];
-        eq_seen += sm.wsum[0][w];
-      }
-      const bool keep = gt || (eq && er < need);
-      const uint32_t bk = __ballot_sync(0xffffffffu, keep);
-      if (lane == 0) sm.wsum[1][warp] = __popc(bk);
-      __syncthreads();
-      int at = written + __popc(bk & ((1u << lane) - 1));
-      for (int w = 0; w < kSelThreads / 32; ++w) {
-        if (w < warp) at += sm.wsum[1][w];
-        written += sm.wsum[1][w];
-      }
-      // at <= i, and every key of this tile is in registers: in place
-      if (keep && at < a.top_k) {
-        if (last)
-          out[at] = id;
-        else {
-          skey[at] = key;
-          sid[at] = id;
+      // ---- which to keep: a near one by its rank among the near.  Lane t
+      // holds the flags of the 32 blocks of tiles t and t + 32 ----
+      uint32_t flags[2] = {0, 0};
+      for (int t0 = 0; t0 < total; t0 += 32) {
+        const int i = t0 + lane;
+        const float v = i < total ? sc[i] : 0.0f;
+        const bool is = i < total && (all || (v >= lo && v <= hi));
+        bool keep = i < total && !all && v > hi;
+        if (near <= need) {
+          keep = keep || is;
+        } else {
+          uint32_t todo = __ballot_sync(kAll, is);
+          while (todo) {
+            const int j = t0 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            const uint64_t mine = ex[j];
+            int ahead = 0;
+            for (int x = lane; x < total; x += 32)
+              if (all || (sc[x] >= lo && sc[x] <= hi))
+                ahead += ex[x] > mine || (ex[x] == mine && x < j);
+            ahead = __reduce_add_sync(kAll, ahead);
+            if (i == j) keep = ahead < need;
+          }
         }
+        const uint32_t kb = __ballot_sync(kAll, keep);
+        if (lane == ((t0 >> 5) & 31)) (t0 < 1024 ? flags[0] : flags[1]) = kb;
       }
-      __syncthreads();
+      // ---- move them up, in index order ----
+      int at = 0;
+      for (int t0 = 0; t0 < total; t0 += 32) {
+        const int i = t0 + lane;
+        const uint32_t kb = __shfl_sync(kAll, t0 < 1024 ? flags[0] : flags[1], (t0 >> 5) & 31);
+        const float v = i < total ? sc[i] : 0.0f;
+        const int id = i < total ? (i < kept ? kd[i] : b0 + i - kept) : 0;
+        __syncwarp();
+        if ((kb >> lane) & 1) {
+          const int to = at + __popc(kb & ((1u << lane) - 1));
+          if (last) {
+            out[warp * a.top_k + to] = id;
+          } else {
+            score[warp * cap + to] = v;
+            kd[to] = id;
+          }
+        }
+        __syncwarp();
+        at += __popc(kb);
+      }
+    } else if (rank == 0 && warp < ng) {
+      for (int i = lane; i < m; i += 32) kid[warp * a.top_k + kept + i] = b0 + i;
     }
-    kept = a.top_k;
-    if (X > 1 && !last) cluster_barrier();
+    kept = min(total, a.top_k);
+    if (last) return;
+    if (X > 1)
+      cluster_barrier();  // the first CTA has picked: its memory may be written
+    else
+      __syncthreads();
   }
 }
 
@@ -679,31 +755,53 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 // ---------------------------------------------------------------------------
 // Attention of 128-row tiles on tcgen05
 // ---------------------------------------------------------------------------
-// One CTA a (segment, group): Q tile, one K and one V buffer of 128 keys (two
-// listed 64-key halves a step), S / P and O in TMEM; two CTAs share an SM, so
-// one's softmax runs while the tensor pipe works for the other.  Warp 0 loads
-// (TMA), warp 1 issues the MMAs, warps 2-5 are the softmax (thread = row).
-//   K(j+1) loads once Q.K(j) has committed (during softmax j), V(j+1) once
-//   P.V(j) has; both have a whole softmax to arrive in, so one buffer of each
-//   suffices and two CTAs fit an SM.
-// The tensor pipe runs a CTA's MMAs in issue order, so Q.K(j+1), which
-// overwrites P(j), follows P.V(j), and S(j+1) seen means O is complete.
-// Rows of V behind a segment's end (or of a half that is not there) are
-// zeroed in shared memory: their weights are 0, but 0 * inf would not be.
+// One CTA a (segment, group); a step is one listed half block of 64 keys.  Two
+// K and two V buffers, two S buffers of 64 columns in TMEM (P overwrites its S
+// as bf16 pairs) and O: 256 columns, so two CTAs share an SM.  Warp 0 loads
+// (TMA), warp 1 issues the MMAs in the order
+//   QK(0) QK(1) | PV(0) QK(2) | PV(1) QK(3) | ...
+// and warps 2-5 are the softmax (thread = row = TMEM lane).  S(j+1) is ready
+// while the softmax of step j runs, so the softmax warps, of two CTAs a
+// scheduler, never wait for the tensor pipe but at the ends.
+//   The tensor pipe runs a CTA's MMAs in issue order: QK(j+2), which overwrites
+// P(j), follows PV(j).  PV(j) runs during the softmax of j + 1, so a row whose
+// maximum grew waits for PV(j) before it rescales O.
+//   K buffer j & 1 is free once S(j) has committed, V buffer j & 1 once PV(j)
+// has: their next loads have a step and a half to arrive in.
+//   Rows of V behind a segment's end are zeroed in shared memory: their weights
+// are 0, but 0 * inf would not be.
 constexpr int kTcThreads = 192;
+constexpr int kStepKeys = 64;
 constexpr int kMaxHalves = 2 * kMaxTopK;
-constexpr int kAhead = 2;  // steps whose keys are pulled into L2 ahead of their loads
 
 template <int D>
 struct __align__(1024) SparseTcSmem {
   uint8_t q[kBM * D * 2];
-  uint8_t k[kBN * D * 2];
-  uint8_t v[kBN * D * 2];
-  uint64_t q_full, k_full, v_full, s_full, p_full, pv_done, drain;
+  uint8_t k[2][kStepKeys * D * 2];
+  uint8_t v[2][kStepKeys * D * 2];
+  uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], drain;
   uint32_t tmem_base;
   int abort, halves;
   int list[kMaxHalves];
 };
+
+// Row max over 64 raw scores held as bits.
+__device__ __forceinline__ float row_max64(const uint32_t (&s)[2][32]) {
+  float m[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    float a[11];
+#pragma unroll
+    for (int i = 0; i < 10; ++i)
+      a[i] = max3(__uint_as_float(s[q][3 * i]), __uint_as_float(s[q][3 * i + 1]),
+                  __uint_as_float(s[q][3 * i + 2]));
+    a[10] = fmaxf(__uint_as_float(s[q][30]), __uint_as_float(s[q][31]));
+    const float b0 = max3(a[0], a[1], a[2]), b1 = max3(a[3], a[4], a[5]);
+    const float b2 = max3(a[6], a[7], a[8]), b3 = fmaxf(a[9], a[10]);
+    m[q] = fmaxf(max3(b0, b1, b2), b3);
+  }
+  return fmaxf(m[0], m[1]);
+}
 
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 2)
@@ -713,9 +811,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   SparseTcSmem<D>& sm = *reinterpret_cast<SparseTcSmem<D>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kCols = D / 64;                  // 64-column halves of a row
-  constexpr uint32_t kColBytes = kBM * 64 * 2;   // one of them, 128 rows
-  constexpr uint32_t kHalfKeys = 64 * 64 * 2;    // 64 keys of one of them
+  constexpr int kCols = D / 64;                    // 64-column halves of a row
+  constexpr uint32_t kQCol = kBM * 64 * 2;         // one of them, 128 query rows
+  constexpr uint32_t kKCol = kStepKeys * 64 * 2;   // one of them, 64 keys
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   const int unit = blockIdx.x;
@@ -728,11 +826,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   if (threadIdx.x == 0) {
     sm.abort = 0;
     mbar_init(&sm.q_full, 1);
-    mbar_init(&sm.k_full, 1);
-    mbar_init(&sm.v_full, 1);
-    mbar_init(&sm.s_full, 1);
-    mbar_init(&sm.p_full, 4);
-    mbar_init(&sm.pv_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 4);
+      mbar_init(&sm.pv_done[i], 1);
+    }
     mbar_init(&sm.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -766,8 +866,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem_base;
-  const int nh = sm.halves, steps = (nh + 1) >> 1;
+  const uint32_t tmem = sm.tmem_base;  // S0 | S1 | O: 64 + 64 + D columns
+  const int steps = sm.halves;
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -776,94 +876,87 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const int row0 = ch * a.rows_per_chunk + r0;
 #pragma unroll
       for (int x = 0; x < kCols; ++x)
-        tma_load_3d(sm.q + x * kColBytes, &tm_q, &sm.q_full, 64 * x, h, row0);
-      // keys of the next steps go to L2 while this one's are in use: a list
-      // jumps about, so its loads would each wait for HBM
-      auto pull = [&](int i) {
-        if (i >= nh) return;
-        const int y = sg.start + sm.list[i] * 64;
-#pragma unroll
-        for (int x = 0; x < kCols; ++x) {
-          tma_prefetch_2d(&tm_k, 64 * x, y);
-          tma_prefetch_2d(&tm_v, 64 * x, y);
-        }
-      };
-      for (int i = 0; i < 2 * kAhead; ++i) pull(2 + i);
+        tma_load_3d(sm.q + x * kQCol, &tm_q, &sm.q_full, 64 * x, h, row0);
       int kj = 0, vj = 0;  // loads issued
       for (int j = 0; j < steps; ++j) {
-        const int here = 2 * j + 1 < nh ? 2 : 1;
-        const int y0 = sg.start + sm.list[2 * j] * 64;
-        const int y1 = here == 2 ? sg.start + sm.list[2 * j + 1] * 64 : 0;
-        if (j > 0 && !mbar_wait(&sm.s_full, (j - 1) & 1, abort, a.status)) break;
-        mbar_expect_tx(&sm.k_full, here * kHalfKeys * kCols);
+        const int b = j & 1;
+        const uint32_t prev = ((j >> 1) + 1) & 1;  // parity of step j - 2
+        const int y = sg.start + sm.list[j] * kStepKeys;
+        if (j > 1 && !mbar_wait(&sm.s_full[b], prev, abort, a.status)) break;
+        mbar_expect_tx(&sm.k_full[b], kKCol * kCols);
 #pragma unroll
-        for (int x = 0; x < kCols; ++x) {
-          tma_load_2d(sm.k + x * kColBytes, &tm_k, &sm.k_full, 64 * x, y0);
-          if (here == 2) tma_load_2d(sm.k + x * kColBytes + kHalfKeys, &tm_k, &sm.k_full, 64 * x, y1);
-        }
+        for (int x = 0; x < kCols; ++x)
+          tma_load_2d(sm.k[b] + x * kKCol, &tm_k, &sm.k_full[b], 64 * x, y);
         ++kj;
-        if (j > 0 && !mbar_wait(&sm.pv_done, (j - 1) & 1, abort, a.status)) break;
-        mbar_expect_tx(&sm.v_full, here * kHalfKeys * kCols);
+        if (j > 1 && !mbar_wait(&sm.pv_done[b], prev, abort, a.status)) break;
+        mbar_expect_tx(&sm.v_full[b], kKCol * kCols);
 #pragma unroll
-        for (int x = 0; x < kCols; ++x) {
-          tma_load_2d(sm.v + x * kColBytes, &tm_v, &sm.v_full, 64 * x, y0);
-          if (here == 2) tma_load_2d(sm.v + x * kColBytes + kHalfKeys, &tm_v, &sm.v_full, 64 * x, y1);
-        }
+        for (int x = 0; x < kCols; ++x)
+          tma_load_2d(sm.v[b] + x * kKCol, &tm_v, &sm.v_full[b], 64 * x, y);
         ++vj;
-        pull(2 * (j + 1 + kAhead));
-        pull(2 * (j + 1 + kAhead) + 1);
       }
       if (*abort) {  // this CTA's own copies land before its memory goes away
         const uint64_t t0 = now_ns();
         while (!mbar_try(&sm.q_full, 0) && now_ns() - t0 < kTimeoutNs) {
         }
-        while (kj > 0 && !mbar_try(&sm.k_full, (kj - 1) & 1) && now_ns() - t0 < kTimeoutNs) {
-        }
-        while (vj > 0 && !mbar_try(&sm.v_full, (vj - 1) & 1) && now_ns() - t0 < kTimeoutNs) {
-        }
+        for (int j = kj > 2 ? kj - 2 : 0; j < kj; ++j)
+          while (!mbar_try(&sm.k_full[j & 1], (j >> 1) & 1) && now_ns() - t0 < kTimeoutNs) {
+          }
+        for (int j = vj > 2 ? vj - 2 : 0; j < vj; ++j)
+          while (!mbar_try(&sm.v_full[j & 1], (j >> 1) & 1) && now_ns() - t0 < kTimeoutNs) {
+          }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0 && steps > 0) {
-      constexpr uint32_t id_qk = idesc_bf16(false);
-      constexpr uint32_t id_pv =
-          (idesc_bf16(true) & ~(uint32_t(kBN >> 3) << 17)) | (uint32_t(D >> 3) << 17);
+      constexpr uint32_t kN = uint32_t(kBN >> 3) << 17;  // N of idesc_bf16
+      constexpr uint32_t id_qk = (idesc_bf16(false) & ~kN) | (uint32_t(kStepKeys >> 3) << 17);
+      constexpr uint32_t id_pv = (idesc_bf16(true) & ~kN) | (uint32_t(D >> 3) << 17);
       const uint64_t dq = sdesc_sw128(su32(sm.q), 16, 1024);
-      const uint64_t dk = sdesc_sw128(su32(sm.k), 16, 1024);
-      const uint64_t dv = sdesc_sw128(su32(sm.v), kColBytes, 1024);
+      const uint64_t dv = sdesc_sw128(su32(sm.v[0]), kKCol, 1024);
       const uint32_t d_hi = uint32_t(dq >> 32), v_hi = uint32_t(dv >> 32);
-      const uint32_t q_lo = uint32_t(dq), k_lo = uint32_t(dk), v_lo = uint32_t(dv);
-      auto issue_qk = [&]() {
+      const uint32_t q_lo = uint32_t(dq), v_lo0 = uint32_t(dv);
+      const uint32_t v_lo1 = uint32_t(sdesc_sw128(su32(sm.v[1]), kKCol, 1024));
+      const uint32_t k_lo0 = uint32_t(sdesc_sw128(su32(sm.k[0]), 16, 1024));
+      const uint32_t k_lo1 = uint32_t(sdesc_sw128(su32(sm.k[1]), 16, 1024));
+      auto issue_qk = [&](int b) {
+        const uint32_t k_lo = b ? k_lo1 : k_lo0;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * kColBytes + (kk & 3) * 32) >> 4;
-          mma_ss(tmem, (uint64_t(d_hi) << 32) | (q_lo + off), (uint64_t(d_hi) << 32) | (k_lo + off),
-                 id_qk, kk > 0 ? 1u : 0u);
+          const uint32_t qo = ((kk >> 2) * kQCol + (kk & 3) * 32) >> 4;
+          const uint32_t ko = ((kk >> 2) * kKCol + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + b * 64, (uint64_t(d_hi) << 32) | (q_lo + qo),
+                 (uint64_t(d_hi) << 32) | (k_lo + ko), id_qk, kk > 0 ? 1u : 0u);
         }
-        tc_commit(&sm.s_full);
+        tc_commit(&sm.s_full[b]);
       };
-      bool ok = mbar_wait(&sm.q_full, 0, abort, a.status) &&
-                mbar_wait(&sm.k_full, 0, abort, a.status);
-      if (ok) {
-        tc_fence_after();
-        issue_qk();
-      }
-      for (int j = 0; ok && j < steps; ++j) {
-        ok = mbar_wait(&sm.v_full, j & 1, abort, a.status) &&
-             mbar_wait(&sm.p_full, j & 1, abort, a.status);
+      bool ok = mbar_wait(&sm.q_full, 0, abort, a.status);
+      for (int j = 0; ok && j < 2 && j < steps; ++j) {
+        ok = mbar_wait(&sm.k_full[j], 0, abort, a.status);
         if (!ok) break;
         tc_fence_after();
+        issue_qk(j);
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        const int b = j & 1;
+        const uint32_t par = (j >> 1) & 1;
+        ok = mbar_wait(&sm.v_full[b], par, abort, a.status) &&
+             mbar_wait(&sm.p_full[b], par, abort, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_lo = b ? v_lo1 : v_lo0;
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          mma_ts(tmem + 128, tmem + kk * 8, (uint64_t(v_hi) << 32) | (v_lo + ((kk * 2048) >> 4)),
-                 id_pv, (kk > 0 || j > 0) ? 1u : 0u);
-        tc_commit(&sm.pv_done);
-        if (j + 1 < steps) {
-          ok = mbar_wait(&sm.k_full, (j + 1) & 1, abort, a.status);
+        for (int kk = 0; kk < kStepKeys / 16; ++kk)
+          mma_ts(tmem + 128, tmem + b * 64 + kk * 8,
+                 (uint64_t(v_hi) << 32) | (v_lo + ((kk * 2048) >> 4)), id_pv,
+                 (kk > 0 || j > 0) ? 1u : 0u);
+        tc_commit(&sm.pv_done[b]);
+        if (j + 2 < steps) {
+          ok = mbar_wait(&sm.k_full[b], par ^ 1, abort, a.status);
           if (!ok) break;
           tc_fence_after();
-          issue_qk();
+          issue_qk(b);
         }
       }
       // every MMA issued here completes before the CTA frees TMEM
@@ -877,58 +970,60 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
-    const uint32_t s_tm = tmem + lane_off, o_tm = tmem + 128 + lane_off;
+    const uint32_t o_tm = tmem + 128 + lane_off;
     const float sc = a.scale_log2;
     float m_ref = -INFINITY, l_sum = 0.0f;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
-      const int v0 = min(64, sg.len - sm.list[2 * j] * 64);  // keys of the halves
-      const int v1 = 2 * j + 1 < nh ? min(64, sg.len - sm.list[2 * j + 1] * 64) : 0;
-      const bool partial = v0 < 64 || v1 < 64;
-      if (!mbar_wait(&sm.s_full, j & 1, abort, a.status)) {
+      const int b = j & 1;
+      const uint32_t par = (j >> 1) & 1;
+      const uint32_t s_tm = tmem + b * 64 + lane_off;
+      const int valid = sg.len - sm.list[j] * kStepKeys;  // keys inside the segment
+      const bool partial = valid < kStepKeys;
+      if (!mbar_wait(&sm.s_full[b], par, abort, a.status)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      uint32_t sr[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(s_tm + q * 32, sr[q]);
+      uint32_t sr[2][32];
+      tmem_ld32(s_tm, sr[0]);
+      tmem_ld32(s_tm + 32, sr[1]);
       tmem_wait_ld();
       if (partial) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((q & 1) * 32 + e >= (q < 2 ? v0 : v1)) sr[q][e] = __float_as_uint(-INFINITY);
-        // zero this thread's row of V when it holds no key
-        if (!mbar_wait(&sm.v_full, j & 1, abort, a.status)) {
+            if (q * 32 + e >= valid) sr[q][e] = __float_as_uint(-INFINITY);
+        if (!mbar_wait(&sm.v_full[b], par, abort, a.status)) {
           ok = false;
           break;
         }
-        if ((row & 63) >= (row < 64 ? v0 : v1)) {
+        if (row < kStepKeys && row >= valid) {  // this row of V holds no key
 #pragma unroll
           for (int x = 0; x < kCols; ++x)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(sm.v + x * kColBytes + row * 128 + e * 16) =
+              *reinterpret_cast<uint4*>(sm.v[b] + x * kKCol + row * 128 + e * 16) =
                   make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
       }
-      const float m_new = fmaxf(m_ref, row_max128(sr) * sc);
+      const float m_new = fmaxf(m_ref, row_max64(sr) * sc);
       const bool grow = m_new > m_ref + kRescaleThreshold || j == 0;
       float alpha = 1.0f;
       if (grow) {
         alpha = (j == 0 || m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
         m_ref = m_new;
       }
+      // a row whose scores are all -inf keeps a reference of 0
       const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
       const f2 scale2 = mk2(sc, sc), negm2 = mk2(-m_use, -m_use);
-      f2 acc[8];
+      f2 acc[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = mk2(0.0f, 0.0f);
+      for (int i = 0; i < 4; ++i) acc[i] = mk2(0.0f, 0.0f);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
         uint32_t pr[16];
         if (partial)
           softmax_chunk<false>(sr[q], scale2, negm2, acc[2 * q], acc[2 * q + 1], pr);
@@ -936,13 +1031,17 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           softmax_chunk<true>(sr[q], scale2, negm2, acc[2 * q], acc[2 * q + 1], pr);
         tmem_st16(s_tm + q * 16, pr);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], acc[i + 4]);
       acc[0] = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
       float e0, e1;
       un2(acc[0], e0, e1);
       l_sum = l_sum * alpha + (e0 + e1);
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        // PV(j - 1) may still be running
+        if (!mbar_wait(&sm.pv_done[b ^ 1], ((j - 1) >> 1) & 1, abort, a.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
           uint32_t orr[32];
@@ -956,7 +1055,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full);
+      if (lane == 0) mbar_arrive(&sm.p_full[b]);
     }
     uint16_t* dst = a.out + (int64_t(ch) * a.rows_per_chunk + r0 + row) * a.o_rs +
                     int64_t(h) * a.o_hs;
@@ -964,7 +1063,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (row < nr)
         for (int e = 0; e < D; e += 8)
           *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
-    } else if (ok && mbar_wait(&sm.pv_done, (steps - 1) & 1, abort, a.status)) {
+    } else if (ok && mbar_wait(&sm.pv_done[(steps - 1) & 1], ((steps - 1) >> 1) & 1, abort,
+                               a.status)) {
       tc_fence_after();
       const float inv = l_sum > 0.0f ? 1.0f / l_sum : (l_sum == 0.0f ? 0.0f : l_sum);
 #pragma unroll
@@ -1015,22 +1115,35 @@ int launch_cluster(void (*kernel)(A), const A& a, int64_t units, int X, int thre
   return PKV_OK;
 }
 
-template <int D>
-int launch_select(const SelectArgs& a, int64_t units, cudaStream_t stream) {
-  const size_t most = sizeof(SelectSmem) + size_t(kMaxTopK + kSelChunk) * 12;
-  const size_t smem = sizeof(SelectSmem) + size_t(a.top_k + kSelChunk) * 12;
+template <int D, int GQ>
+int select_shape(SelectArgs a, int64_t segs, cudaStream_t stream) {
+  using Shape = SelectShape<D, GQ>;
+  static_assert(Shape::kChunk + kMaxTopK <= 2048, "a lane holds the flags of two tiles");
   static std::mutex mu;
   static int done[kMaxDevices] = {};
-  if (smem_opt_in(done, mu, select_blocks_kernel<D>, most) <= 0) {
+  if (smem_opt_in(done, mu, select_blocks_kernel<D, GQ>, Shape::bytes(kMaxTopK)) <= 0) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
+  a.packs = (a.groups + GQ - 1) / GQ;
+  const int64_t units = segs * a.packs;
   // a cluster while the groups leave SMs idle and the keys could make blocks
-  // enough to share (16 a round and CTA)
+  // enough to share
   int X = 1;
   const int64_t blocks = a.kv_rows / a.block;
-  while (X < kSelCluster && units * X * 2 <= sm_count() && blocks >= int64_t(X) * 64) X *= 2;
-  return launch_cluster(select_blocks_kernel<D>, a, units, X, kSelThreads, smem, stream);
+  if (GQ == 1)
+    while (X < kSelCluster && units * X * 2 <= sm_count() && blocks >= int64_t(X) * 64) X *= 2;
+  return launch_cluster(select_blocks_kernel<D, GQ>, a, units, X, kSelThreads,
+                        Shape::bytes(a.top_k), stream);
+}
+
+// Four groups share a segment's means where that still leaves a CTA for most
+// SMs.
+template <int D>
+int launch_select(const SelectArgs& a, int64_t segs, cudaStream_t stream) {
+  if (a.groups >= 4 && segs * ((a.groups + 3) / 4) * 4 >= int64_t(sm_count()) * 3)
+    return select_shape<D, 4>(a, segs, stream);
+  return select_shape<D, 1>(a, segs, stream);
 }
 
 template <int D>
@@ -1143,11 +1256,10 @@ extern "C" int pkv_select_blocks(const uint16_t* q, int64_t q_row_stride, int64_
   a.query_block = query_block;
   a.block = block;
   a.top_k = top_k;
-  const int64_t grid = int64_t(num_chunks) * num_heads * a.groups;
-  if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  const int64_t segs = int64_t(num_chunks) * num_heads;
+  if (segs * a.groups >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   auto s = static_cast<cudaStream_t>(stream);
-  const int rc = head_dim == 128 ? launch_select<128>(a, grid, s) : launch_select<64>(a, grid, s);
-  return rc;
+  return head_dim == 128 ? launch_select<128>(a, segs, s) : launch_select<64>(a, segs, s);
 }
 
 extern "C" int pkv_block_attention(const uint16_t* q, int64_t q_row_stride, int64_t q_head_stride,

@@ -155,6 +155,52 @@ def test_select_blocks_ties_zeros_and_nan(cuda):
     assert 4 not in select_blocks(ones, odd, cu, k.shape[0], 1, 1, 39).flatten().tolist()
 
 
+@pytest.mark.parametrize("R", [1, 600])
+@pytest.mark.parametrize("nb,top", [(40, 7), (300, 20), (2500, 64)])
+def test_select_blocks_scores_closer_than_fp32(cuda, R, nb, top):
+    """Blocks whose keys differ in one element by one bf16 step: scores apart by
+    less than the error of an fp32 sum, many of them equal."""
+    from pyramidkv.sparse import block_means, select_blocks
+    D, B = 128, 64
+    g = torch.Generator().manual_seed(nb + R)
+    base = torch.randn(B, D, generator=g)
+    base[:, :16] *= 1e-2
+    k = base.to(BF).repeat(nb, 1).view(nb, B, D)
+    at = torch.randint(0, 16, (nb,), generator=g)
+    bits = k[torch.arange(nb), 5, at].view(torch.int16) + torch.randint(-1, 2, (nb,), generator=g).short()
+    k[torch.arange(nb), 5, at] = bits.view(BF)
+    k = k.reshape(nb * B, D).to(cuda)
+    cu = torch.tensor([0, nb * B], dtype=torch.int32, device=cuda)
+    q = torch.randn(R, 1, D, generator=g).to(cuda, BF)
+    means = block_means(k, cu, B)
+    got = select_blocks(q, means, cu, k.shape[0], 1, R, top)
+    assert torch.equal(got, _exact_lists(q, k, cu, 1, R, top, 128, B))
+
+
+def test_select_blocks_huge_and_infinite(cuda):
+    """Products past fp32's range, infinite queries and means: the float64
+    order, NaN last, equal ones by index."""
+    from pyramidkv.sparse import select_blocks
+    D, nb = 64, 700
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(3, 1, D, generator=g).to(cuda, BF)
+    means = torch.randn(nb + 1, D, generator=g).to(cuda)
+    cu = torch.tensor([0, nb * 64], dtype=torch.int32, device=cuda)
+
+    def want(q, m, top):
+        s = (m[:nb].double() @ q[:, 0].double().sum(0)).cpu()
+        s = torch.where(torch.isnan(s), -torch.inf, s)
+        return torch.argsort(s, descending=True, stable=True)[:top].sort().values.int().tolist()
+    for qs, ms in ((1e30, 1e30), (1e-30, 1e-30), (1.0, 3e38), (1e-38, 1.0)):
+        m, qq = means * ms, (q.float() * qs).to(BF)
+        got = select_blocks(qq, m, cu, nb * 64, 1, 3, 33)
+        assert got.flatten().tolist() == want(qq, m, 33), (qs, ms)
+    inf = means.clone()
+    inf[5, 3], inf[77, 3], inf[400, 3] = float("inf"), -float("inf"), float("inf")
+    ones = q.abs()
+    assert select_blocks(ones, inf, cu, nb * 64, 1, 3, 9).flatten().tolist() == want(ones, inf, 9)
+
+
 ATTEND = [
     # segment lengths, chunks, heads, rows, D, query_block, block: few rows ...
     ([700, 0, 64, 3001], 1, 4, 1, 128, 128, 64),
