@@ -162,6 +162,9 @@ __device__ __forceinline__ void st_first(float* p, float v) {
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelCluster = 8;  // most CTAs a group
+constexpr int kSelKeys = 8;     // keys a thread holds: kMaxTopK and a round of kSelChunk
+constexpr int kSelChunk = 1024;
+static_assert(kMaxTopK + kSelChunk == kSelKeys * kSelThreads, "a thread's keys");
 
 struct SelectArgs {
   const uint16_t* q;
@@ -172,15 +175,11 @@ struct SelectArgs {
   int H, rows_per_chunk, groups, packs, query_block, block, top_k;
 };
 
-// Groups of a CTA, blocks scored per round, bytes of shared memory for top_k.
-template <int D, int GQ>
-struct SelectShape {
-  static constexpr int kChunk = GQ == 1 ? 1024 : 512;
-  static size_t bytes(int top_k) {
-    const size_t cap = size_t(top_k) + kChunk;
-    return sizeof(double) * (GQ + kSelWarps) * D + GQ * cap * 12 + size_t(GQ) * top_k * 4;
-  }
-};
+// Dynamic shared memory of GQ groups a CTA.
+size_t select_bytes(int D, int GQ, int top_k) {
+  const size_t cap = size_t(top_k) + kSelChunk;
+  return sizeof(double) * (GQ + kSelWarps) * D + GQ * cap * 12 + size_t(GQ) * top_k * 4;
+}
 
 // Scores as integers in the same order; NaN below all, -0 as 0.
 __device__ __forceinline__ uint64_t order_key(double s) {
@@ -199,49 +198,114 @@ __device__ __forceinline__ float unorder_f32(uint32_t k) {
   return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
-// The k-th largest of n > k scores, by a warp: the bits below the highest in
-// which the scores differ, from the top, by counting.
-__device__ __forceinline__ float kth_score(const float* s, int n, int k) {
-  constexpr uint32_t kAll = 0xffffffffu;
-  constexpr int kRegs = 16;
-  const int lane = threadIdx.x & 31;
-  uint32_t r[kRegs];
-  uint32_t mn = 0xffffffffu, mx = 0;
-  const bool held = n <= 32 * kRegs;  // the keys fit the warp's registers
-  if (held) {
+// Sum of a count over the block, in every thread.
+__device__ __forceinline__ int block_count(int c, int* buf) {
+  c = __reduce_add_sync(0xffffffffu, c);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = c;
+  __syncthreads();
+  c = 0;
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      r[i] = 0;
-      if (i * 32 + lane < n) {
-        r[i] = order_f32(s[i * 32 + lane]);
-        mn = min(mn, r[i]);
-        mx = max(mx, r[i]);
-      }
+  for (int w = 0; w < kSelWarps; ++w) c += buf[w];
+  __syncthreads();
+  return c;
+}
+
+// Scratch of pick_kth and of the list's compaction.
+struct PickSmem {
+  int hist[256];
+  uint32_t few[32];
+  int nfew;
+  uint32_t mn[kSelWarps], mx[kSelWarps];
+  int count[kSelKeys * kSelWarps];
+};
+
+// The k-th largest of the block's keys (thread t holds keys t, t + 256, ..;
+// n > k of them are there), the same in every thread: 8 bits a pass from the
+// highest in which the keys differ, by a histogram; once a digit's keys fit a
+// warp they are ranked there.  Every warp scans and ranks for itself.
+__device__ __forceinline__ uint32_t pick_kth(const uint32_t (&key)[kSelKeys], int n, int k,
+                                             PickSmem& sm) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t mn = 0xffffffffu, mx = 0;
+#pragma unroll
+  for (int t = 0; t < kSelKeys; ++t)
+    if (t * kSelThreads + tid < n) {
+      mn = min(mn, key[t]);
+      mx = max(mx, key[t]);
     }
-  } else {
-    for (int i = lane; i < n; i += 32) {
-      const uint32_t key = order_f32(s[i]);
-      mn = min(mn, key);
-      mx = max(mx, key);
-    }
-  }
   mn = __reduce_min_sync(kAll, mn);
   mx = __reduce_max_sync(kAll, mx);
-  if (mn == mx) return unorder_f32(mx);
-  uint32_t bit = 1u << (31 - __clz(int(mn ^ mx)));
-  uint32_t prefix = mx & ~(bit | (bit - 1));
-  for (; bit != 0; bit >>= 1) {
-    const uint32_t cand = prefix | bit;
-    int c = 0;
-    if (held) {
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i) c += r[i] >= cand;
-    } else {
-      for (int i = lane; i < n; i += 32) c += order_f32(s[i]) >= cand;
-    }
-    if (int(__reduce_add_sync(kAll, c)) >= k) prefix = cand;
+  if (lane == 0) {
+    sm.mn[warp] = mn;
+    sm.mx[warp] = mx;
   }
-  return unorder_f32(prefix);
+  sm.hist[tid] = 0;
+  if (tid == 0) sm.nfew = 0;
+  __syncthreads();
+  mn = __reduce_min_sync(kAll, sm.mn[lane & (kSelWarps - 1)]);
+  mx = __reduce_max_sync(kAll, sm.mx[lane & (kSelWarps - 1)]);
+  if (mn == mx) return mx;
+  int shift = 32 - __clz(int(mn ^ mx));  // bits below `shift` differ
+  uint32_t prefix = shift == 32 ? 0 : mx >> shift;
+  while (true) {
+    const int bits = min(8, shift), above = shift;
+    shift -= bits;
+#pragma unroll
+    for (int t = 0; t < kSelKeys; ++t)
+      if (t * kSelThreads + tid < n && (above == 32 ? 0 : key[t] >> above) == prefix)
+        atomicAdd(&sm.hist[(key[t] >> shift) & ((1u << bits) - 1)], 1);
+    __syncthreads();
+    // lane owns bins 255 - 8 lane .. 248 - 8 lane: a scan from the top
+    int cnt[8], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += cnt[i] = sm.hist[255 - 8 * lane - i];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(kAll, before, o);
+      if (lane >= o) before += y;
+    }
+    before -= sum;
+    int digit = -1, left = 0, size = 0;
+    if (before < k && before + sum >= k) {
+      int acc = before;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (digit < 0 && acc + cnt[i] >= k) {
+          digit = 255 - 8 * lane - i;
+          left = k - acc;
+          size = cnt[i];
+        }
+        acc += cnt[i];
+      }
+    }
+    const int owner = __ffs(__ballot_sync(kAll, digit >= 0)) - 1;
+    prefix = (prefix << bits) | uint32_t(__shfl_sync(kAll, digit, owner));
+    k = __shfl_sync(kAll, left, owner);
+    size = __shfl_sync(kAll, size, owner);
+    if (shift == 0) return prefix;
+    if (size <= 32) {
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t)
+        if (t * kSelThreads + tid < n && (key[t] >> shift) == prefix)
+          sm.few[atomicAdd(&sm.nfew, 1)] = key[t];
+      __syncthreads();
+      const uint32_t mine = lane < size ? sm.few[lane] : 0;
+      int gt = 0, ge = 0;
+      for (int i = 0; i < size; ++i) {
+        const uint32_t o = __shfl_sync(kAll, mine, i);
+        gt += o > mine;
+        ge += o >= mine;
+      }
+      const uint32_t b = __ballot_sync(kAll, lane < size && gt < k && ge >= k);
+      return __shfl_sync(kAll, mine, __ffs(b) - 1);
+    }
+    __syncthreads();  // every warp has scanned
+    sm.hist[tid] = 0;
+    __syncthreads();
+  }
 }
 
 // A CTA GQ groups of a segment, which share the loads of its means; with few
@@ -255,12 +319,12 @@ __device__ __forceinline__ float kth_score(const float* s, int n, int k) {
 // scored in float64 and ranked, unless all of them are in.  Infinite or NaN
 // queries or means make every block such a one.
 template <int D, int GQ>
-__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a) {
-  constexpr int kChunk = SelectShape<D, GQ>::kChunk;
+__global__ void __launch_bounds__(kSelThreads, 3) select_blocks_kernel(SelectArgs a) {
   constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ float nmax[kSelCluster * kSelWarps];
-  const int cap = a.top_k + kChunk;
+  __shared__ PickSmem pick;
+  const int cap = a.top_k + kSelChunk;
   double* qs = reinterpret_cast<double*>(raw);               // [GQ][D] summed queries
   double* red = qs + GQ * D;                                 // [warps][D]
   uint64_t* exact = reinterpret_cast<uint64_t*>(red + kSelWarps * D);  // [GQ][cap]
@@ -295,15 +359,16 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
     const uint16_t* p =
         a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
     double acc[8] = {};
-    for (int r = sub; r < nr; r += 8 * kRows) {
-      uint4 v[8];
+    constexpr int kLoads = 8 * GQ;  // a group of 128 rows at once
+    for (int r = sub; r < nr; r += kLoads * kRows) {
+      uint4 v[kLoads];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kLoads; ++i)
         v[i] = r + i * kRows < nr
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs))
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 8; i += 4)
+      for (int i = 0; i < kLoads; i += 4)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float lo4[4], hi4[4];
@@ -334,7 +399,7 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
     __syncthreads();
   }
   // ---- rounds of scores: 16 lanes a block, D / 16 products a lane ----
-  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = GQ == 1 ? 4 : 2;
+  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = 4;
   const int l16 = tid & 15;
   float q[GQ][kPer];
 #pragma unroll
@@ -346,9 +411,9 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
   int kept = 0;
   float most = 0.0f;              // largest |mean|^2 that this warp has seen
   if (X > 1) cluster_barrier();  // the first CTA runs: its memory may be written
-  for (int b0 = 0; b0 < nblk; b0 += kChunk) {
-    const int m = min(kChunk, nblk - b0);
-    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kChunk; i0 += stride * kBatch) {
+  for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
+    const int m = min(kSelChunk, nblk - b0);
+    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kSelChunk; i0 += stride * kBatch) {
       if (i0 - (lane >> 4) >= m) break;  // (the whole warp)
       float4 f[kBatch][kVec];
 #pragma unroll
@@ -398,106 +463,131 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(SelectArgs a
     const int total = kept + m;
     const bool last = b0 + m == nblk;
     if (rank != 0 && last) return;
-    if (rank == 0 && total > a.top_k && warp < ng) {
-      // ---- pick: a warp a group ----
-      const float* sc = score + warp * cap;
-      uint64_t* ex = exact + warp * cap;
-      int* kd = kid + warp * a.top_k;
-      const double* qg = qs + warp * D;
+    for (int g = 0; rank == 0 && g < ng; ++g) {
+      float* sc = score + g * cap;
+      int* kd = kid + g * a.top_k;
+      if (total <= a.top_k) {  // (not the last round)
+        for (int i = tid; i < m; i += kSelThreads) kd[kept + i] = b0 + i;
+        continue;
+      }
+      uint64_t* ex = exact + g * cap;
+      const double* qg = qs + g * D;
+      // 2.25 e, rounded up; the addend covers products that underflow
       double qn = 0.0;
-      for (int d = lane; d < D; d += 32) qn = fma(qg[d], qg[d], qn);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) qn += __shfl_xor_sync(kAll, qn, o);
+      for (int d = 0; d < D; d += 32) qn = fma(qg[d + lane], qg[d + lane], qn);
       float mm = 0.0f;
       for (int i = lane; i < X * kSelWarps; i += 32) mm = fmaxf(mm, nmax[i]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
-      // 2.25 e, rounded up; the addend covers products that underflow
-      const float e2 = 2.25f * 9.5367431640625e-7f * 1.001f * float(sqrt(qn)) * sqrtf(mm) + 1e-36f;
-      const bool all = !(e2 < INFINITY);
+      for (int o = 16; o > 0; o >>= 1) {
+        qn += __shfl_xor_sync(kAll, qn, o);
+        mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
+      }
+      const float qf = float(qn);  // (infinite past fp32's range: every block is near)
+      const float e2 = 2.25f * 9.5367431640625e-7f * 1.001f * sqrtf(qf) * sqrtf(mm) + 1e-36f;
+      const bool all = !(e2 < INFINITY) || !(qf >= 1e-30f);
+      float v[kSelKeys];
+      uint32_t key[kSelKeys];
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t) {
+        const int i = t * kSelThreads + tid;
+        v[t] = i < total ? sc[i] : 0.0f;
+        key[t] = order_f32(v[t]);
+      }
       float lo = 0.0f, hi = 0.0f;
       if (!all) {
-        const float T = kth_score(sc, total, a.top_k);
+        const float T = unorder_f32(pick_kth(key, total, a.top_k, pick));
         lo = T - e2;
         hi = T + e2;
       }
+      // keys become flags: 1 in for certain, 2 near
       int sure = 0, near = 0;
-      for (int i = lane; i < total; i += 32) {
-        sure += !all && sc[i] > hi;
-        near += all || (sc[i] >= lo && sc[i] <= hi);
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t) {
+        key[t] = 0;
+        if (t * kSelThreads + tid < total)
+          key[t] = all ? 2u : v[t] > hi ? 1u : v[t] >= lo ? 2u : 0u;
+        sure += key[t] == 1u;
+        near += key[t] == 2u;
       }
-      sure = __reduce_add_sync(kAll, sure);
-      near = __reduce_add_sync(kAll, near);
+      sure = block_count(sure, pick.count);
+      near = block_count(near, pick.count);
       const int need = a.top_k - sure;
-      if (near > need) {  // float64 scores of the near ones
-        for (int t0 = 0; t0 < total; t0 += 32) {
-          const int i = t0 + lane;
-          const bool is = i < total && (all || (sc[i] >= lo && sc[i] <= hi));
-          uint32_t todo = __ballot_sync(kAll, is);
+      if (near > need) {
+        // float64 scores of the near ones, a warp a block, then each near
+        // one's rank among them
+#pragma unroll
+        for (int t = 0; t < kSelKeys; ++t) {
+          uint32_t todo = __ballot_sync(kAll, key[t] == 2u);
+          if (t * kSelThreads + tid < total) ex[t * kSelThreads + tid] = 0;
+          __syncwarp();
           while (todo) {
-            const int j = t0 + __ffs(todo) - 1;
+            const int j = t * kSelThreads + warp * 32 + __ffs(todo) - 1;
             todo &= todo - 1;
             const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
-            double t = 0.0;
+            double x = 0.0;
             if (row >= 0 && row < a.means_rows)
               for (int d = lane; d < D; d += 32)
-                t = fma(double(__ldg(a.means + row * D + d)), qg[d], t);
+                x = fma(double(__ldg(a.means + row * D + d)), qg[d], x);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kAll, t, o);
-            if (lane == 0) ex[j] = order_key(t);
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
+            if (lane == 0) ex[j] = order_key(x) + 1;  // 0: not a near one
           }
         }
-        __syncwarp();
-      }
-      // ---- which to keep: a near one by its rank among the near.  Lane t
-      // holds the flags of the 32 blocks of tiles t and t + 32 ----
-      uint32_t flags[2] = {0, 0};
-      for (int t0 = 0; t0 < total; t0 += 32) {
-        const int i = t0 + lane;
-        const float v = i < total ? sc[i] : 0.0f;
-        const bool is = i < total && (all || (v >= lo && v <= hi));
-        bool keep = i < total && !all && v > hi;
-        if (near <= need) {
-          keep = keep || is;
-        } else {
-          uint32_t todo = __ballot_sync(kAll, is);
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < kSelKeys; ++t) {
+          uint32_t todo = __ballot_sync(kAll, key[t] == 2u);
           while (todo) {
-            const int j = t0 + __ffs(todo) - 1;
+            const int bit = __ffs(todo) - 1, j = t * kSelThreads + warp * 32 + bit;
             todo &= todo - 1;
             const uint64_t mine = ex[j];
             int ahead = 0;
             for (int x = lane; x < total; x += 32)
-              if (all || (sc[x] >= lo && sc[x] <= hi))
-                ahead += ex[x] > mine || (ex[x] == mine && x < j);
+              ahead += ex[x] > mine || (ex[x] == mine && x < j);
             ahead = __reduce_add_sync(kAll, ahead);
-            if (i == j) keep = ahead < need;
+            if (lane == bit && ahead >= need) key[t] = 0;
           }
         }
-        const uint32_t kb = __ballot_sync(kAll, keep);
-        if (lane == ((t0 >> 5) & 31)) (t0 < 1024 ? flags[0] : flags[1]) = kb;
       }
-      // ---- move them up, in index order ----
-      int at = 0;
-      for (int t0 = 0; t0 < total; t0 += 32) {
-        const int i = t0 + lane;
-        const uint32_t kb = __shfl_sync(kAll, t0 < 1024 ? flags[0] : flags[1], (t0 >> 5) & 31);
-        const float v = i < total ? sc[i] : 0.0f;
-        const int id = i < total ? (i < kept ? kd[i] : b0 + i - kept) : 0;
-        __syncwarp();
-        if ((kb >> lane) & 1) {
-          const int to = at + __popc(kb & ((1u << lane) - 1));
+      // ---- the kept ones, in index order ----
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t) {
+        const uint32_t kb = __ballot_sync(kAll, key[t] != 0);
+        if (lane == 0) pick.count[t * kSelWarps + warp] = __popc(kb);
+      }
+      int id[kSelKeys];
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t) {
+        const int i = t * kSelThreads + tid;
+        id[t] = key[t] != 0 ? (i < kept ? kd[i] : b0 + i - kept) : 0;
+      }
+      __syncthreads();
+      // counts before this warp's, of tile 0 and then from tile to tile
+      int mine = 0;
+#pragma unroll
+      for (int t = 0; t < kSelKeys; ++t) {
+        int add = 0;
+#pragma unroll
+        for (int w = 0; w < kSelWarps; ++w) {
+          const int n = pick.count[t * kSelWarps + w];
+          if (w < warp) mine += n;
+          add += w >= warp ? n : 0;
+        }
+        const uint32_t kb = __ballot_sync(kAll, key[t] != 0);
+        const int to = mine + __popc(kb & ((1u << lane) - 1));
+        if (key[t] != 0) {
           if (last) {
-            out[warp * a.top_k + to] = id;
+            out[g * a.top_k + to] = id[t];
           } else {
-            score[warp * cap + to] = v;
-            kd[to] = id;
+            sc[to] = v[t];
+            kd[to] = id[t];
           }
         }
-        __syncwarp();
-        at += __popc(kb);
+        mine += add;
+        if ((t + 1) * kSelThreads >= total) break;
       }
-    } else if (rank == 0 && warp < ng) {
-      for (int i = lane; i < m; i += 32) kid[warp * a.top_k + kept + i] = b0 + i;
+      __syncthreads();
     }
     kept = min(total, a.top_k);
     if (last) return;
@@ -1117,11 +1207,9 @@ int launch_cluster(void (*kernel)(A), const A& a, int64_t units, int X, int thre
 
 template <int D, int GQ>
 int select_shape(SelectArgs a, int64_t segs, cudaStream_t stream) {
-  using Shape = SelectShape<D, GQ>;
-  static_assert(Shape::kChunk + kMaxTopK <= 2048, "a lane holds the flags of two tiles");
   static std::mutex mu;
   static int done[kMaxDevices] = {};
-  if (smem_opt_in(done, mu, select_blocks_kernel<D, GQ>, Shape::bytes(kMaxTopK)) <= 0) {
+  if (smem_opt_in(done, mu, select_blocks_kernel<D, GQ>, select_bytes(D, GQ, kMaxTopK)) <= 0) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
@@ -1134,15 +1222,14 @@ int select_shape(SelectArgs a, int64_t segs, cudaStream_t stream) {
   if (GQ == 1)
     while (X < kSelCluster && units * X * 2 <= sm_count() && blocks >= int64_t(X) * 64) X *= 2;
   return launch_cluster(select_blocks_kernel<D, GQ>, a, units, X, kSelThreads,
-                        Shape::bytes(a.top_k), stream);
+                        select_bytes(D, GQ, a.top_k), stream);
 }
 
-// Four groups share a segment's means where that still leaves a CTA for most
-// SMs.
+// Two groups share a segment's means where that leaves four CTAs for every SM.
 template <int D>
 int launch_select(const SelectArgs& a, int64_t segs, cudaStream_t stream) {
-  if (a.groups >= 4 && segs * ((a.groups + 3) / 4) * 4 >= int64_t(sm_count()) * 3)
-    return select_shape<D, 4>(a, segs, stream);
+  if (a.groups >= 2 && segs * ((a.groups + 1) / 2) >= int64_t(sm_count()) * 4)
+    return select_shape<D, 2>(a, segs, stream);
   return select_shape<D, 1>(a, segs, stream);
 }
 
