@@ -13,16 +13,17 @@
 //  * block_means_kernel -- one pass over K, bound by HBM.  Segment s's block j
 //    has row cu[s] / block + s + j of the table: a closed form, so the table
 //    needs no offsets of its own (ceil(n / B) <= floor((a + n) / B) - floor(a / B) + 1).
-//  * select_blocks_kernel -- scores in fp32 with a bound on their error; only
-//    blocks within that bound of the last place are scored again in float64
-//    (queries summed in float64, products of fp32 means exact before their
-//    float64 sum), so the lists are those of the definition.
+//  * select_blocks_kernel -- scores on the tensor cores with a bound on their
+//    error; only blocks within that bound of the last place are scored again in
+//    float64 (queries summed in float64, products of fp32 means exact before
+//    their float64 sum), so the lists are those of the definition.
 //  * attention over the listed blocks, by the rows of a group:
 //    up to 16 rows (a decoded token, a small group): warps each take 16 keys,
 //    K and V go from memory straight into mma fragments, a thread-block
 //    cluster splits the list and joins the parts through distributed shared
 //    memory -- bound by latency and by the bytes of the listed blocks;
 //    more rows: tcgen05 tiles of 128 rows (see sparse_tc_kernel).
+#include <cfloat>
 #include <mutex>
 
 #include "pkv_internal.h"
@@ -149,11 +150,20 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
   return v;
 }
 
-// Into the first CTA of the cluster.
-__device__ __forceinline__ void st_first(float* p, float v) {
+// Into CTA `rank` of the cluster.
+__device__ __forceinline__ void st_cluster(float* p, uint32_t rank, float v) {
   uint32_t addr;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(addr) : "r"(su32(p)));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(su32(p)), "r"(rank));
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---------------------------------------------------------------------------
@@ -161,10 +171,11 @@ __device__ __forceinline__ void st_first(float* p, float v) {
 // ---------------------------------------------------------------------------
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelCluster = 8;  // most CTAs a group
-constexpr int kSelKeys = 8;     // keys a thread holds: kMaxTopK and a round of kSelChunk
+constexpr int kSelGroups = 16;  // groups of a cluster: the rows of an mma
+constexpr int kSelCluster = 8;  // most CTAs of one
+constexpr int kSelHeld = 16;    // scores a lane of a picking warp keeps in registers
 constexpr int kSelChunk = 1024;
-static_assert(kMaxTopK + kSelChunk == kSelKeys * kSelThreads, "a thread's keys");
+static_assert(kMaxTopK + kSelChunk <= 64 * 32, "a lane holds the flags of two tiles of 32");
 
 struct SelectArgs {
   const uint16_t* q;
@@ -175,10 +186,11 @@ struct SelectArgs {
   int H, rows_per_chunk, groups, packs, query_block, block, top_k;
 };
 
-// Dynamic shared memory of GQ groups a CTA.
-size_t select_bytes(int D, int GQ, int top_k) {
-  const size_t cap = size_t(top_k) + kSelChunk;
-  return sizeof(double) * (GQ + kSelWarps) * D + GQ * cap * 12 + size_t(GQ) * top_k * 4;
+// Dynamic shared memory with X CTAs a cluster (kSelGroups / X groups a CTA).
+size_t select_bytes(int D, int X, int top_k) {
+  const size_t cap = size_t(top_k) + kSelChunk, g = kSelGroups / X;
+  return sizeof(double) * (g + kSelWarps) * D + sizeof(float) * kSelGroups * (D + 2) +
+         g * cap * 12 + g * top_k * 4;
 }
 
 // Scores as integers in the same order; NaN below all, -0 as 0.
@@ -189,186 +201,157 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
-// fp32 scores as integers in the same order (not NaN), and back.
-__device__ __forceinline__ uint32_t order_f32(float s) {
-  const uint32_t b = __float_as_uint(s + 0.0f);  // -0 as 0
-  return (b >> 31) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float unorder_f32(uint32_t k) {
-  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
-}
+// Scores of a picking warp: the first kSelHeld tiles of 32 in registers when
+// that is all of them, else in shared memory.
+struct Scores {
+  float v[kSelHeld];
+  const float* s;
+  int n;
+  bool held;
 
-// Sum of a count over the block, in every thread.
-__device__ __forceinline__ int block_count(int c, int* buf) {
-  c = __reduce_add_sync(0xffffffffu, c);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = c;
-  __syncthreads();
-  c = 0;
+  __device__ __forceinline__ Scores(const float* scores, int total) : s(scores), n(total) {
+    const int lane = threadIdx.x & 31;
+    held = n <= 32 * kSelHeld;
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) c += buf[w];
-  __syncthreads();
-  return c;
-}
-
-// Scratch of pick_kth and of the list's compaction.
-struct PickSmem {
-  int hist[256];
-  uint32_t few[32];
-  int nfew;
-  uint32_t mn[kSelWarps], mx[kSelWarps];
-  int count[kSelKeys * kSelWarps];
+    for (int t = 0; t < kSelHeld; ++t)
+      v[t] = t * 32 + lane < n ? s[t * 32 + lane] : -INFINITY;
+  }
+  // Scores at or above x.
+  __device__ __forceinline__ int at_least(float x) const {
+    int c = 0;
+    if (held) {
+#pragma unroll
+      for (int t = 0; t < kSelHeld; ++t) c += v[t] >= x;
+    } else {
+      for (int i = threadIdx.x & 31; i < n; i += 32) c += s[i] >= x;
+    }
+    return __reduce_add_sync(0xffffffffu, c);
+  }
+  // Least score at or above x.
+  __device__ __forceinline__ float least_from(float x) const {
+    float m = INFINITY;
+    if (held) {
+#pragma unroll
+      for (int t = 0; t < kSelHeld; ++t) m = fminf(m, v[t] >= x ? v[t] : INFINITY);
+    } else {
+      for (int i = threadIdx.x & 31; i < n; i += 32) m = fminf(m, s[i] >= x ? s[i] : INFINITY);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fminf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  }
+  __device__ __forceinline__ float greatest() const {
+    float m = -INFINITY;
+    if (held) {
+#pragma unroll
+      for (int t = 0; t < kSelHeld; ++t) m = fmaxf(m, v[t]);
+    } else {
+      for (int i = threadIdx.x & 31; i < n; i += 32) m = fmaxf(m, s[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  }
 };
 
-// The k-th largest of the block's keys (thread t holds keys t, t + 256, ..;
-// n > k of them are there), the same in every thread: 8 bits a pass from the
-// highest in which the keys differ, by a histogram; once a digit's keys fit a
-// warp they are ranked there.  Every warp scans and ranks for itself.
-__device__ __forceinline__ uint32_t pick_kth(const uint32_t (&key)[kSelKeys], int n, int k,
-                                             PickSmem& sm) {
-  constexpr uint32_t kAll = 0xffffffffu;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t mn = 0xffffffffu, mx = 0;
-#pragma unroll
-  for (int t = 0; t < kSelKeys; ++t)
-    if (t * kSelThreads + tid < n) {
-      mn = min(mn, key[t]);
-      mx = max(mx, key[t]);
-    }
-  mn = __reduce_min_sync(kAll, mn);
-  mx = __reduce_max_sync(kAll, mx);
-  if (lane == 0) {
-    sm.mn[warp] = mn;
-    sm.mx[warp] = mx;
-  }
-  sm.hist[tid] = 0;
-  if (tid == 0) sm.nfew = 0;
-  __syncthreads();
-  mn = __reduce_min_sync(kAll, sm.mn[lane & (kSelWarps - 1)]);
-  mx = __reduce_max_sync(kAll, sm.mx[lane & (kSelWarps - 1)]);
-  if (mn == mx) return mx;
-  int shift = 32 - __clz(int(mn ^ mx));  // bits below `shift` differ
-  uint32_t prefix = shift == 32 ? 0 : mx >> shift;
+// The k-th largest of n > k finite scores, by halving the range until exactly
+// k are above (then it is the least of those) or the range is below `close`
+// (then its lower end, less than `close` below the k-th).
+__device__ __forceinline__ float kth_score(const Scores& sc, int k, float close) {
+  float lo = sc.least_from(-FLT_MAX), hi = sc.greatest();
+  if (sc.at_least(hi) >= k) return hi;
   while (true) {
-    const int bits = min(8, shift), above = shift;
-    shift -= bits;
-#pragma unroll
-    for (int t = 0; t < kSelKeys; ++t)
-      if (t * kSelThreads + tid < n && (above == 32 ? 0 : key[t] >> above) == prefix)
-        atomicAdd(&sm.hist[(key[t] >> shift) & ((1u << bits) - 1)], 1);
-    __syncthreads();
-    // lane owns bins 255 - 8 lane .. 248 - 8 lane: a scan from the top
-    int cnt[8], sum = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += cnt[i] = sm.hist[255 - 8 * lane - i];
-    int before = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(kAll, before, o);
-      if (lane >= o) before += y;
-    }
-    before -= sum;
-    int digit = -1, left = 0, size = 0;
-    if (before < k && before + sum >= k) {
-      int acc = before;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (digit < 0 && acc + cnt[i] >= k) {
-          digit = 255 - 8 * lane - i;
-          left = k - acc;
-          size = cnt[i];
-        }
-        acc += cnt[i];
-      }
-    }
-    const int owner = __ffs(__ballot_sync(kAll, digit >= 0)) - 1;
-    prefix = (prefix << bits) | uint32_t(__shfl_sync(kAll, digit, owner));
-    k = __shfl_sync(kAll, left, owner);
-    size = __shfl_sync(kAll, size, owner);
-    if (shift == 0) return prefix;
-    if (size <= 32) {
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t)
-        if (t * kSelThreads + tid < n && (key[t] >> shift) == prefix)
-          sm.few[atomicAdd(&sm.nfew, 1)] = key[t];
-      __syncthreads();
-      const uint32_t mine = lane < size ? sm.few[lane] : 0;
-      int gt = 0, ge = 0;
-      for (int i = 0; i < size; ++i) {
-        const uint32_t o = __shfl_sync(kAll, mine, i);
-        gt += o > mine;
-        ge += o >= mine;
-      }
-      const uint32_t b = __ballot_sync(kAll, lane < size && gt < k && ge >= k);
-      return __shfl_sync(kAll, mine, __ffs(b) - 1);
-    }
-    __syncthreads();  // every warp has scanned
-    sm.hist[tid] = 0;
-    __syncthreads();
+    const float mid = 0.5f * lo + 0.5f * hi;
+    if (!(mid > lo && mid < hi) || hi - lo < close) return lo;
+    const int c = sc.at_least(mid);
+    if (c == k) return sc.least_from(mid);
+    if (c > k)
+      lo = mid;
+    else
+      hi = mid;
   }
 }
 
-// A CTA GQ groups of a segment, which share the loads of its means; with few
-// groups (GQ = 1, single tokens) a cluster a group, whose CTAs share the
-// scores and whose first picks: the table is then read by many SMs.
+// Two fp32 values as bf16 pairs, hi + lo: 16 bits of each.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x, y);
+  lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
+// A cluster of X CTAs serves 16 groups of a segment: each CTA sums the queries
+// of its share of the groups (group i belongs to rank i % X), all of them score
+// their share of the blocks for all 16 groups on mma.m16n8k16 (rows = groups,
+// columns = blocks), hand the scores to the groups' owners through distributed
+// shared memory, and every CTA picks for its groups.  A block's mean is read
+// once for 16 groups, and a single token's table by many SMs.
 //
-// An fp32 score differs from the exact one by at most e = 2^-20 |q| |mean|
-// (q rounded once, D / 16 products a lane in a chain, 4 levels of adds: 13
-// roundings of 2^-24).  With T the top_k-th fp32 score, a block above T + 2 e
-// is in the list for certain and one below T - 2 e is not; those between are
-// scored in float64 and ranked, unless all of them are in.  Infinite or NaN
-// queries or means make every block such a one.
-template <int D, int GQ>
-__global__ void __launch_bounds__(kSelThreads, 3) select_blocks_kernel(SelectArgs a) {
+// Operands are split into bf16 hi + lo and multiplied as hi hi + hi lo + lo hi:
+// off by at most 3 * 2^-18 |q| |mean|, and the fp32 accumulation of 3 * 128
+// products by less than 2^-17 |q| |mean|; e = 2^-15 |q| |mean| bounds both
+// twice over.  With T the top_k-th such score, a block above T + 2 e is in the
+// list for certain and one below T - 2 e is not; those between are scored in
+// float64 and ranked, unless all of them are in.  Infinite or NaN queries or
+// means make every block such a one.
+template <int D, int X>
+__global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArgs a) {
   constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kMine = kSelGroups / X;  // groups a CTA owns
+  constexpr int kQs = D + 2;             // row stride of qf: no bank conflicts
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ float nmax[kSelCluster * kSelWarps];
-  __shared__ PickSmem pick;
   const int cap = a.top_k + kSelChunk;
-  double* qs = reinterpret_cast<double*>(raw);               // [GQ][D] summed queries
-  double* red = qs + GQ * D;                                 // [warps][D]
-  uint64_t* exact = reinterpret_cast<uint64_t*>(red + kSelWarps * D);  // [GQ][cap]
-  float* score = reinterpret_cast<float*>(exact + GQ * cap);           // [GQ][cap]
-  int* kid = reinterpret_cast<int*>(score + GQ * cap);       // [GQ][top_k] earlier rounds' ids
+  double* qs = reinterpret_cast<double*>(raw);                     // [kMine][D] summed queries
+  double* red = qs + kMine * D;                                    // [warps][D]
+  uint64_t* exact = reinterpret_cast<uint64_t*>(red + kSelWarps * D);  // [kMine][cap] float64
+  float* qf = reinterpret_cast<float*>(exact + kMine * cap);       // [16][D + 2] of all groups
+  float* score = qf + kSelGroups * kQs;                            // [kMine][cap]
+  int* kid = reinterpret_cast<int*>(score + kMine * cap);          // [kMine][top_k] kept earlier
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int X = int(cluster_size()), rank = int(cluster_rank());
+  const int rank = X > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / X;
-  const int s = unit / a.packs, g0 = (unit - s * a.packs) * GQ;
-  const int ng = min(GQ, a.groups - g0);
+  const int s = unit / a.packs, g0 = (unit - s * a.packs) * kSelGroups;
+  const int ng = min(kSelGroups, a.groups - g0);
   const int c = s / a.H, h = s - c * a.H;
   const SegView sg = segment(a.cu, s, a.kv_rows);
   const int nblk = (sg.len + a.block - 1) / a.block;
   int32_t* out = a.blocks + (int64_t(s) * a.groups + g0) * a.top_k;  // ng lists
   if (nblk <= a.top_k) {  // every block is kept (the whole cluster leaves)
-    if (rank == 0)
-      for (int i = tid; i < ng * a.top_k; i += kSelThreads) {
-        const int j = i % a.top_k;
-        out[i] = j < nblk ? j : -1;
-      }
+    for (int i = rank * kSelThreads + tid; i < ng * a.top_k; i += X * kSelThreads) {
+      const int j = i % a.top_k;
+      out[i] = j < nblk ? j : -1;
+    }
     return;
   }
-  // ---- sums of the groups' queries in float64 (exact for bf16 of like size;
-  // four rows are added in fp32 first, as block_means_kernel does) ----
-  {
-    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / GQ;
-    const int g = warp / kWarps, w = warp - g * kWarps;
-    const int sub = w * kPerWarp + lane / kLanes, d0 = (lane % kLanes) * 8;
+  auto barrier = [] {
+    if constexpr (X > 1)
+      cluster_barrier();
+    else
+      __syncthreads();
+  };
+  // ---- sums of this CTA's groups' queries in float64 (exact for bf16 of like
+  // size; four rows are added in fp32 first, as block_means_kernel does) ----
+  for (int i = tid; i < (kSelGroups - ng) * kQs; i += kSelThreads) qf[ng * kQs + i] = 0.0f;
+  constexpr int kTogether = kMine < 4 ? kMine : 4;  // groups summed side by side
+#pragma unroll 1
+  for (int m0 = 0; m0 < kMine; m0 += kTogether) {
+    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / kTogether;
     constexpr int kRows = kWarps * kPerWarp;
+    const int g = (m0 + warp / kWarps) * X + rank;
+    const int sub = warp % kWarps * kPerWarp + lane / kLanes, d0 = (lane % kLanes) * 8;
     const int r0 = (g0 + g) * a.query_block;
     const int nr = g < ng ? min(a.query_block, a.rows_per_chunk - r0) : 0;
     const uint16_t* p =
         a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
     double acc[8] = {};
-    constexpr int kLoads = 8 * GQ;  // a group of 128 rows at once
-    for (int r = sub; r < nr; r += kLoads * kRows) {
-      uint4 v[kLoads];
+    for (int r = sub; r < nr; r += 16 * kRows) {
+      uint4 v[16];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
+      for (int i = 0; i < 16; ++i)
         v[i] = r + i * kRows < nr
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs))
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < kLoads; i += 4)
+      for (int i = 0; i < 16; i += 4)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float lo4[4], hi4[4];
@@ -389,90 +372,117 @@ __global__ void __launch_bounds__(kSelThreads, 3) select_blocks_kernel(SelectArg
     if (lane < kLanes)
 #pragma unroll
       for (int e = 0; e < 8; ++e) red[warp * D + d0 + e] = acc[e];
-    __syncthreads();
-    for (int i = tid; i < GQ * D; i += kSelThreads) {
+    // the other CTAs run: their memory may be written (first time round)
+    if (m0 == 0)
+      barrier();
+    else
+      __syncthreads();
+    for (int i = tid; i < kTogether * D; i += kSelThreads) {
       double t = 0.0;
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) t += red[(i / D * kWarps + x) * D + i % D];
-      qs[i] = t;
+      qs[m0 * D + i] = t;
+      const int gi = (m0 + i / D) * X + rank;
+      if (gi < ng) {
+        if constexpr (X > 1) {
+#pragma unroll
+          for (int x = 0; x < X; ++x) st_cluster(&qf[gi * kQs + i % D], x, float(t));
+        } else {
+          qf[gi * kQs + i % D] = float(t);
+        }
+      }
     }
-    __syncthreads();
+    if (m0 + kTogether < kMine) __syncthreads();
   }
-  // ---- rounds of scores: 16 lanes a block, D / 16 products a lane ----
-  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = 4;
-  const int l16 = tid & 15;
-  float q[GQ][kPer];
+  barrier();
+  // ---- queries as A fragments: with lane (g, c) = (lane / 4, lane % 4),
+  // k-steps 2i, 2i + 1 take dims 32 i + 8 c .. + 7 (the order of the
+  // contraction is free), so a mean's lanes load 32 bytes each ----
+  const int gr = lane >> 2, cc = lane & 3;
+  uint32_t ah[D / 32][8], al[D / 32][8];
 #pragma unroll
-  for (int g = 0; g < GQ; ++g)
+  for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) q[g][i] = float(qs[g * D + (i / 4) * 64 + l16 * 4 + (i & 3)]);
+    for (int hrow = 0; hrow < 2; ++hrow) {
+      const float* p = qf + (gr + 8 * hrow) * kQs + 32 * i + 8 * cc;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 w = *reinterpret_cast<const float2*>(p + 2 * e);
+        split2(w.x, w.y, ah[i][2 * e + hrow], al[i][2 * e + hrow]);
+      }
+    }
   const int64_t base = int64_t(a.cu[s]) / a.block + s;
-  const int stride = X * (kSelThreads / 16);
   int kept = 0;
-  float most = 0.0f;              // largest |mean|^2 that this warp has seen
-  if (X > 1) cluster_barrier();  // the first CTA runs: its memory may be written
+  float most = 0.0f;  // largest |mean|^2 that this warp has seen
   for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
     const int m = min(kSelChunk, nblk - b0);
-    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kSelChunk; i0 += stride * kBatch) {
-      if (i0 - (lane >> 4) >= m) break;  // (the whole warp)
-      float4 f[kBatch][kVec];
+    for (int t = rank * kSelWarps + warp; t * 8 < m; t += X * kSelWarps) {
+      const int64_t row = base + b0 + t * 8 + gr;
+      const bool ok = t * 8 + gr < m && row >= 0 && row < a.means_rows;
+      const float* p = a.means + row * D + 8 * cc;
+      float4 f[D / 32][2];
 #pragma unroll
-      for (int x = 0; x < kBatch; ++x) {
-        const int64_t row = base + b0 + i0 + x * stride;
-        const bool ok = i0 + x * stride < m && row >= 0 && row < a.means_rows;
-        const float* p = a.means + row * D + l16 * 4;
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          f[x][e] = ok ? __ldg(reinterpret_cast<const float4*>(p + e * 64))
+        for (int e = 0; e < 2; ++e)
+          f[i][e] = ok ? __ldg(reinterpret_cast<const float4*>(p + 32 * i + 4 * e))
                        : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      float part[4][4] = {};  // independent chains of mma
+      float n2 = 0.0f;
 #pragma unroll
-      for (int x = 0; x < kBatch; ++x) {
-        float t[GQ + 1];
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int g = 0; g <= GQ; ++g) t[g] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float v[4] = {f[x][e].x, f[x][e].y, f[x][e].z, f[x][e].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int g = 0; g < GQ; ++g) t[g] = fmaf(v[i], q[g][4 * e + i], t[g]);
-            t[GQ] = fmaf(v[i], v[i], t[GQ]);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const float4 v = f[i][e];
+          n2 = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, n2))));
+          uint32_t bh0, bl0, bh1, bl1;
+          split2(v.x, v.y, bh0, bl0);
+          split2(v.z, v.w, bh1, bl1);
+          const uint32_t* x = ah[i] + 4 * e;
+          const uint32_t* y = al[i] + 4 * e;
+          mma_16816(part[0], y[0], y[1], y[2], y[3], bh0, bh1);
+          mma_16816(part[1], x[0], x[1], x[2], x[3], bl0, bl1);
+          mma_16816(part[2 + e], x[0], x[1], x[2], x[3], bh0, bh1);
         }
+      n2 += __shfl_xor_sync(kAll, n2, 1);
+      n2 += __shfl_xor_sync(kAll, n2, 2);
+      most = n2 < INFINITY ? fmaxf(most, n2) : INFINITY;
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1)
-#pragma unroll
-          for (int g = 0; g <= GQ; ++g) t[g] += __shfl_xor_sync(kAll, t[g], o);
-        most = t[GQ] < INFINITY ? fmaxf(most, t[GQ]) : INFINITY;
-        const int i = i0 + x * stride;
-        if (i < m) {
-#pragma unroll
-          for (int g = 0; g < GQ; ++g)
-            if (l16 == g) st_first(&score[g * cap + kept + i], t[g]);
+      for (int e = 0; e < 4; ++e) {
+        const int gi = gr + 8 * (e >> 1), i = t * 8 + 2 * cc + (e & 1);
+        const float v = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
+        if (gi < ng && i < m) {
+          float* to = &score[gi / X * cap + kept + i];
+          if constexpr (X > 1)
+            st_cluster(to, gi % X, v);
+          else
+            *to = v;
         }
       }
     }
-    const float both = fmaxf(most, __shfl_xor_sync(kAll, most, 16));
-    if (lane == 0) st_first(&nmax[rank * kSelWarps + warp], both);
-    if (X > 1)
-      cluster_barrier();  // every score is in the first CTA's memory
-    else
-      __syncthreads();
+    float all_most = most;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) all_most = fmaxf(all_most, __shfl_xor_sync(kAll, all_most, o));
+    if (lane < X) {
+      if constexpr (X > 1)
+        st_cluster(&nmax[rank * kSelWarps + warp], lane, all_most);
+      else
+        nmax[warp] = all_most;
+    }
+    barrier();  // the scores of this CTA's groups are here
     const int total = kept + m;
     const bool last = b0 + m == nblk;
-    if (rank != 0 && last) return;
-    for (int g = 0; rank == 0 && g < ng; ++g) {
-      float* sc = score + g * cap;
+    // ---- pick: a warp a group ----
+    for (int g = warp; g < kMine && g * X + rank < ng; g += kSelWarps) {
       int* kd = kid + g * a.top_k;
       if (total <= a.top_k) {  // (not the last round)
-        for (int i = tid; i < m; i += kSelThreads) kd[kept + i] = b0 + i;
+        for (int i = lane; i < m; i += 32) kd[kept + i] = b0 + i;
         continue;
       }
+      int32_t* list = out + int64_t(g * X + rank) * a.top_k;
+      float* sc = score + g * cap;
       uint64_t* ex = exact + g * cap;
       const double* qg = qs + g * D;
-      // 2.25 e, rounded up; the addend covers products that underflow
       double qn = 0.0;
 #pragma unroll
       for (int d = 0; d < D; d += 32) qn = fma(qg[d + lane], qg[d + lane], qn);
@@ -483,46 +493,31 @@ __global__ void __launch_bounds__(kSelThreads, 3) select_blocks_kernel(SelectArg
         qn += __shfl_xor_sync(kAll, qn, o);
         mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
       }
-      const float qf = float(qn);  // (infinite past fp32's range: every block is near)
-      const float e2 = 2.25f * 9.5367431640625e-7f * 1.001f * sqrtf(qf) * sqrtf(mm) + 1e-36f;
-      const bool all = !(e2 < INFINITY) || !(qf >= 1e-30f);
-      float v[kSelKeys];
-      uint32_t key[kSelKeys];
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t) {
-        const int i = t * kSelThreads + tid;
-        v[t] = i < total ? sc[i] : 0.0f;
-        key[t] = order_f32(v[t]);
-      }
-      float lo = 0.0f, hi = 0.0f;
+      // 2.25 e, rounded up; the addend covers parts that underflow
+      const float ql = sqrtf(float(qn)), ml = sqrtf(mm);
+      const float e2 = 2.25f * 3.0517578125e-5f * 1.001f * ql * ml + 1e-35f * (ql + ml) + 1e-36f;
+      const bool all = !(e2 < INFINITY) || !(ql > 1e-15f) || !(ml > 1e-15f);
+      const Scores held(sc, total);
+      float lo = -INFINITY, hi = INFINITY;
+      int nsure = 0, nnear = total;
       if (!all) {
-        const float T = unorder_f32(pick_kth(key, total, a.top_k, pick));
+        // (T may be 0.1 e2 below the top_k-th: the margin of 2.25 covers it)
+        const float T = kth_score(held, a.top_k, 0.1f * e2);
         lo = T - e2;
         hi = T + e2;
+        nsure = held.at_least(hi);
+        nnear = held.at_least(lo) - nsure;
       }
-      // keys become flags: 1 in for certain, 2 near
-      int sure = 0, near = 0;
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t) {
-        key[t] = 0;
-        if (t * kSelThreads + tid < total)
-          key[t] = all ? 2u : v[t] > hi ? 1u : v[t] >= lo ? 2u : 0u;
-        sure += key[t] == 1u;
-        near += key[t] == 2u;
-      }
-      sure = block_count(sure, pick.count);
-      near = block_count(near, pick.count);
-      const int need = a.top_k - sure;
-      if (near > need) {
-        // float64 scores of the near ones, a warp a block, then each near
-        // one's rank among them
-#pragma unroll
-        for (int t = 0; t < kSelKeys; ++t) {
-          uint32_t todo = __ballot_sync(kAll, key[t] == 2u);
-          if (t * kSelThreads + tid < total) ex[t * kSelThreads + tid] = 0;
-          __syncwarp();
+      // near: at least lo (or all) and below hi
+      auto is_near = [&](float x) { return all || (x >= lo && x < hi); };
+      const int need = a.top_k - nsure;
+      if (nnear > need) {
+        // float64 scores of the near ones
+        for (int t0 = 0; t0 < total; t0 += 32) {
+          const int i = t0 + lane;
+          uint32_t todo = __ballot_sync(kAll, i < total && is_near(sc[i]));
           while (todo) {
-            const int j = t * kSelThreads + warp * 32 + __ffs(todo) - 1;
+            const int j = t0 + __ffs(todo) - 1;
             todo &= todo - 1;
             const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
             double x = 0.0;
@@ -531,70 +526,59 @@ __global__ void __launch_bounds__(kSelThreads, 3) select_blocks_kernel(SelectArg
                 x = fma(double(__ldg(a.means + row * D + d)), qg[d], x);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
-            if (lane == 0) ex[j] = order_key(x) + 1;  // 0: not a near one
+            if (lane == 0) ex[j] = order_key(x);
           }
         }
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < kSelKeys; ++t) {
-          uint32_t todo = __ballot_sync(kAll, key[t] == 2u);
+        __syncwarp();
+      }
+      // ---- which to keep: a near one by its rank among the near (or all of
+      // them: the usual case).  Lane t holds the flags of tiles t and t + 32 ----
+      uint32_t flags[2] = {0, 0};
+      for (int t0 = 0; t0 < total; t0 += 32) {
+        const int i = t0 + lane;
+        const float v = i < total ? sc[i] : -INFINITY;
+        bool keep = !all && i < total && v >= (nnear > need ? hi : lo);
+        if (nnear > need) {
+          uint32_t todo = __ballot_sync(kAll, i < total && is_near(v));
           while (todo) {
-            const int bit = __ffs(todo) - 1, j = t * kSelThreads + warp * 32 + bit;
+            const int j = t0 + __ffs(todo) - 1;
             todo &= todo - 1;
             const uint64_t mine = ex[j];
             int ahead = 0;
             for (int x = lane; x < total; x += 32)
-              ahead += ex[x] > mine || (ex[x] == mine && x < j);
+              if (is_near(sc[x])) ahead += ex[x] > mine || (ex[x] == mine && x < j);
             ahead = __reduce_add_sync(kAll, ahead);
-            if (lane == bit && ahead >= need) key[t] = 0;
+            if (i == j) keep = ahead < need;
           }
         }
+        const uint32_t kb = __ballot_sync(kAll, keep);
+        if (lane == ((t0 >> 5) & 31)) (t0 < 1024 ? flags[0] : flags[1]) = kb;
       }
-      // ---- the kept ones, in index order ----
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t) {
-        const uint32_t kb = __ballot_sync(kAll, key[t] != 0);
-        if (lane == 0) pick.count[t * kSelWarps + warp] = __popc(kb);
-      }
-      int id[kSelKeys];
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t) {
-        const int i = t * kSelThreads + tid;
-        id[t] = key[t] != 0 ? (i < kept ? kd[i] : b0 + i - kept) : 0;
-      }
-      __syncthreads();
-      // counts before this warp's, of tile 0 and then from tile to tile
-      int mine = 0;
-#pragma unroll
-      for (int t = 0; t < kSelKeys; ++t) {
-        int add = 0;
-#pragma unroll
-        for (int w = 0; w < kSelWarps; ++w) {
-          const int n = pick.count[t * kSelWarps + w];
-          if (w < warp) mine += n;
-          add += w >= warp ? n : 0;
-        }
-        const uint32_t kb = __ballot_sync(kAll, key[t] != 0);
-        const int to = mine + __popc(kb & ((1u << lane) - 1));
-        if (key[t] != 0) {
-          if (last) {
-            out[g * a.top_k + to] = id[t];
-          } else {
-            sc[to] = v[t];
-            kd[to] = id[t];
+      // ---- move them up, in index order ----
+      int at = 0;
+      for (int t0 = 0; t0 < total; t0 += 32) {
+        const int i = t0 + lane;
+        const uint32_t kb = __shfl_sync(kAll, t0 < 1024 ? flags[0] : flags[1], (t0 >> 5) & 31);
+        const bool keep = kb >> lane & 1;
+        const int to = at + __popc(kb & ((1u << lane) - 1));
+        const int id = keep ? (i < kept ? kd[i] : b0 + i - kept) : 0;
+        if (last) {
+          if (keep) list[to] = id;
+        } else {
+          const float v = keep ? sc[i] : 0.0f;
+          __syncwarp();
+          if (keep) {
+            sc[to] = v;
+            kd[to] = id;
           }
+          __syncwarp();
         }
-        mine += add;
-        if ((t + 1) * kSelThreads >= total) break;
+        at += __popc(kb);
       }
-      __syncthreads();
     }
     kept = min(total, a.top_k);
     if (last) return;
-    if (X > 1)
-      cluster_barrier();  // the first CTA has picked: its memory may be written
-    else
-      __syncthreads();
+    barrier();  // every CTA has picked: its memory may be written
   }
 }
 
@@ -615,15 +599,6 @@ struct SparseArgs {
 };
 
 constexpr int kFewWarps = 8;
-
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 // Partial results of the warps and of the CTA: unnormalised O, maximum, sum.
 template <int D>
@@ -1205,32 +1180,26 @@ int launch_cluster(void (*kernel)(A), const A& a, int64_t units, int X, int thre
   return PKV_OK;
 }
 
-template <int D, int GQ>
-int select_shape(SelectArgs a, int64_t segs, cudaStream_t stream) {
+template <int D, int X>
+int select_shape(const SelectArgs& a, int64_t units, cudaStream_t stream) {
   static std::mutex mu;
   static int done[kMaxDevices] = {};
-  if (smem_opt_in(done, mu, select_blocks_kernel<D, GQ>, select_bytes(D, GQ, kMaxTopK)) <= 0) {
+  if (smem_opt_in(done, mu, select_blocks_kernel<D, X>, select_bytes(D, X, kMaxTopK)) <= 0) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
-  a.packs = (a.groups + GQ - 1) / GQ;
-  const int64_t units = segs * a.packs;
-  // a cluster while the groups leave SMs idle and the keys could make blocks
-  // enough to share
-  int X = 1;
-  const int64_t blocks = a.kv_rows / a.block;
-  if (GQ == 1)
-    while (X < kSelCluster && units * X * 2 <= sm_count() && blocks >= int64_t(X) * 64) X *= 2;
-  return launch_cluster(select_blocks_kernel<D, GQ>, a, units, X, kSelThreads,
-                        select_bytes(D, GQ, a.top_k), stream);
+  return launch_cluster(select_blocks_kernel<D, X>, a, units, X, kSelThreads,
+                        select_bytes(D, X, a.top_k), stream);
 }
 
-// Two groups share a segment's means where that leaves four CTAs for every SM.
+// Eight CTAs a cluster where that leaves room for all of them at once (a
+// cluster shares a few SMs of one GPC, so not every SM can be used), else four.
 template <int D>
-int launch_select(const SelectArgs& a, int64_t segs, cudaStream_t stream) {
-  if (a.groups >= 2 && segs * ((a.groups + 1) / 2) >= int64_t(sm_count()) * 4)
-    return select_shape<D, 2>(a, segs, stream);
-  return select_shape<D, 1>(a, segs, stream);
+int launch_select(SelectArgs a, int64_t segs, cudaStream_t stream) {
+  a.packs = (a.groups + kSelGroups - 1) / kSelGroups;
+  const int64_t units = segs * a.packs;
+  if (units * 8 <= sm_count()) return select_shape<D, 8>(a, units, stream);
+  return select_shape<D, 4>(a, units, stream);
 }
 
 template <int D>
