@@ -221,10 +221,10 @@ struct Scores {
     int c = 0;
     if (held) {
 #pragma unroll
-      for (int t = 0; t < kSelHeld; ++t) c += v[t] >= x;
-    } else {
-      for (int i = threadIdx.x & 31; i < n; i += 32) c += s[i] >= x;
+      for (int t = 0; t < kSelHeld; ++t) c += __popc(__ballot_sync(0xffffffffu, v[t] >= x));
+      return c;
     }
+    for (int i = threadIdx.x & 31; i < n; i += 32) c += s[i] >= x;
     return __reduce_add_sync(0xffffffffu, c);
   }
   // Least score at or above x.
@@ -511,6 +511,59 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
       // near: at least lo (or all) and below hi
       auto is_near = [&](float x) { return all || (x >= lo && x < hi); };
       const int need = a.top_k - nsure;
+      // exact score of the block at index j of this round's scores
+      auto score64 = [&](int j) {
+        const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
+        double x = 0.0;
+        if (row >= 0 && row < a.means_rows)
+#pragma unroll
+          for (int d = 0; d < D; d += 32)
+            x = fma(double(__ldg(a.means + row * D + d + lane)), qg[d + lane], x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
+        return order_key(x);
+      };
+      if (!all && held.held && kept == 0 && last && nnear <= 32) {
+        // ---- the usual case: scores in registers, few near ones.  Bit p of
+        // `in`: the p-th near one is in the list ----
+        uint32_t in = 0xffffffffu;
+        if (nnear > need) {
+          int* idx = reinterpret_cast<int*>(ex);  // the near ones' indices
+          int at = 0;
+#pragma unroll
+          for (int t = 0; t < kSelHeld; ++t) {
+            const bool is = is_near(held.v[t]);
+            const uint32_t nb = __ballot_sync(kAll, is);
+            if (is) idx[at + __popc(nb & ((1u << lane) - 1))] = t * 32 + lane;
+            at += __popc(nb);
+          }
+          __syncwarp();
+          uint64_t mine = 0;  // lane p: the p-th one's score
+          for (int p = 0; p < nnear; ++p) {
+            const uint64_t x = score64(idx[p]);
+            if (lane == p) mine = x;
+          }
+          int ahead = 0;
+          for (int p = 0; p < nnear; ++p) {
+            const uint64_t x = __shfl_sync(kAll, mine, p);
+            ahead += x > mine || (x == mine && p < lane);
+          }
+          in = __ballot_sync(kAll, lane < nnear && ahead < need);
+        }
+        int at = 0, seen = 0;
+#pragma unroll
+        for (int t = 0; t < kSelHeld; ++t) {
+          const uint32_t below = (1u << lane) - 1;
+          const bool is = is_near(held.v[t]);
+          const uint32_t nb = __ballot_sync(kAll, is);
+          const bool keep = held.v[t] >= hi || (is && (in >> (seen + __popc(nb & below)) & 1));
+          const uint32_t kb = __ballot_sync(kAll, keep);
+          if (keep) list[at + __popc(kb & below)] = t * 32 + lane;
+          at += __popc(kb);
+          seen += __popc(nb);
+        }
+        continue;
+      }
       if (nnear > need) {
         // float64 scores of the near ones
         for (int t0 = 0; t0 < total; t0 += 32) {
@@ -519,20 +572,14 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
           while (todo) {
             const int j = t0 + __ffs(todo) - 1;
             todo &= todo - 1;
-            const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
-            double x = 0.0;
-            if (row >= 0 && row < a.means_rows)
-              for (int d = lane; d < D; d += 32)
-                x = fma(double(__ldg(a.means + row * D + d)), qg[d], x);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
-            if (lane == 0) ex[j] = order_key(x);
+            const uint64_t x = score64(j);
+            if (lane == 0) ex[j] = x;
           }
         }
         __syncwarp();
       }
       // ---- which to keep: a near one by its rank among the near (or all of
-      // them: the usual case).  Lane t holds the flags of tiles t and t + 32 ----
+      // them).  Lane t holds the flags of tiles t and t + 32 ----
       uint32_t flags[2] = {0, 0};
       for (int t0 = 0; t0 < total; t0 += 32) {
         const int i = t0 + lane;
