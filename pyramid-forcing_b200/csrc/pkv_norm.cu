@@ -642,47 +642,55 @@ __global__ void __launch_bounds__(kNormThreads) norm_cols_kernel(NormBwdArgs a) 
 }
 
 // Column sums of a group's parts, in a fixed order, rounded to the weight's
-// type.  32 columns x 32 slices of the parts a block, four parts of a slice on
-// their way at once; the slices meet in shared memory.
-template <typename TW>
-__global__ void __launch_bounds__(1024)
+// type: VC columns a thread, 32 threads x 8 slices of the parts a block, eight
+// parts of a slice on their way at once; the slices meet in shared memory.
+template <typename TW, int VC>
+__global__ void __launch_bounds__(256)
     norm_parts_kernel(const float* part, int parts, int C, TW* dw, TW* db) {
-  __shared__ float sm[2][32][33];
+  constexpr int kCols = 32 * VC, kMany = 8;
+  __shared__ float sm[2][8][kCols];
   const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5;
-  const int c = blockIdx.y * 32 + lane;
+  const int c = blockIdx.y * kCols + lane * VC;
   const int64_t grp = blockIdx.x;
-  float sw = 0.0f, sb = 0.0f;
+  float s[2][VC] = {};
   if (c < C) {
     const float* q = part + grp * parts * 2 * int64_t(C) + c;
-    for (int p = sl; p < parts; p += 128) {
-      float w[4], b[4];
+    for (int p = sl; p < parts; p += 8 * kMany) {
+      Vec<float, VC> v[kMany][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = p + 32 * i < parts;
-        w[i] = in ? q[int64_t(p + 32 * i) * 2 * C] : 0.0f;
-        b[i] = in ? q[int64_t(p + 32 * i) * 2 * C + C] : 0.0f;
-      }
-      sw += (w[0] + w[1]) + (w[2] + w[3]);
-      sb += (b[0] + b[1]) + (b[2] + b[3]);
+      for (int i = 0; i < kMany; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (p + 8 * i < parts) v[i][k] = ld_vec<float, VC>(q + (int64_t(p + 8 * i) * 2 + k) * C);
+#pragma unroll
+      for (int i = 0; i < kMany; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (p + 8 * i < parts)
+#pragma unroll
+            for (int e = 0; e < VC; ++e) s[k][e] += v[i][k].v[e];
     }
   }
-  sm[0][sl][lane] = sw;
-  sm[1][sl][lane] = sb;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < VC; ++e) sm[k][sl][lane * VC + e] = s[k][e];
   __syncthreads();
-  // warp x adds column x: lanes are the slices
-  sw = warp_sum(sm[0][lane][sl]);
-  sb = warp_sum(sm[1][lane][sl]);
-  const int col = blockIdx.y * 32 + sl;
-  if (lane == 0 && col < C) {
-    if (dw) dw[grp * C + col] = from_f32<TW>(sw);
-    if (db) db[grp * C + col] = from_f32<TW>(sb);
+  for (int i = threadIdx.x; i < 2 * kCols; i += 256) {
+    const int k = i / kCols, col = i - k * kCols;
+    TW* out = k ? db : dw;
+    if (out == nullptr || blockIdx.y * kCols + col >= C) continue;
+    float t = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) t += sm[k][x][col];
+    out[grp * C + blockIdx.y * kCols + col] = from_f32<TW>(t);
   }
 }
 
-// Blocks that share a group's rows: about `per_sm` an SM over all groups, at
-// least `least` rows each.
+// Blocks that share a group's rows: at most `per_sm` an SM over all groups (one
+// more would be a second wave), at least `least` rows each.
 int64_t row_parts(int64_t rows_per_group, int64_t groups, int per_sm, int least) {
-  const int64_t want = (int64_t(sm_count()) * per_sm + groups - 1) / groups;
+  const int64_t want = int64_t(sm_count()) * per_sm / groups;
   const int64_t most = (rows_per_group + least - 1) / least;
   const int64_t p = want < most ? want : most;
   return p < 1 ? 1 : p;
@@ -835,9 +843,15 @@ int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream
   else
     rc = launch_bwd<TX, TW, 1>(a, groups, s);
   if (rc != PKV_OK || a.part == nullptr) return rc;
-  const dim3 grid(unsigned(groups), unsigned((a.C + 31) / 32));
-  norm_parts_kernel<TW><<<grid, 1024, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
-                                             static_cast<TW*>(db));
+  if (a.C % 4 == 0 && vec_ok(a.part, 0, 16, 1)) {
+    const dim3 grid(unsigned(groups), unsigned((a.C + 127) / 128));
+    norm_parts_kernel<TW, 4><<<grid, 256, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
+                                                  static_cast<TW*>(db));
+  } else {
+    const dim3 grid(unsigned(groups), unsigned((a.C + 31) / 32));
+    norm_parts_kernel<TW, 1><<<grid, 256, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
+                                                  static_cast<TW*>(db));
+  }
   return launch_status();
 }
 

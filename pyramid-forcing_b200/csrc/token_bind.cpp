@@ -92,9 +92,11 @@ std::tuple<Tensor, Tensor, Tensor> op_layer_norm(Tensor x, std::optional<Tensor>
   const NormParams p = norm_params(op, x, weight, bias);
   const Tensor xx = dense_rows(x);
   const Tensor y = at::empty(x.sizes(), x.options());
-  const auto f32 = x.options().dtype(at::kFloat);
-  const Tensor mean = at::empty({stats ? x.size(0) : 0}, f32);
-  const Tensor rstd = at::empty({stats ? x.size(0) : 0}, f32);
+  Tensor mean, rstd;
+  if (stats) {
+    mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    rstd = at::empty_like(mean);
+  }
   check_rc(pkv_layer_norm(ptr(xx), xx.stride(0), ptr(p.w), ptr(p.b), dt, p.wtype, x.size(0),
                           x.size(1), p.groups, float(eps), one_plus, mut(y), y.stride(0),
                           static_cast<float*>(mut(mean)), static_cast<float*>(mut(rstd)),
@@ -262,10 +264,22 @@ Tensor rot_rows(const Tensor& x) {
   return x.dim() == 3 ? x : x.reshape({n, x.size(-2), x.size(-1)});
 }
 
+// Positions of any leading shape and whole-number type as int64 [tokens, axes].
+Tensor pos_rows(const Tensor& q, const Tensor& positions, int64_t axes) {
+  const int64_t per = q.size(-2) * q.size(-1), n = per > 0 ? q.numel() / per : 0;
+  Tensor p = positions.scalar_type() == at::kLong ? positions : positions.to(at::kLong);
+  TORCH_CHECK(axes >= 1 && (per == 0 || p.numel() == n * axes),
+              "pkv_rotary: positions must hold ", axes, " axes for each of ", n, " tokens");
+  if (p.dim() != 2 || p.size(1) != axes) p = p.reshape({p.numel() / axes, axes});
+  return p.contiguous();
+}
+
 std::tuple<Tensor, Tensor> op_rotary_apply(Tensor q, std::optional<Tensor> k, Tensor positions,
-                                           Tensor inv_freq, std::optional<Tensor> axis, bool half,
-                                           double scale) {
+                                           int64_t axes, Tensor inv_freq,
+                                           std::optional<Tensor> axis, bool half, double scale) {
+  TORCH_CHECK(q.dim() >= 3, "pkv_rotary: q must be [..., heads, dim]");
   const bool two = k.has_value() && k->defined();
+  positions = pos_rows(q, positions, axes);
   auto [qo, ko] = op_rotary(rot_rows(q), two ? std::optional<Tensor>(rot_rows(*k)) : std::nullopt,
                             positions, inv_freq, axis, half, scale, false);
   return {qo.view(q.sizes()), two ? ko.view(k->sizes()) : ko};
@@ -273,9 +287,11 @@ std::tuple<Tensor, Tensor> op_rotary_apply(Tensor q, std::optional<Tensor> k, Te
 
 struct RotaryFn : torch::autograd::Function<RotaryFn> {
   static variable_list forward(AutogradContext* ctx, Tensor q, std::optional<Tensor> k,
-                               Tensor positions, Tensor inv_freq, std::optional<Tensor> axis,
-                               bool half, double scale) {
-    auto [qo, ko] = op_rotary_apply(q, k, positions, inv_freq, axis, half, scale);
+                               Tensor positions, int64_t axes, Tensor inv_freq,
+                               std::optional<Tensor> axis, bool half, double scale) {
+    TORCH_CHECK(q.dim() >= 3, "pkv_rotary: q must be [..., heads, dim]");
+    positions = pos_rows(q, positions, axes);
+    auto [qo, ko] = op_rotary_apply(q, k, positions, axes, inv_freq, axis, half, scale);
     ctx->save_for_backward({positions, inv_freq, axis.value_or(Tensor())});
     ctx->saved_data["half"] = half;
     ctx->saved_data["scale"] = scale;
@@ -292,7 +308,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     Tensor dq = grads[0], dk = two ? grads[1] : Tensor();
     if (!ctx->needs_input_grad(0)) dq = Tensor();
     if (two && !ctx->needs_input_grad(1)) dk = Tensor();
-    variable_list out(7);
+    variable_list out(8);
     const Tensor first = dq.defined() ? dq : dk;
     if (!first.defined()) return out;
     const bool both = dq.defined() && dk.defined();
@@ -307,16 +323,17 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
 };
 
 std::tuple<Tensor, Tensor> op_rotary_autograd(Tensor q, std::optional<Tensor> k, Tensor positions,
-                                              Tensor inv_freq, std::optional<Tensor> axis,
-                                              bool half, double scale) {
+                                              int64_t axes, Tensor inv_freq,
+                                              std::optional<Tensor> axis, bool half,
+                                              double scale) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
               "pkv_rotary_apply: inv_freq has no gradient here; detach it");
   if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) {
-    const variable_list r = RotaryFn::apply(q, k, positions, inv_freq, axis, half, scale);
+    const variable_list r = RotaryFn::apply(q, k, positions, axes, inv_freq, axis, half, scale);
     return {r[0], r.size() > 1 ? r[1] : Tensor()};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return op_rotary_apply(q, k, positions, inv_freq, axis, half, scale);
+  return op_rotary_apply(q, k, positions, axes, inv_freq, axis, half, scale);
 }
 
 // ---- block-sparse attention ----------------------------------------------------
@@ -453,8 +470,8 @@ using namespace pkv_torch;
 
 TORCH_LIBRARY_FRAGMENT(adahead, m) {
   m.def("pkv_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool one_plus) -> Tensor");
-  m.def("pkv_rotary_apply(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, Tensor? axis, "
-        "bool half, float scale) -> (Tensor, Tensor)");
+  m.def("pkv_rotary_apply(Tensor q, Tensor? k, Tensor positions, int axes, Tensor inv_freq, "
+        "Tensor? axis, bool half, float scale) -> (Tensor, Tensor)");
   m.def("pkv_layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool one_plus, "
         "bool stats) -> (Tensor, Tensor, Tensor)");
   m.def("pkv_layer_norm_backward(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, "

@@ -27,6 +27,18 @@ def ops():
     return torch.ops.adahead
 
 
+_OVERLOADS: dict = {}
+
+
+def overload(name: str):
+    """The resolved overload of ``torch.ops.adahead.<name>`` (a lookup by name
+    costs as much host time as a small kernel takes)."""
+    op = _OVERLOADS.get(name)
+    if op is None:
+        op = _OVERLOADS[name] = getattr(ops(), name).default
+    return op
+
+
 def scatter_copy(src_ptrs, lengths, offsets, dst, col_dim: int) -> None:
     ops().scatter_copy(src_ptrs, lengths, offsets, dst, int(col_dim))
 

@@ -32,4 +32,4 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
             raise ValueError("layer_norm: weight and bias must have one type")
         if weight.shape != bias.shape:
             weight, bias = torch.broadcast_tensors(weight, bias)
-    return _ops.ops().pkv_norm(x, weight, bias, eps, one_plus)
+    return _ops.overload("pkv_norm")(x, weight, bias, eps, one_plus)

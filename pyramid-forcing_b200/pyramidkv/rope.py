@@ -118,16 +118,18 @@ def rotary_apply(x, positions: torch.Tensor, inv_freq: torch.Tensor,
     for t in (q, k):
         if t is not None and (not t.is_cuda or t.dim() < 3):
             raise ValueError("rotary_apply: x must be a [..., heads, D] CUDA tensor")
-    lead = q.shape[:-2]
+    lead, shape = q.shape[:-2], positions.shape
     if k is not None and (k.shape[:-2] != lead or k.shape[-1] != q.shape[-1]):
         raise ValueError("rotary_apply: q and k must agree in tokens and head size")
     if positions.is_floating_point():
         raise ValueError("rotary_apply: positions must be whole numbers")
-    if positions.shape != lead and positions.shape[:-1] != lead:
+    if shape == lead:
+        axes = 1
+    elif shape[:-1] == lead:
+        axes = shape[-1]
+    else:
         raise ValueError("rotary_apply: positions must have x's leading shape, with or without "
                          "a dimension of axes behind it")
-    tokens = math.prod(lead)
-    axes = 1 if positions.shape == lead else positions.shape[-1]
-    pos = positions.reshape(tokens, axes).to(torch.int64).contiguous()
-    out = _ops.ops().pkv_rotary_apply(q, k, pos, inv_freq, axis, layout == "half", scale)
+    out = _ops.overload("pkv_rotary_apply")(q, k, positions, axes, inv_freq, axis,
+                                            layout == "half", scale)
     return out[0] if k is None else out

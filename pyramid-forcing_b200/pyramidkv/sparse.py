@@ -28,7 +28,7 @@ def block_means(k: torch.Tensor, cu_seqlens_k: torch.Tensor, block: int = 64) ->
     cu_seqlens_k[s + 1], its block j the row cu_seqlens_k[s] // block + s + j
     of the table.  Rows between segments and behind the last are zero.
     """
-    return _ops.ops().pkv_block_means(k, cu_seqlens_k, int(block), True)
+    return _ops.overload("pkv_block_means")(k, cu_seqlens_k, int(block), True)
 
 
 def select_blocks(q: torch.Tensor, means: torch.Tensor, cu_seqlens_k: torch.Tensor, kv_rows: int,
@@ -38,7 +38,7 @@ def select_blocks(q: torch.Tensor, means: torch.Tensor, cu_seqlens_k: torch.Tens
     every group of query rows its top_k blocks by score (the group's queries
     summed, times the block's mean), equal scores by index, listed ascending,
     -1 behind the last.  kv_rows: rows of the k that ``means`` was made from."""
-    return _ops.ops().pkv_select_blocks(q, means, cu_seqlens_k, int(kv_rows), int(num_chunks),
+    return _ops.overload("pkv_select_blocks")(q, means, cu_seqlens_k, int(kv_rows), int(num_chunks),
                                         int(rows_per_chunk), int(top_k), int(query_block),
                                         int(block))
 
@@ -55,7 +55,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise RuntimeError("pkv_block_attention has no gradient: call it under torch.no_grad()")
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
-    return _ops.ops().pkv_block_attention(q, k, v, cu_seqlens_k, int(num_chunks),
+    return _ops.overload("pkv_block_attention")(q, k, v, cu_seqlens_k, int(num_chunks),
                                           int(rows_per_chunk), blocks, int(query_block),
                                           int(block), scale, status)
 
@@ -68,7 +68,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """(output, blocks): select_blocks and block_attention, and block_means
     where the caller does not keep the table."""
     if means is None:
-        means = _ops.ops().pkv_block_means(k, cu_seqlens_k[:num_chunks * q.shape[1] + 1],
+        means = _ops.overload("pkv_block_means")(k, cu_seqlens_k[:num_chunks * q.shape[1] + 1],
                                            int(block), False)
     blocks = select_blocks(q, means, cu_seqlens_k, k.numel() // q.shape[-1], num_chunks,
                            rows_per_chunk, top_k, query_block=query_block, block=block)
