@@ -46,6 +46,12 @@ class WanConfig:
     patch: tuple = (1, 2, 2)
     eps: float = 1e-6
     text_len: int = 512
+    # layer norms and their modulation as one kernel each (pyramidkv.norm); the
+    # default is torch's, rounded to bf16 after every step
+    fused_norm: bool = False
+    # blocks of 64 keys that each group of 128 queries attends in the
+    # self-attention (MegaCache.attend(top_blocks=)); 0: the whole cache
+    top_blocks: int = 0
 
 
 def rope_table(head_dim: int, max_len: int = 1024) -> torch.Tensor:
@@ -128,6 +134,16 @@ class CausalWanDiT:
             self.cross.append((kh, vh))
         self.cross_cu = torch.arange(0, (H + 1) * n, n, dtype=torch.int32, device=self.device)
 
+    def _norm(self, x, weight, bias, one_plus=True):
+        """LN(x) * (1 + weight) + bias, or LN(x) * weight + bias."""
+        c = self.cfg
+        if c.fused_norm:
+            from pyramidkv.norm import layer_norm
+            return layer_norm(x, weight, bias, eps=c.eps, one_plus=one_plus)
+        if one_plus:
+            return F.layer_norm(x, (c.dim,), eps=c.eps) * (1 + weight) + bias
+        return F.layer_norm(x, (c.dim,), weight, bias, eps=c.eps)
+
     # -- one block ---------------------------------------------------------------
     def forward(self, latent: torch.Tensor, t: float, caches, current_start: int,
                 mode: str) -> torch.Tensor:
@@ -154,7 +170,7 @@ class CausalWanDiT:
         scale = hd ** -0.5
         for li, p in enumerate(self.layers):
             m = (p["mod"] + e0)[0]                      # [6, d]
-            y = F.layer_norm(x, (d,), eps=c.eps) * (1 + m[1]) + m[0]
+            y = self._norm(x, m[1], m[0])
             qkv = F.linear(y, p["qkv_w"], p["qkv_b"])
             q = _rms(qkv[:, :d], p["nq"], c.eps).view(1, L, H, hd)
             k = _rms(qkv[:, d:2 * d], p["nk"], c.eps).view(1, L, H, hd)
@@ -162,20 +178,20 @@ class CausalWanDiT:
             rq = causal_rope_apply(q, None, self.freqs, start_frame=current_start // (gh * gw),
                                    grid_int=grid)
             caches[li].update(k, v, current_start, cache_update_mode=mode)
-            a = caches[li].attend(rq, current_start)
+            a = caches[li].attend(rq, current_start, top_blocks=c.top_blocks or None)
             x = x + F.linear(a.view(L, d), p["o_w"], p["o_b"]) * m[2]
             # cross-attention over the cached text K/V
-            y = F.layer_norm(x, (d,), p["n3_w"], p["n3_b"], eps=c.eps)
+            y = self._norm(x, p["n3_w"], p["n3_b"], one_plus=False)
             cq = _rms(F.linear(y, p["cq_w"], p["cq_b"]), p["cnq"], c.eps).view(L, H, hd)
             kh, vh = self.cross[li]
             ca = ops.pkv_attention(cq, kh, vh, self.cross_cu, 1, L, scale)
             x = x + F.linear(ca.view(L, d), p["co_w"], p["co_b"])
             # feed-forward
-            y = F.layer_norm(x, (d,), eps=c.eps) * (1 + m[4]) + m[3]
+            y = self._norm(x, m[4], m[3])
             h1 = F.gelu(F.linear(y, p["f1_w"], p["f1_b"]), approximate="tanh")
             x = x + F.linear(h1, p["f2_w"], p["f2_b"]) * m[5]
         hm = (self.head_mod + e.view(1, 1, d))[0]
-        y = F.layer_norm(x, (d,), eps=c.eps) * (1 + hm[1]) + hm[0]
+        y = self._norm(x, hm[1], hm[0])
         out = F.linear(y, self.head_w, self.head_b)       # [L, C * 4]
         return out.view(Fr, gh, gw, C, 2, 2).permute(3, 0, 1, 4, 2, 5).reshape(1, C, Fr, Hh, Ww)
 

@@ -104,6 +104,43 @@ inline int launch_status() {
   return e == cudaSuccess ? PKV_OK : PKV_ELAUNCH;
 }
 
+// Programmatic dependent launch.  A kernel that begins with grid_wait() may be
+// launched early by launch_clusters(): its blocks come to the SMs while the kernel
+// before it in the stream still runs (once all of that one's blocks have called
+// grid_release() or ended) and stop at grid_wait() until that one is complete
+// and its writes are visible.  It hides the launch and the ramp.
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_release() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launch in clusters of X blocks along x (X = 1: none); `early`: behind the
+// previous kernel of the stream as above.
+template <typename... P, typename... A>
+inline int launch_clusters(void (*kernel)(P...), dim3 grid, int X, bool early, int threads,
+                           size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(X);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) != cudaSuccess) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  return PKV_OK;
+}
+
 constexpr int kMaxDevices = 64;
 
 // A positive value computed once per device, on the first call made with

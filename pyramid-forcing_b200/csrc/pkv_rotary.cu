@@ -58,10 +58,14 @@ struct RotArgs {
   float scale, sign;
 };
 
+// Eight blocks an SM (32 registers; a few spilled words) keep enough loads on
+// their way: 65521 tokens of 24 heads x 128 fp16, a quarter of them turned,
+// take 127 us a pass, 806 MB at 6.3 TB/s, 0.97 of the copy rate; with 36
+// registers and 7 blocks 133 us, four units a thread at once (80 registers) 222.
 // kPair: a unit is V pairs out of two vectors (half layout, and interleaved
 // single elements); else it is one vector of V / 2 interleaved pairs.
 template <typename T, int V, bool kHalf>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 8) rotary_kernel(RotArgs a) {
   constexpr bool kPair = kHalf || V == 1;
   __shared__ float2 tab[kRotTable];
   const int64_t t0 = blockIdx.x * int64_t(a.tile);

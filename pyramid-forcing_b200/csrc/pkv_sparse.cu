@@ -53,22 +53,27 @@ __device__ __forceinline__ uint32_t word(const uint4& w, int i) {
 // ---------------------------------------------------------------------------
 // Block means
 // ---------------------------------------------------------------------------
-// A warp a table row: 16 (D = 128) or 8 lanes a key, 8 elements each.  Four
-// keys are added in fp32 (exact unless their exponents differ by 14) before a
-// float64 add, which keeps the conversions off the critical pipe.
-template <int D>
+// W warps a table row (1, or 4 where there are few rows: each then has its
+// quarter of the keys on its way at once); 16 (D = 128) or 8 lanes a key, 8
+// elements each.  Four keys are added in fp32 (exact unless their exponents
+// differ by 14) before a float64 add, which keeps the conversions off the
+// critical pipe.  663 000 keys of 128 take 34 us, 5.0 TB/s; 2.8 M keys 113 us,
+// 6.3 TB/s.
+template <int D, int W>
 __global__ void __launch_bounds__(256)
     block_means_kernel(const uint16_t* __restrict__ k, int64_t kv_rows,
                        const int32_t* __restrict__ cu, int n_seg, int block,
                        float* __restrict__ means, int64_t rows, int zero_rest) {
-  constexpr int kLanes = D / 8, kKeys = 32 / kLanes;
-  const int lane = threadIdx.x & 31;
+  constexpr int kLanes = D / 8, kKeys = 32 / kLanes, kRows = 8 / W;  // rows of a block
+  __shared__ double part[W > 1 ? 8 : 1][D];
+  grid_release();  // the selection may queue up behind this grid
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % W;
   const int sub = lane / kLanes, d0 = (lane % kLanes) * 8;
-  const int64_t step = int64_t(gridDim.x) * (blockDim.x >> 5);
   const int64_t used = int64_t(cu[n_seg]) / block + n_seg;
-  for (int64_t row = blockIdx.x * int64_t(blockDim.x >> 5) + (threadIdx.x >> 5); row < rows;
-       row += step) {
-    if (row >= used && !zero_rest) break;
+  for (int64_t row0 = blockIdx.x * int64_t(kRows); row0 < rows;
+       row0 += int64_t(gridDim.x) * kRows) {
+    if (row0 >= used && !zero_rest) break;  // (the whole block)
+    const int64_t row = row0 + warp / W;
     // last segment whose first row is <= row
     int lo = 0, hi = n_seg - 1;
     while (lo < hi) {
@@ -81,21 +86,16 @@ __global__ void __launch_bounds__(256)
     const SegView sg = segment(cu, lo, kv_rows);
     const int64_t j = row - (int64_t(cu[lo]) / block + lo);
     const int64_t first = j * block;
-    float* out = means + row * D;
-    if (j < 0 || first >= sg.len) {  // no block has this row
-      if (zero_rest)
-        for (int d = lane * 4; d < D; d += 128)
-          *reinterpret_cast<float4*>(out + d) = make_float4(0.f, 0.f, 0.f, 0.f);
-      continue;
-    }
-    const int n = min(int64_t(block), sg.len - first);
+    const bool there = row < rows && j >= 0 && first < sg.len;  // a block has this row
+    const int n = there ? int(min(int64_t(block), sg.len - first)) : 0;
     const uint16_t* p = k + (sg.start + first) * D + d0;
     double acc[8] = {};
-    for (int r = sub; r < n; r += 8 * kKeys) {
-      uint4 w[8];  // 8 loads a lane on their way: 4 KB a warp
+    const int per = block / W, end = min(n, (w + 1) * per);
+    for (int r = w * per + sub; r < end; r += 8 * kKeys) {
+      uint4 v[8];  // 8 loads a lane on their way: 4 KB a warp
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        w[i] = r + i * kKeys < n
+        v[i] = r + i * kKeys < end
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kKeys) * D))
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256)
           float lo4[4], hi4[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const uint32_t u = word(w[i + x], e);
+            const uint32_t u = word(v[i + x], e);
             lo4[x] = bf16_bits_to_f32(u & 0xffffu);
             hi4[x] = __uint_as_float(u & 0xffff0000u);
           }
@@ -117,14 +117,28 @@ __global__ void __launch_bounds__(256)
     for (int o = kLanes; o < 32; o <<= 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
-    if (sub == 0) {
-      const double inv = 1.0 / double(n);
-      const bool pow2 = (n & (n - 1)) == 0;  // then the product is exact
-      float m[8];
+    if constexpr (W > 1) {
+      if (sub == 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m[e] = float(pow2 ? acc[e] * inv : acc[e] / double(n));
-      *reinterpret_cast<float4*>(out + d0) = make_float4(m[0], m[1], m[2], m[3]);
-      *reinterpret_cast<float4*>(out + d0 + 4) = make_float4(m[4], m[5], m[6], m[7]);
+        for (int e = 0; e < 8; ++e) part[warp][d0 + e] = acc[e];
+      __syncthreads();
+      if (w == 0 && sub == 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          for (int x = 1; x < W; ++x) acc[e] += part[warp + x][d0 + e];
+      __syncthreads();
+    }
+    if (w != 0 || sub != 0 || row >= rows) continue;
+    float m[8];
+    const bool pow2 = (n & (n - 1)) == 0;  // then the product is exact
+    const double inv = 1.0 / double(max(n, 1));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      m[e] = n == 0 ? 0.0f : float(pow2 ? acc[e] * inv : acc[e] / double(n));
+    if (there || zero_rest) {
+      float* out = means + row * D + d0;
+      *reinterpret_cast<float4*>(out) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(out + 4) = make_float4(m[4], m[5], m[6], m[7]);
     }
   }
 }
@@ -307,6 +321,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
   float* score = qf + kSelGroups * kQs;                            // [kMine][cap]
   int* kid = reinterpret_cast<int*>(score + kMine * cap);          // [kMine][top_k] kept earlier
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_wait();
+  grid_release();  // the attention of few rows may queue up behind this grid
   const int rank = X > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / X;
   const int s = unit / a.packs, g0 = (unit - s * a.packs) * kSelGroups;
@@ -671,6 +687,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
   extern __shared__ __align__(16) uint8_t raw[];
   FewSmem<D>& sm = *reinterpret_cast<FewSmem<D>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_wait();
   const int X = int(cluster_size()), rank = int(cluster_rank());
   const int unit = blockIdx.x / X;
   const int s = unit / a.groups, grp = unit - s * a.groups;
@@ -933,7 +950,6 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   const int ch = s / a.H, h = s - ch * a.H;
   const int r0 = grp * a.query_block;
   const int nr = min(a.query_block, a.rows_per_chunk - r0);
-  const SegView sg = segment(a.cu, s, a.kv_rows);
 
   if (threadIdx.x == 0) {
     sm.abort = 0;
@@ -948,6 +964,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     mbar_init(&sm.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     su32(&sm.tmem_base)),
+                 "r"(256));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  const SegView sg = segment(a.cu, s, a.kv_rows);
   if (warp == 1) {  // the listed 64-key halves that hold keys, in order
     const int nblk = (sg.len + a.block - 1) / a.block, per = a.block / 64;
     const int32_t* lst = a.blocks + int64_t(unit) * a.top_k;
@@ -968,12 +991,6 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       n += total;
     }
     if (lane == 0) sm.halves = n;
-  }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     su32(&sm.tmem_base)),
-                 "r"(256));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
@@ -1097,16 +1114,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         break;
       }
       tc_fence_after();
-      uint32_t sr[2][32];
-      tmem_ld32(s_tm, sr[0]);
-      tmem_ld32(s_tm + 32, sr[1]);
-      tmem_wait_ld();
       if (partial) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (q * 32 + e >= valid) sr[q][e] = __float_as_uint(-INFINITY);
         if (!mbar_wait(&sm.v_full[b], par, abort, a.status)) {
           ok = false;
           break;
@@ -1120,6 +1128,22 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                   make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+      }
+      if (quad * 32 >= nr) {  // no row of this warp is the group's: P and O may
+        __syncwarp();         // hold anything there
+        if (lane == 0) mbar_arrive(&sm.p_full[b]);
+        continue;
+      }
+      uint32_t sr[2][32];
+      tmem_ld32(s_tm, sr[0]);
+      tmem_ld32(s_tm + 32, sr[1]);
+      tmem_wait_ld();
+      if (partial) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (q * 32 + e >= valid) sr[q][e] = __float_as_uint(-INFINITY);
       }
       const float m_new = fmaxf(m_ref, row_max64(sr) * sc);
       const bool grow = m_new > m_ref + kRescaleThreshold || j == 0;
@@ -1204,27 +1228,12 @@ bool shape_ok(int num_chunks, int H, int rows_per_chunk, int query_block, int bl
          query_block <= kBM && (block == 64 || block == 128) && top_k >= 1;
 }
 
-// One-dimensional grid in clusters of X.
+// One-dimensional grid of units in clusters of X.
 template <typename A>
-int launch_cluster(void (*kernel)(A), const A& a, int64_t units, int X, int threads, size_t smem,
-                   cudaStream_t stream) {
+int launch_units(void (*kernel)(A), const A& a, int64_t units, int X, bool early, int threads,
+                 size_t smem, cudaStream_t stream) {
   if (units * X >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(units * X));
-  cfg.blockDim = dim3(unsigned(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = unsigned(X);
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
-    cudaGetLastError();
-    return PKV_ELAUNCH;
-  }
-  return PKV_OK;
+  return launch_clusters(kernel, dim3(unsigned(units * X)), X, early, threads, smem, stream, a);
 }
 
 template <int D, int X>
@@ -1235,8 +1244,8 @@ int select_shape(const SelectArgs& a, int64_t units, cudaStream_t stream) {
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
-  return launch_cluster(select_blocks_kernel<D, X>, a, units, X, kSelThreads,
-                        select_bytes(D, X, a.top_k), stream);
+  return launch_units(select_blocks_kernel<D, X>, a, units, X, true, kSelThreads,
+                      select_bytes(D, X, a.top_k), stream);
 }
 
 // Eight CTAs a cluster where that leaves room for all of them at once (a
@@ -1263,7 +1272,7 @@ int launch_few(const SparseArgs& a, int64_t units, cudaStream_t stream) {
   const int chunks = a.top_k * (a.block / 16);
   int X = 1;
   while (X < 8 && X * kFewWarps < chunks && units * X < int64_t(sm_count()) * 2) X *= 2;
-  return launch_cluster(sparse_few_kernel<D>, a, units, X, kFewWarps * 32, smem, stream);
+  return launch_units(sparse_few_kernel<D>, a, units, X, true, kFewWarps * 32, smem, stream);
 }
 
 template <int D>
@@ -1317,16 +1326,17 @@ extern "C" int pkv_block_means(const uint16_t* k, int64_t kv_rows, int head_dim,
   if ((head_dim != 64 && head_dim != 128) || kv_rows >= (int64_t(1) << 31) ||
       reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(means) % 16)
     return PKV_EUNSUPPORTED;
-  int64_t grid = (means_rows + 7) / 8;
+  // four warps a row while one would not fill the GPU: 246 blocks of 128 keys
+  // of 64 take 5 us instead of 8
+  const bool few = means_rows <= int64_t(sm_count()) * 8;
+  int64_t grid = few ? (means_rows + 1) / 2 : (means_rows + 7) / 8;
   const int64_t cap = int64_t(sm_count()) * 8;
   if (grid > cap) grid = cap;
   auto s = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    block_means_kernel<128><<<int(grid), 256, 0, s>>>(k, kv_rows, cu_seqlens_k, segments, block,
-                                                      means, means_rows, zero_rest);
-  else
-    block_means_kernel<64><<<int(grid), 256, 0, s>>>(k, kv_rows, cu_seqlens_k, segments, block,
-                                                     means, means_rows, zero_rest);
+  auto kernel = head_dim == 128 ? (few ? block_means_kernel<128, 4> : block_means_kernel<128, 1>)
+                                : (few ? block_means_kernel<64, 4> : block_means_kernel<64, 1>);
+  kernel<<<int(grid), 256, 0, s>>>(k, kv_rows, cu_seqlens_k, segments, block, means, means_rows,
+                                   zero_rest);
   return launch_status();
 }
 

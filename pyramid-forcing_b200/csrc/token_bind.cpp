@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <optional>
 #include <tuple>
 
@@ -385,6 +386,58 @@ SparseCall sparse_call(const char* op, const Tensor& q, const Tensor* k, const T
   return c;
 }
 
+// The three steps over one checked call.
+Tensor run_means(const char* op, const Tensor& k, int64_t D, const Tensor& cu, int64_t segs,
+                 int64_t block, bool zero_rest) {
+  const int64_t rows = pkv_block_rows(k.size(0), int(segs), int(block));
+  const Tensor means = at::empty({rows, D}, k.options().dtype(at::kFloat));
+  check_rc(pkv_block_means(u16(k), k.size(0), int(D), cu.data_ptr<int32_t>(), int(segs),
+                           int(block), static_cast<float*>(mut(means)), rows, zero_rest,
+                           stream_of(k)),
+           op);
+  return means;
+}
+
+Tensor run_select(const char* op, const SparseCall& c, const Tensor& means, int64_t kv_rows,
+                  int64_t query_block, int64_t block, int64_t top_k) {
+  TORCH_CHECK(means.device() == c.q.device() && means.scalar_type() == at::kFloat &&
+                  means.dim() == 2 && means.size(1) == c.D && kv_rows >= 0 &&
+                  means.size(0) >= pkv_block_rows(kv_rows, int(c.C * c.H), int(block)),
+              op, ": means must be the fp32 table pkv_block_means gives for these keys");
+  Tensor mm = means.contiguous();
+  if (reinterpret_cast<uintptr_t>(mm.data_ptr()) % 16) mm = mm.clone();
+  const Tensor blocks = at::empty({c.C * c.H, c.groups, top_k}, c.cu.options());
+  check_rc(pkv_select_blocks(u16(c.q), c.q.stride(0), c.q.stride(1),
+                             static_cast<const float*>(ptr(mm)), mm.size(0),
+                             c.cu.data_ptr<int32_t>(), kv_rows, int(c.C), int(c.H), int(c.R),
+                             int(c.D), int(query_block), int(block), int(top_k),
+                             static_cast<int32_t*>(mut(blocks)), stream_of(c.q)),
+           op);
+  return blocks;
+}
+
+Tensor run_attention(const char* op, const SparseCall& c, const Tensor& blocks,
+                     int64_t query_block, int64_t block, double scale,
+                     const std::optional<Tensor>& status) {
+  TORCH_CHECK(scale > 0.0, op, ": softmax_scale must be positive");
+  int32_t* st = nullptr;
+  if (status.has_value() && status->defined()) {
+    TORCH_CHECK(status->device() == c.q.device() && status->scalar_type() == at::kInt &&
+                    status->numel() >= 1,
+                op, ": status must be int32 on q's device");
+    st = status->data_ptr<int32_t>();
+  }
+  const Tensor out = at::empty({c.C * c.R, c.H, c.D}, c.q.options());
+  check_rc(pkv_block_attention(u16(c.q), c.q.stride(0), c.q.stride(1), u16(c.k), u16(c.v),
+                               c.k.size(0), c.cu.data_ptr<int32_t>(), int(c.C), int(c.H),
+                               int(c.R), int(c.D), float(scale),
+                               static_cast<const int32_t*>(ptr(blocks)), int(query_block),
+                               int(block), int(blocks.size(2)), static_cast<uint16_t*>(mut(out)),
+                               out.stride(0), out.stride(1), st, stream_of(c.q)),
+           op);
+  return out;
+}
+
 Tensor op_block_means(Tensor k, Tensor cu, int64_t block, bool zero_rest) {
   const char* op = "pkv_block_means";
   TORCH_CHECK(k.is_cuda() && k.dim() >= 2 && k.scalar_type() == at::kBFloat16, op,
@@ -399,13 +452,7 @@ Tensor op_block_means(Tensor k, Tensor cu, int64_t block, bool zero_rest) {
   Tensor kk = k.reshape({k.numel() / D, D}).contiguous();
   if (reinterpret_cast<uintptr_t>(kk.data_ptr()) % 16) kk = kk.clone();
   const Tensor cc = cu.contiguous();
-  const int segs = int(cc.numel() - 1);
-  const int64_t rows = pkv_block_rows(kk.size(0), segs, int(block));
-  const Tensor means = at::empty({rows, D}, k.options().dtype(at::kFloat));
-  check_rc(pkv_block_means(u16(kk), kk.size(0), int(D), cc.data_ptr<int32_t>(), segs, int(block),
-                           static_cast<float*>(mut(means)), rows, zero_rest, stream_of(k)),
-           op);
-  return means;
+  return run_means(op, kk, D, cc, cc.numel() - 1, block, zero_rest);
 }
 
 Tensor op_select_blocks(Tensor q, Tensor means, Tensor cu, int64_t kv_rows, int64_t num_chunks,
@@ -415,20 +462,7 @@ Tensor op_select_blocks(Tensor q, Tensor means, Tensor cu, int64_t kv_rows, int6
                                                    : std::nullopt);
   const SparseCall c =
       sparse_call(op, q, nullptr, nullptr, cu, num_chunks, rows, query_block, block, top_k);
-  TORCH_CHECK(means.device() == q.device() && means.scalar_type() == at::kFloat &&
-                  means.dim() == 2 && means.size(1) == c.D && kv_rows >= 0 &&
-                  means.size(0) >= pkv_block_rows(kv_rows, int(c.C * c.H), int(block)),
-              op, ": means must be the fp32 table pkv_block_means gives for these keys");
-  Tensor mm = means.contiguous();
-  if (reinterpret_cast<uintptr_t>(mm.data_ptr()) % 16) mm = mm.clone();
-  const Tensor blocks = at::empty({c.C * c.H, c.groups, top_k}, c.cu.options());
-  check_rc(pkv_select_blocks(u16(c.q), c.q.stride(0), c.q.stride(1),
-                             static_cast<const float*>(ptr(mm)), mm.size(0),
-                             c.cu.data_ptr<int32_t>(), kv_rows, int(c.C), int(c.H), int(c.R),
-                             int(c.D), int(query_block), int(block), int(top_k),
-                             static_cast<int32_t*>(mut(blocks)), stream_of(q)),
-           op);
-  return blocks;
+  return run_select(op, c, means, kv_rows, query_block, block, top_k);
 }
 
 Tensor op_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu, int64_t num_chunks,
@@ -443,24 +477,26 @@ Tensor op_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu, int64_t num_c
   TORCH_CHECK(blocks.device() == q.device() && blocks.scalar_type() == at::kInt &&
                   blocks.size(0) == c.C * c.H && blocks.size(1) == c.groups,
               op, ": blocks must be int32 [", c.C * c.H, ", ", c.groups, ", top_k] on q's device");
-  TORCH_CHECK(scale > 0.0, op, ": softmax_scale must be positive");
-  const Tensor bb = blocks.contiguous();
-  int32_t* st = nullptr;
-  if (status.has_value() && status->defined()) {
-    TORCH_CHECK(status->device() == q.device() && status->scalar_type() == at::kInt &&
-                    status->numel() >= 1,
-                op, ": status must be int32 on q's device");
-    st = status->data_ptr<int32_t>();
-  }
-  const Tensor out = at::empty(q.sizes(), q.options());
-  check_rc(pkv_block_attention(u16(c.q), c.q.stride(0), c.q.stride(1), u16(c.k), u16(c.v),
-                               c.k.size(0), c.cu.data_ptr<int32_t>(), int(c.C), int(c.H),
-                               int(c.R), int(c.D), float(scale),
-                               static_cast<const int32_t*>(ptr(bb)), int(query_block), int(block),
-                               int(blocks.size(2)), static_cast<uint16_t*>(mut(out)),
-                               out.stride(0), out.stride(1), st, stream_of(q)),
-           op);
-  return out;
+  return run_attention(op, c, blocks.contiguous(), query_block, block, scale, status);
+}
+
+std::tuple<Tensor, Tensor> op_sparse_attention(Tensor q, Tensor k, Tensor v, Tensor cu,
+                                               int64_t num_chunks, int64_t rows, int64_t top_k,
+                                               int64_t query_block, int64_t block,
+                                               std::optional<double> scale,
+                                               std::optional<Tensor> means,
+                                               std::optional<Tensor> status) {
+  const char* op = "pkv_sparse_attention";
+  const c10::cuda::OptionalCUDAGuard g(q.is_cuda() ? std::optional<c10::Device>(q.device())
+                                                   : std::nullopt);
+  const SparseCall c =
+      sparse_call(op, q, &k, &v, cu, num_chunks, rows, query_block, block, top_k);
+  const Tensor table = means.has_value() && means->defined()
+                           ? *means
+                           : run_means(op, c.k, c.D, c.cu, c.C * c.H, block, false);
+  const Tensor blocks = run_select(op, c, table, c.k.size(0), query_block, block, top_k);
+  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt(double(c.D));
+  return {run_attention(op, c, blocks, query_block, block, sc, status), blocks};
 }
 
 }  // namespace
@@ -485,6 +521,9 @@ TORCH_LIBRARY_FRAGMENT(adahead, m) {
   m.def("pkv_block_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_k, int num_chunks, "
         "int rows_per_chunk, Tensor blocks, int query_block, int block, float softmax_scale, "
         "Tensor(a!)? status) -> Tensor");
+  m.def("pkv_sparse_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_k, int num_chunks, "
+        "int rows_per_chunk, int top_k, int query_block, int block, float? softmax_scale, "
+        "Tensor? means, Tensor(a!)? status) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
@@ -494,6 +533,7 @@ TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
   m.impl("pkv_block_means", op_block_means);
   m.impl("pkv_select_blocks", op_select_blocks);
   m.impl("pkv_block_attention", op_block_attention);
+  m.impl("pkv_sparse_attention", op_sparse_attention);
   m.impl("pkv_norm", op_norm);
   m.impl("pkv_rotary_apply", op_rotary_apply);
 }

@@ -21,6 +21,12 @@ import torch
 from . import _ops
 
 
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("block-sparse attention has no gradient: call it under "
+                           "torch.no_grad()")
+
+
 def block_means(k: torch.Tensor, cu_seqlens_k: torch.Tensor, block: int = 64) -> torch.Tensor:
     """Mean key of every block, fp32 [rows // block + segments, D].
 
@@ -52,8 +58,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     rows_per_chunk, H, D], k / v bf16 [rows, D].  Entries of ``blocks`` outside
     a segment are skipped, a block listed twice counts twice, a row with no
     keys gives zeros."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise RuntimeError("pkv_block_attention has no gradient: call it under torch.no_grad()")
+    _no_grad(q, k, v)
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
     return _ops.overload("pkv_block_attention")(q, k, v, cu_seqlens_k, int(num_chunks),
                                           int(rows_per_chunk), blocks, int(query_block),
@@ -66,13 +71,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      softmax_scale: float | None = None, means: torch.Tensor | None = None,
                      status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(output, blocks): select_blocks and block_attention, and block_means
-    where the caller does not keep the table."""
-    if means is None:
-        means = _ops.overload("pkv_block_means")(k, cu_seqlens_k[:num_chunks * q.shape[1] + 1],
-                                           int(block), False)
-    blocks = select_blocks(q, means, cu_seqlens_k, k.numel() // q.shape[-1], num_chunks,
-                           rows_per_chunk, top_k, query_block=query_block, block=block)
-    out = block_attention(q, k, v, cu_seqlens_k, num_chunks, rows_per_chunk, blocks,
-                          query_block=query_block, block=block, softmax_scale=softmax_scale,
-                          status=status)
-    return out, blocks
+    where the caller does not keep the table, in one call."""
+    _no_grad(q, k, v)
+    return _ops.overload("pkv_sparse_attention")(q, k, v, cu_seqlens_k, num_chunks,
+                                                 rows_per_chunk, top_k, query_block, block,
+                                                 softmax_scale, means, status)

@@ -261,6 +261,27 @@ def test_layer_norm_side_stream_and_graph(cuda):
         assert all(torch.equal(p, q) for p, q in zip(res, ref))
 
 
+def test_layer_norm_captured_backward(cuda):
+    """A training step captured through autograd (no eager graph of the same
+    leaves alive) and replayed with another gradient: the eager bits."""
+    from pyramidkv.norm import layer_norm
+    x, w, b, dy = _data(cuda, 640, 256, 2, BF, FP, seed=3)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    static = dy.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer_norm(x, w, b, one_plus=True)
+        grads = torch.autograd.grad(y, leaves, static)
+    other = dy.flip(0).contiguous()
+    static.copy_(other)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in grads]
+    del y
+    want = torch.autograd.grad(layer_norm(x, w, b, one_plus=True), leaves, other)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_layer_norm_refusals(cuda):
     from pyramidkv.norm import layer_norm
     x = torch.randn(6, 8, device=cuda)
@@ -274,6 +295,9 @@ def test_layer_norm_refusals(cuda):
             layer_norm(x, **bad)
     with pytest.raises(RuntimeError, match="bf16, fp16 or fp32"):
         layer_norm(x.double())
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(layer_norm(leaf).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="no channels"):
         layer_norm(x[:, :0])
     with pytest.raises(ValueError, match="one type"):
