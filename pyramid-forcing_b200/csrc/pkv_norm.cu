@@ -128,7 +128,7 @@ __device__ __forceinline__ float fold(f2 a) {
 template <typename TX, typename TW, int V, int NV>
 __device__ __forceinline__ void norm_store(const NormArgs& a, int64_t row, int tid, int tpr,
                                            int nvec, const float (&f)[NV][V], float rstd) {
-  const int64_t g = row / a.rows_per_group;
+  const int64_t g = uint32_t(row) / uint32_t(a.rows_per_group);  // (rows < 2^31)
   const TW* w = a.w ? static_cast<const TW*>(a.w) + g * a.C : nullptr;
   const TW* b = a.b ? static_cast<const TW*>(a.b) + g * a.C : nullptr;
   TX* y = static_cast<TX*>(a.y) + row * a.y_rs;
@@ -197,79 +197,81 @@ __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
   norm_store<TX, TW, V, NV>(a, row, tid, tpr, nvec, f, rstd);
 }
 
-// A warp a row, many rows a warp: the next kStages - 1 rows are on their way
-// into shared memory while one is in registers, so HBM stays busy through the
-// reductions.  Each lane copies exactly what it will read: no barriers.
-constexpr int kFwdStages = 4;
+// Short rows: L lanes a row, 32 / L rows a warp, one vector a lane; the next
+// seven rounds' rows are on their way into shared memory while one is in
+// registers, so HBM stays busy through the reductions.  Each lane copies exactly
+// what it will read: no barriers.
+constexpr int kShortStages = 8;
 
-template <typename TX, typename TW, int V, int NV>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_stream_kernel(NormArgs a) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Vec<TX, V>* ring = reinterpret_cast<Vec<TX, V>*>(raw) + warp * (kFwdStages * NV * 32) + lane;
-  const int64_t step = int64_t(gridDim.x) * (kNormThreads / 32);
-  const int64_t first = blockIdx.x * int64_t(kNormThreads / 32) + warp;
+template <typename TX, typename TW, int V, int L>
+__global__ void __launch_bounds__(kNormThreads) norm_short_kernel(NormArgs a) {
+  __shared__ Vec<TX, V> ring[kShortStages][kNormThreads];
+  constexpr int kPer = kNormThreads / L;  // rows of a block's round
+  const int tid = threadIdx.x, lane = tid % L;
+  const int64_t step = int64_t(gridDim.x) * kPer;
+  const int64_t first = blockIdx.x * int64_t(kPer) + tid / L;
   const int nvec = a.C / V;
   const float inv_c = 1.0f / float(a.C);
   auto fetch = [&](int64_t row, int st) {
-    if (row < a.rows) {
-      const TX* x = static_cast<const TX*>(a.x) + row * a.x_rs;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = lane + i * 32;
-        if (j < nvec) cp_async<TX, V>(ring + (st * NV + i) * 32, x + j * V);
-      }
-    }
+    if (row < a.rows && lane < nvec)
+      cp_async<TX, V>(&ring[st][tid], static_cast<const TX*>(a.x) + row * a.x_rs + lane * V);
     cp_commit();  // an empty group counts too
   };
-  for (int i = 0; i < kFwdStages - 1; ++i) fetch(first + i * step, i);
+  for (int i = 0; i < kShortStages - 1; ++i) fetch(first + i * step, i);
   int st = 0;
-  for (int64_t row = first; row < a.rows; row += step) {
-    cp_wait<kFwdStages - 2>();
-    float f[NV][V];
+  // (the whole warp goes on while one of its rows is there: shuffles)
+  for (int64_t row = first; row - tid / L < a.rows; row += step) {
+    cp_wait<kShortStages - 2>();
+    const bool live = row < a.rows && lane < nvec;
+    float f[1][V];
+    if (live)
+      widen<TX, V>(ring[st][tid], f[0]);
+    else
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[0][e] = 0.0f;
+    // the slot read one round ago is free: its values are in registers
+    fetch(row + (kShortStages - 1) * step, st == 0 ? kShortStages - 1 : st - 1);
+    st = st + 1 == kShortStages ? 0 : st + 1;
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (lane + i * 32 < nvec) {
-        widen<TX, V>(ring[(st * NV + i) * 32], f[i]);
+    for (int e = 0; e < V; ++e) s += f[0][e];
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += f[i][e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[i][e] = 0.0f;
-      }
-    }
-    // the slot read one row ago is free: its values are in registers
-    fetch(row + (kFwdStages - 1) * step, st == 0 ? kFwdStages - 1 : st - 1);
-    st = st + 1 == kFwdStages ? 0 : st + 1;
-    const float mu = warp_sum(s) * inv_c;
+    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float mu = s * inv_c;
     float q = 0.0f;
+    if (lane < nvec)
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (lane + i * 32 < nvec)
+      for (int e = 0; e < V; ++e) {
+        f[0][e] -= mu;
+        q = fmaf(f[0][e], f[0][e], q);
+      }
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          f[i][e] -= mu;
-          q = fmaf(f[i][e], f[i][e], q);
-        }
-    const float rstd = rsqrtf(warp_sum(q) * inv_c + a.eps);
-    if (lane == 0) {
-      if (a.mean) a.mean[row] = mu;
-      if (a.rstd) a.rstd[row] = rstd;
+    for (int o = L / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    const float rstd = rsqrtf(q * inv_c + a.eps);
+    if (row < a.rows) {
+      if (lane == 0) {
+        if (a.mean) a.mean[row] = mu;
+        if (a.rstd) a.rstd[row] = rstd;
+      }
+      norm_store<TX, TW, V, 1>(a, row, lane, L, nvec, f, rstd);
     }
-    norm_store<TX, TW, V, NV>(a, row, lane, 32, nvec, f, rstd);
   }
 }
 
 // A block a range of a group's rows, every column (thread = fixed columns, as
 // the backward pass): weight and bias are read once and stay in registers,
-// kFwdRows rows share the two barriers of their statistics, and the next
+// R rows share the two barriers of their statistics, and the next
 // rounds' rows are on their way into shared memory meanwhile.
-constexpr int kFwdRows = 4, kColStages = 3;
+// (16-bit single elements are too small for asynchronous copies: loaded
+// directly.)
+constexpr int kColStages = 3;
+__host__ __device__ constexpr int fwd_rows(int elems) { return elems <= 8 ? 4 : 2; }
 
 template <typename TX, typename TW, int V, int NV, int kThreads>
-__global__ void __launch_bounds__(kThreads, 768 / kThreads) norm_cols_fwd_kernel(NormArgs a) {
-  constexpr int R = kFwdRows, E = V * NV;
+__global__ void __launch_bounds__(kThreads, V * NV <= 8 ? 768 / kThreads : 1)
+    norm_cols_fwd_kernel(NormArgs a) {
+  constexpr int E = V * NV, R = fwd_rows(E);
+  constexpr bool kRing = V * sizeof(TX) >= 4;
   __shared__ __align__(16) float red[2][kThreads / 32][4];
   extern __shared__ __align__(16) uint8_t raw[];
   const int tid = threadIdx.x, nthr = blockDim.x;
@@ -285,17 +287,19 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) norm_cols_fwd_kernel
   TX* yp = static_cast<TX*>(a.y) + r0 * a.y_rs + tid * V;
   int ahead = 0;  // rows asked for
   auto fetch = [&](int st) {
+    if constexpr (kRing) {
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      if (ahead + k < n)
+      for (int k = 0; k < R; ++k) {
+        if (ahead + k < n)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (tid + i * nthr < nvec)
-            cp_async<TX, V>(ring + ((st * R + k) * NV + i) * nthr, xp + i * nthr * V);
-      xp += a.x_rs;
+          for (int i = 0; i < NV; ++i)
+            if (tid + i * nthr < nvec)
+              cp_async<TX, V>(ring + ((st * R + k) * NV + i) * nthr, xp + i * nthr * V);
+        xp += a.x_rs;
+      }
+      ahead += R;
+      cp_commit();
     }
-    ahead += R;
-    cp_commit();
   };
   for (int i = 0; i < kColStages - 1; ++i) fetch(i);
   Pairs<E> w, b;
@@ -323,19 +327,34 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) norm_cols_fwd_kernel
   }
   int st = 0;
   for (int r = 0; r < n; r += R) {
-    cp_wait<kColStages - 2>();
+    if constexpr (kRing) cp_wait<kColStages - 2>();
     Pairs<E> f[R];
     float s[R];
+    Vec<TX, V> direct[kRing ? 1 : R][NV];
+    if constexpr (!kRing) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (r + k < n && tid + i * nthr < nvec)
+            direct[k][i] = ld_vec<TX, V>(xp + i * nthr * V);
+        xp += a.x_rs;
+      }
+    }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       Vec<TX, V> v[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (r + k < n && tid + i * nthr < nvec)
-          v[i] = ring[((st * R + k) * NV + i) * nthr];
-        else
+        if (r + k < n && tid + i * nthr < nvec) {
+          if constexpr (kRing)
+            v[i] = ring[((st * R + k) * NV + i) * nthr];
+          else
+            v[i] = direct[k][i];
+        } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) v[i].v[e] = from_f32<TX>(0.0f);
+        }
       }
       f[k] = to_pairs<TX, V, NV>(v);
       f2 t = f[k].p[0];
@@ -431,6 +450,8 @@ struct NormBwdArgs {
   const float* rstd;
   void* dx;
   float* part;  // [groups * parts][2][C] column sums, or nullptr
+  void* dw;     // the sums themselves where a group is one part, or nullptr
+  void* db;
   int64_t dy_rs, x_rs, dx_rs, rows_per_group;
   int C, parts;
   float plus;
@@ -576,8 +597,10 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 192 ? 3 : kThreads <= 25
       }
     }
   }
-  if (a.part != nullptr) {
+  if (a.part != nullptr || a.dw != nullptr || a.db != nullptr) {
     float* pw = a.part + int64_t(blockIdx.x) * 2 * a.C;
+    TW* dw = static_cast<TW*>(a.dw) + grp * a.C;
+    TW* db = static_cast<TW*>(a.db) + grp * a.C;
     float sw[2 * w.kN], sb[2 * w.kN];
 #pragma unroll
     for (int i = 0; i < w.kN; ++i) {
@@ -590,8 +613,13 @@ __global__ void __launch_bounds__(kThreads, kThreads <= 192 ? 3 : kThreads <= 25
       if (j < nvec)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          pw[j * V + e] = sw[i * V + e];
-          pw[a.C + j * V + e] = sb[i * V + e];
+          if (a.part != nullptr) {
+            pw[j * V + e] = sw[i * V + e];
+            pw[a.C + j * V + e] = sb[i * V + e];
+          } else {
+            if (a.dw != nullptr) dw[j * V + e] = from_f32<TW>(sw[i * V + e]);
+            if (a.db != nullptr) db[j * V + e] = from_f32<TW>(sb[i * V + e]);
+          }
         }
     }
   }
@@ -695,32 +723,29 @@ int64_t row_parts(int64_t rows_per_group, int64_t groups, int per_sm, int least)
   const int64_t p = want < most ? want : most;
   return p < 1 ? 1 : p;
 }
-int64_t bwd_parts(int64_t rows_per_group, int64_t groups) {
-  return row_parts(rows_per_group, groups, 3, 8);
+// Backward: three blocks of 192 threads an SM, more of the smaller ones that
+// short rows (16-byte vectors) leave.
+int64_t bwd_parts(int64_t rows_per_group, int64_t groups, int64_t cols) {
+  const int64_t thr = (cols / 8 + 31) / 32 * 32;
+  const int per_sm = thr >= 192 ? 3 : thr <= 32 ? 18 : int(576 / thr);
+  return row_parts(rows_per_group, groups, per_sm, 4);
 }
 
 constexpr int round_warp(int n) { return (n + 31) / 32 * 32; }
 
-template <typename TX, typename TW, int V, int NV>
-int stream_fwd(const NormArgs& a, cudaStream_t s) {
-  constexpr size_t smem = size_t(kNormThreads) * kFwdStages * NV * V * sizeof(TX);
-  static std::mutex mu;
-  static int done[kMaxDevices] = {};
-  if (smem_opt_in(done, mu, norm_stream_kernel<TX, TW, V, NV>, smem) <= 0) {
-    cudaGetLastError();
-    return PKV_ELAUNCH;
-  }
-  const int64_t need = (a.rows + kNormThreads / 32 - 1) / (kNormThreads / 32);
-  const int64_t most = int64_t(sm_count()) * 2;
-  norm_stream_kernel<TX, TW, V, NV>
-      <<<int(need < most ? need : most), kNormThreads, smem, s>>>(a);
+template <typename TX, typename TW, int V, int L>
+int short_fwd(const NormArgs& a, cudaStream_t s) {
+  const int64_t need = (a.rows + kNormThreads / L - 1) / (kNormThreads / L);
+  const int64_t most = int64_t(sm_count()) * 5;
+  norm_short_kernel<TX, TW, V, L><<<int(need < most ? need : most), kNormThreads, 0, s>>>(a);
   return launch_status();
 }
 
 template <typename TX, typename TW, int V, int NV, int kThreads>
 int cols_fwd(NormArgs a, cudaStream_t s) {
   const int thr = round_warp((a.C / V + NV - 1) / NV);
-  constexpr size_t per = size_t(kColStages) * kFwdRows * NV * V * sizeof(TX);
+  constexpr int R = fwd_rows(V * NV);
+  constexpr size_t per = V * sizeof(TX) >= 4 ? size_t(kColStages) * R * NV * V * sizeof(TX) : 0;
   static_assert(per * kThreads <= 200 * 1024, "the rounds of a block fit its shared memory");
   static std::mutex mu;
   static int done[kMaxDevices] = {};
@@ -729,7 +754,8 @@ int cols_fwd(NormArgs a, cudaStream_t s) {
     return PKV_ELAUNCH;
   }
   const int64_t groups = a.rows / a.rows_per_group;
-  a.parts = int(row_parts(a.rows_per_group, groups, 1024 / kThreads, 2 * kFwdRows));
+  const int per_sm = V * NV <= 8 ? 768 / thr : 1;  // (what the registers allow)
+  a.parts = int(row_parts(a.rows_per_group, groups, per_sm > 0 ? per_sm : 1, 2 * R));
   const int64_t grid = groups * a.parts;
   if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   norm_cols_fwd_kernel<TX, TW, V, NV, kThreads><<<int(grid), thr, per * thr, s>>>(a);
@@ -739,22 +765,38 @@ int cols_fwd(NormArgs a, cudaStream_t s) {
 template <typename TX, typename TW, int V>
 int launch_fwd(const NormArgs& a, cudaStream_t s) {
   const int nvec = a.C / V;
-  if constexpr (V * sizeof(TX) >= 4) {
-    if (a.rows >= int64_t(sm_count()) * 16) {
-      // short rows: a warp a row; longer ones, in groups that give a block
-      // rows to share its weights over: fixed columns
-      if (nvec <= 32) return stream_fwd<TX, TW, V, 1>(a, s);
-      if (nvec <= 64) return stream_fwd<TX, TW, V, 2>(a, s);
-      if (a.rows_per_group >= 2 * kFwdRows) {
-        if (nvec <= 256) return cols_fwd<TX, TW, V, 1, 256>(a, s);
-        if (nvec <= 512) return cols_fwd<TX, TW, V, 2, 256>(a, s);
+  if (a.rows >= int64_t(sm_count()) * 16) {
+    // rows enough to fill the GPU.  Short ones: a few lanes a row; longer
+    // ones, in groups that give a block rows to share its weights over: fixed
+    // columns
+    if constexpr (V * sizeof(TX) >= 4) {
+      if (nvec <= 4) return short_fwd<TX, TW, V, 4>(a, s);
+      if (nvec <= 8) return short_fwd<TX, TW, V, 8>(a, s);
+      if (nvec <= 16) return short_fwd<TX, TW, V, 16>(a, s);
+      if (nvec <= 32) return short_fwd<TX, TW, V, 32>(a, s);
+    }
+    if (a.rows_per_group >= 8) {
+      if (nvec <= 256) return cols_fwd<TX, TW, V, 1, 256>(a, s);
+      if (nvec <= 512) return cols_fwd<TX, TW, V, 2, 256>(a, s);
+      if constexpr (V >= 8) {
+        if (nvec <= 1024) return cols_fwd<TX, TW, V, 2, 512>(a, s);
+      } else {
+        if (nvec <= 1024) return cols_fwd<TX, TW, V, 4, 256>(a, s);
+        if constexpr (V >= 4) {
+          if (nvec <= 2048) return cols_fwd<TX, TW, V, 4, 512>(a, s);
+        } else {
+          if (nvec <= 2048) return cols_fwd<TX, TW, V, 8, 256>(a, s);
+          if (nvec <= 4096) return cols_fwd<TX, TW, V, 8, 512>(a, s);
+          if constexpr (V == 1)
+            if (nvec <= 8192) return cols_fwd<TX, TW, V, 16, 512>(a, s);
+        }
       }
     }
   }
   const int grid = int(a.rows);
   auto threads = [nvec](int nv) { return round_warp((nvec + nv - 1) / nv); };
-  // about 256 threads a row; up to 1024 where the row is longer than NV = 8
-  // vectors (or 16 elements) a thread
+  // few rows, or a group a row: about 256 threads a row, up to 1024 where the
+  // row is longer than 8 vectors (or 16 elements) a thread
   constexpr int kMost = V >= 8 ? 2 : V >= 4 ? 4 : 8;
   if (nvec <= 256)
     norm_fwd_kernel<TX, TW, V, 1><<<grid, threads(1), 0, s>>>(a);
@@ -835,14 +877,22 @@ int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream
     return a.C % v == 0 && vec_ok(a.x, a.x_rs, v, sx) && vec_ok(a.dy, a.dy_rs, v, sx) &&
            vec_ok(a.dx, a.dx_rs, v, sx) && vec_ok(a.w, 0, sw, 1);
   };
+  // (a group of one part needs no second pass: rows in registers only)
+  const bool whole = a.parts == 1 && a.C <= 8192;
+  NormBwdArgs b = a;
+  if (whole) {
+    b.part = nullptr;
+    b.dw = dw;
+    b.db = db;
+  }
   int rc = PKV_OK;
-  if (fits(V))
-    rc = launch_bwd<TX, TW, V>(a, groups, s);
+  if (fits(V) && (sizeof(TX) == 4 || a.C >= 128))
+    rc = launch_bwd<TX, TW, V>(b, groups, s);
   else if (sizeof(TX) == 2 && fits(2))
-    rc = launch_bwd<TX, TW, sizeof(TX) == 2 ? 2 : 1>(a, groups, s);
+    rc = launch_bwd<TX, TW, sizeof(TX) == 2 ? 2 : 1>(b, groups, s);
   else
-    rc = launch_bwd<TX, TW, 1>(a, groups, s);
-  if (rc != PKV_OK || a.part == nullptr) return rc;
+    rc = launch_bwd<TX, TW, 1>(b, groups, s);
+  if (rc != PKV_OK || b.part == nullptr) return rc;
   if (a.C % 4 == 0 && vec_ok(a.part, 0, 16, 1)) {
     const dim3 grid(unsigned(groups), unsigned((a.C + 127) / 128));
     norm_parts_kernel<TW, 4><<<grid, 256, 0, s>>>(a.part, a.parts, a.C, static_cast<TW*>(dw),
@@ -866,7 +916,7 @@ using namespace pkv;
 
 extern "C" int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups) {
   if (rows <= 0 || cols <= 0 || groups <= 0 || rows % groups != 0) return 0;
-  return groups * bwd_parts(rows / groups, groups) * 2 * cols * 4;
+  return groups * bwd_parts(rows / groups, groups, cols) * 2 * cols * 4;
 }
 
 extern "C" int pkv_layer_norm(const void* x, int64_t x_row_stride, const void* weight,
@@ -929,7 +979,7 @@ extern "C" int pkv_layer_norm_backward(const void* dy, int64_t dy_row_stride, co
   a.dx_rs = dx_row_stride;
   a.rows_per_group = rows / groups;
   a.C = int(cols);
-  a.parts = int(bwd_parts(rows / groups, groups));
+  a.parts = int(bwd_parts(rows / groups, groups, cols));
   a.plus = one_plus ? 1.0f : 0.0f;
   auto s = static_cast<cudaStream_t>(stream);
   if (dtype == PKV_BF16)

@@ -65,7 +65,7 @@ struct RotArgs {
 // kPair: a unit is V pairs out of two vectors (half layout, and interleaved
 // single elements); else it is one vector of V / 2 interleaved pairs.
 template <typename T, int V, bool kHalf>
-__global__ void __launch_bounds__(kRotThreads, 8) rotary_kernel(RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, V >= 4 ? 8 : 6) rotary_kernel(RotArgs a) {
   constexpr bool kPair = kHalf || V == 1;
   __shared__ float2 tab[kRotTable];
   const int64_t t0 = blockIdx.x * int64_t(a.tile);
@@ -98,14 +98,14 @@ __global__ void __launch_bounds__(kRotThreads, 8) rotary_kernel(RotArgs a) {
   for (int i = threadIdx.x; i < n; i += kRotThreads) {
     const uint32_t th = a.by_turn.div(i);
     const int u = i - int(th) * turn;
+    const int e = kHalf ? u * V : V == 1 ? 2 * u : u * V;
     const T* x;
     T* o;
     int t;
     rows(th, x, o, t);
-    const float2* cs = tab + t * a.P + (kPair ? u * V : u * V / 2);
-    const int e = kHalf ? u * V : V == 1 ? 2 * u : u * V;
     x += e;
     o += e;
+    const float2* cs = tab + t * a.P + (kPair ? u * V : u * V / 2);
     if constexpr (kPair) {
       const int gap = kHalf ? a.P : 1;
       float p[V], q[V];
@@ -139,12 +139,12 @@ __global__ void __launch_bounds__(kRotThreads, 8) rotary_kernel(RotArgs a) {
   const int m = nt * heads * rest;
   for (int i = threadIdx.x; i < m; i += kRotThreads) {
     const uint32_t th = a.by_rest.div(i);
-    const T* x;
-    T* y;
-    int t;
-    rows(th, x, y, t);
     const int e = 2 * a.P + (i - int(th) * rest) * V;
-    st_vec<T, V>(y + e, ld_vec<T, V>(x + e));
+    const T* x;
+    T* o;
+    int t;
+    rows(th, x, o, t);
+    st_vec<T, V>(o + e, ld_vec<T, V>(x + e));
   }
 }
 
@@ -164,8 +164,9 @@ template <typename T, int V>
 void launch_rotary(RotArgs a, int64_t grid, cudaStream_t s) {
   a.by_heads = Div(uint32_t(a.s[0].heads + a.s[1].heads));
   const int turn = (a.half || V == 1 ? a.P : 2 * a.P) / V;
+  const int rest = (a.D - 2 * a.P) / V;
   if (turn > 0) a.by_turn = Div(uint32_t(turn));
-  if (a.D - 2 * a.P >= V) a.by_rest = Div(uint32_t((a.D - 2 * a.P) / V));
+  if (rest > 0) a.by_rest = Div(uint32_t(rest));
   if (a.half)
     rotary_kernel<T, V, true><<<int(grid), kRotThreads, 0, s>>>(a);
   else

@@ -104,6 +104,22 @@ CASES = [
     (33, 16392, 3, HF, FP, True),
     (2, 40000, 2, FP, FP, False),
     (1, 1, 1, BF, BF, True),
+    # rows enough to fill the GPU: a few lanes a row, ...
+    (3000, 24, 1, BF, FP, True),
+    (2999, 64, 1, FP, FP, False),
+    (2600, 100, 2, HF, HF, True),
+    (2400, 250, 3, BF, BF, False),
+    (4000, 30, 4000, BF, FP, True),     # ... a group a row
+    # ... and fixed columns a thread, of 16, 4 and 2 bytes
+    (2400, 777, 8, BF, FP, True),
+    (2402, 1534, 2, HF, FP, False),
+    (2400, 2050, 1, BF, BF, True),
+    (2400, 4100, 3, FP, FP, True),
+    (2400, 5001, 2, BF, BF, False),
+    (2400, 8192, 1, HF, HF, True),
+    (2400, 6000, 240, FP, FP, False),
+    (2500, 1536, 2500, BF, FP, True),   # modulation of each row
+    (2400, 700, 1200, FP, FP, True),
 ]
 
 

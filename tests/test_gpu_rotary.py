@@ -73,6 +73,9 @@ CASES = [
     (2, 1, 1, 4096, 2048, 1, "half", FP, 4096),      # a table for one token
     (5, 2, 2, 7, 3, 1, "interleaved", FP, 50),       # an odd head
     (5, 2, 2, 8, 0, 1, "half", BF, 50),              # nothing turns
+    (700, 7, 5, 90, 31, 1, "half", BF, 1000),
+    (700, 7, 5, 90, 45, 2, "interleaved", BF, 1000),
+    (40, 3, 2, 74, 34, 1, "interleaved", FP, 100),
 ]
 
 
