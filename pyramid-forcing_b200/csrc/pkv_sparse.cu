@@ -154,6 +154,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
@@ -321,7 +322,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
   float* score = qf + kSelGroups * kQs;                            // [kMine][cap]
   int* kid = reinterpret_cast<int*>(score + kMine * cap);          // [kMine][top_k] kept earlier
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_wait();
+  grid_wait();  // (from here on plain loads: the read-only path is for data that no
+                // kernel still running when this one started has written)
   grid_release();  // the attention of few rows may queue up behind this grid
   const int rank = X > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / X;
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         v[i] = r + i * kRows < nr
-                   ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs))
+                   ? *reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs)
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          f[i][e] = ok ? __ldg(reinterpret_cast<const float4*>(p + 32 * i + 4 * e))
+          f[i][e] = ok ? *reinterpret_cast<const float4*>(p + 32 * i + 4 * e)
                        : make_float4(0.f, 0.f, 0.f, 0.f);
       float part[4][4] = {};  // independent chains of mma
       float n2 = 0.0f;
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
         if (row >= 0 && row < a.means_rows)
 #pragma unroll
           for (int d = 0; d < D; d += 32)
-            x = fma(double(__ldg(a.means + row * D + d + lane)), qg[d + lane], x);
+            x = fma(double(a.means[row * D + d + lane]), qg[d + lane], x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
         return order_key(x);

@@ -542,3 +542,30 @@ TORCH_LIBRARY_IMPL(adahead, AutogradCUDA, m) {
   m.impl("pkv_norm", op_norm_autograd);
   m.impl("pkv_rotary_apply", op_rotary_autograd);
 }
+
+// Shapes only.
+TORCH_LIBRARY_IMPL(adahead, Meta, m) {
+  m.impl("pkv_norm", [](Tensor x, std::optional<Tensor>, std::optional<Tensor>, double, bool) {
+    return at::empty(x.sizes(), x.options());
+  });
+  m.impl("pkv_rotary_apply", [](Tensor q, std::optional<Tensor> k, Tensor, int64_t, Tensor,
+                                std::optional<Tensor>, bool, double) {
+    const bool two = k.has_value() && k->defined();
+    return std::tuple<Tensor, Tensor>(at::empty(q.sizes(), q.options()),
+                                      two ? at::empty(k->sizes(), k->options()) : Tensor());
+  });
+  m.impl("pkv_block_means", [](Tensor k, Tensor cu, int64_t block, bool) {
+    const int64_t D = k.size(-1);
+    return at::empty({pkv_block_rows(k.numel() / D, int(cu.numel() - 1), int(block)), D},
+                     k.options().dtype(at::kFloat));
+  });
+  m.impl("pkv_sparse_attention",
+         [](Tensor q, Tensor, Tensor, Tensor cu, int64_t chunks, int64_t rows, int64_t top_k,
+            int64_t query_block, int64_t, std::optional<double>, std::optional<Tensor>,
+            std::optional<Tensor>) {
+           return std::tuple<Tensor, Tensor>(
+               at::empty(q.sizes(), q.options()),
+               at::empty({chunks * q.size(1), (rows + query_block - 1) / query_block, top_k},
+                         cu.options()));
+         });
+}

@@ -141,3 +141,21 @@ def test_sparse_abi_checks(lib):
                 dict(qs=12), dict(hs=0), dict(qs=0), dict(os_=4), dict(out=PTR(264))):
         assert attend(**bad) == EUNSUPPORTED, bad
     assert attend(R=0) == 0
+
+
+def test_meta_shapes():
+    from pyramidkv import _scatter_ext
+    _scatter_ext.load_library()
+    ops = torch.ops.adahead
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+    assert ops.pkv_norm(meta(2, 3, 8), meta(8), None, 1e-6, True).shape == (2, 3, 8)
+    q, k = ops.pkv_rotary_apply(meta(5, 4, 8), meta(5, 2, 8), meta(5, dtype=torch.int64), 1,
+                                meta(4, dtype=torch.float64), None, True, 1.0)
+    assert q.shape == (5, 4, 8) and k.shape == (5, 2, 8)
+    cu = meta(7, dtype=torch.int32)
+    assert ops.pkv_block_means(meta(1000, 128), cu, 64, True).shape == (1000 // 64 + 6, 128)
+    out, blocks = ops.pkv_sparse_attention(meta(300, 2, 128), meta(1000, 128), meta(1000, 128), cu,
+                                           3, 100, 5, 64, 64, None, None, None)
+    assert out.shape == (300, 2, 128) and blocks.shape == (6, 2, 5)
+    assert blocks.dtype == torch.int32
