@@ -157,6 +157,42 @@ def test_layer_norm_without_weight_or_bias(cuda, have_w, have_b):
         _within(got, want[name], name)
 
 
+@pytest.mark.parametrize("rows,groups", [(300, 2), (40, 40)])
+def test_layer_norm_some_gradients_wanted(cuda, rows, groups):
+    """Any subset of x, weight and bias: the bits of the full call."""
+    from pyramidkv.norm import layer_norm
+    x, w, b, dy = _data(cuda, rows, 256, groups, BF, FP, seed=2)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(layer_norm(*leaves, one_plus=True), leaves, dy)
+    for mask in range(1, 8):
+        args = [t.clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        picked = [t for t in args if t.requires_grad]
+        got = torch.autograd.grad(layer_norm(*args, one_plus=True), picked, dy)
+        assert all(torch.equal(p, want[i]) for p, i in
+                   zip(got, [i for i in range(3) if mask >> i & 1])), mask
+
+
+def test_layer_norm_offsets_past_32_bits(cuda):
+    """Rows whose element offset passes 2^31 (and byte offset 2^32), forward and
+    backward, against the bounds on the last ones."""
+    from pyramidkv import _ops
+    N, C = 1_400_010, 1536
+    ops = _ops.ops()
+    x = torch.zeros(N, C, dtype=BF, device=cuda)
+    tail, w, b, dy = _data(cuda, 10, C, 1, BF, FP, seed=4)
+    x[-10:] = tail
+    y, mean, rstd = ops.pkv_layer_norm(x, w, b, 1e-6, False, True)
+    want = _exact(tail, w, b, dy, 1e-6, False)
+    _within(y[-10:], want["y"], "y")
+    del y
+    g = torch.zeros(N, C, dtype=BF, device=cuda)
+    g[-10:] = dy
+    dx, dw, db = ops.pkv_layer_norm_backward(g, x, w, b, mean, rstd, False, True, True, True)
+    _within(dx[-10:], want["dx"], "dx")
+    _within(dw, want["dw"], "dw")     # the other rows' dy is 0
+    _within(db, want["db"], "db")
+
+
 def test_layer_norm_strided_and_shaped_inputs(cuda):
     """Column slices (row stride three times the width), a transposed view, 4-D
     inputs, expanded gradients, a weight and a bias of different group counts."""

@@ -138,6 +138,18 @@ def test_rotary_strided_shaped_and_expanded(cuda):
     _within(gt, _exact(dy, pos[0, :, None], inv, None, "half", 1.0, -1.0), "expanded")
 
 
+def test_rotary_offsets_past_32_bits(cuda):
+    from pyramidkv.rope import rotary_apply
+    T, H, D = 1_100_003, 16, 128
+    q, _, _, inv, _ = _data(cuda, 5, H, 1, D, 64, 1, BF, 1)
+    x = torch.zeros(T, H, D, dtype=BF, device=cuda)
+    x[-5:] = q
+    pos = torch.arange(T, device=cuda)
+    out = rotary_apply(x, pos, inv, layout="half")
+    _within(out[-5:], _exact(q, pos[-5:, None], inv, None, "half", 1.0), "tail")
+    assert (out[:5] == 0).all()
+
+
 def test_rotary_matches_the_block_rotation(cuda):
     """With a video's (t, y, x) axes it is the rotation causal_rope_apply
     makes from the model's tables, to fp32 arithmetic and one bf16 step."""
