@@ -9,7 +9,7 @@
 //   sel_g    = top_k highest scores, equal ones by index, listed ascending, -1 behind
 //   out_r    = softmax(scale * q_r . k) v over the keys of sel_g
 //
-// Three kernels:
+// Its steps:
 //  * block_means_kernel -- one pass over K, bound by HBM.  Segment s's block j
 //    has row cu[s] / block + s + j of the table: a closed form, so the table
 //    needs no offsets of its own (ceil(n / B) <= floor((a + n) / B) - floor(a / B) + 1).
@@ -17,6 +17,8 @@
 //    error; only blocks within that bound of the last place are scored again in
 //    float64 (queries summed in float64, products of fp32 means exact before
 //    their float64 sum), so the lists are those of the definition.
+//    select_group_kernel -- the same for few groups, in float64 throughout: a
+//    mma has 16 rows however few groups share a segment's means.
 //  * attention over the listed blocks, by the rows of a group:
 //    up to 16 rows (a decoded token, a small group): warps each take 16 keys,
 //    K and V go from memory straight into mma fragments, a thread-block
@@ -172,6 +174,13 @@ __device__ __forceinline__ void st_cluster(float* p, uint32_t rank, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// Into the cluster's first CTA.
+__device__ __forceinline__ void st_leader(uint64_t* p, uint64_t v) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(addr) : "r"(su32(p)));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
   grid_wait();  // (from here on plain loads: the read-only path is for data that no
                 // kernel still running when this one started has written)
   grid_release();  // the attention of few rows may queue up behind this grid
-  const int rank = X > 1 ? int(cluster_rank()) : 0;
+  const int rank = int(cluster_rank());
   const int unit = blockIdx.x / X;
   const int s = unit / a.packs, g0 = (unit - s * a.packs) * kSelGroups;
   const int ng = min(kSelGroups, a.groups - g0);
@@ -340,21 +349,13 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
     }
     return;
   }
-  auto barrier = [] {
-    if constexpr (X > 1)
-      cluster_barrier();
-    else
-      __syncthreads();
-  };
   // ---- sums of this CTA's groups' queries in float64 (exact for bf16 of like
   // size; four rows are added in fp32 first, as block_means_kernel does) ----
   for (int i = tid; i < (kSelGroups - ng) * kQs; i += kSelThreads) qf[ng * kQs + i] = 0.0f;
-  constexpr int kTogether = kMine < 4 ? kMine : 4;  // groups summed side by side
-#pragma unroll 1
-  for (int m0 = 0; m0 < kMine; m0 += kTogether) {
-    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / kTogether;
+  {
+    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / kMine;
     constexpr int kRows = kWarps * kPerWarp;
-    const int g = (m0 + warp / kWarps) * X + rank;
+    const int g = warp / kWarps * X + rank;
     const int sub = warp % kWarps * kPerWarp + lane / kLanes, d0 = (lane % kLanes) * 8;
     const int r0 = (g0 + g) * a.query_block;
     const int nr = g < ng ? min(a.query_block, a.rows_per_chunk - r0) : 0;
@@ -390,29 +391,19 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
     if (lane < kLanes)
 #pragma unroll
       for (int e = 0; e < 8; ++e) red[warp * D + d0 + e] = acc[e];
-    // the other CTAs run: their memory may be written (first time round)
-    if (m0 == 0)
-      barrier();
-    else
-      __syncthreads();
-    for (int i = tid; i < kTogether * D; i += kSelThreads) {
+    cluster_barrier();  // the other CTAs run: their memory may be written
+    for (int i = tid; i < kMine * D; i += kSelThreads) {
       double t = 0.0;
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) t += red[(i / D * kWarps + x) * D + i % D];
-      qs[m0 * D + i] = t;
-      const int gi = (m0 + i / D) * X + rank;
-      if (gi < ng) {
-        if constexpr (X > 1) {
+      qs[i] = t;
+      const int gi = i / D * X + rank;
+      if (gi < ng)
 #pragma unroll
-          for (int x = 0; x < X; ++x) st_cluster(&qf[gi * kQs + i % D], x, float(t));
-        } else {
-          qf[gi * kQs + i % D] = float(t);
-        }
-      }
+        for (int x = 0; x < X; ++x) st_cluster(&qf[gi * kQs + i % D], x, float(t));
     }
-    if (m0 + kTogether < kMine) __syncthreads();
   }
-  barrier();
+  cluster_barrier();
   // ---- queries as A fragments: with lane (g, c) = (lane / 4, lane % 4),
   // k-steps 2i, 2i + 1 take dims 32 i + 8 c .. + 7 (the order of the
   // contraction is free), so a mean's lanes load 32 bytes each ----
@@ -469,25 +460,14 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
       for (int e = 0; e < 4; ++e) {
         const int gi = gr + 8 * (e >> 1), i = t * 8 + 2 * cc + (e & 1);
         const float v = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
-        if (gi < ng && i < m) {
-          float* to = &score[gi / X * cap + kept + i];
-          if constexpr (X > 1)
-            st_cluster(to, gi % X, v);
-          else
-            *to = v;
-        }
+        if (gi < ng && i < m) st_cluster(&score[gi / X * cap + kept + i], gi % X, v);
       }
     }
     float all_most = most;
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) all_most = fmaxf(all_most, __shfl_xor_sync(kAll, all_most, o));
-    if (lane < X) {
-      if constexpr (X > 1)
-        st_cluster(&nmax[rank * kSelWarps + warp], lane, all_most);
-      else
-        nmax[warp] = all_most;
-    }
-    barrier();  // the scores of this CTA's groups are here
+    if (lane < X) st_cluster(&nmax[rank * kSelWarps + warp], lane, all_most);
+    cluster_barrier();  // the scores of this CTA's groups are here
     const int total = kept + m;
     const bool last = b0 + m == nblk;
     // ---- pick: a warp a group ----
@@ -643,7 +623,259 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
     }
     kept = min(total, a.top_k);
     if (last) return;
-    barrier();  // every CTA has picked: its memory may be written
+    cluster_barrier();  // every CTA has picked: its memory may be written
+  }
+}
+
+struct GroupSmem {
+  double red[kSelThreads / 32][128];  // the warps' query sums
+  double q[128];
+  int hist[256];
+  int wsum[2][kSelThreads / 32];
+  uint64_t prefix, lo, hi;
+  int need, done;
+  // [top_k + kSelChunk] keys, then as many ids: the kept blocks of earlier
+  // rounds, then this round's
+  uint64_t key[1];
+};
+
+// The form for few groups: a CTA a group, or a cluster whose CTAs share the
+// scores and whose first picks.  Scores are float64 products straight away, and
+// the pick goes by the scores' digits, 8 bits at a time.
+template <int D>
+__global__ void __launch_bounds__(kSelThreads, 4) select_group_kernel(SelectArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  GroupSmem& sm = *reinterpret_cast<GroupSmem*>(raw);
+  uint64_t* skey = sm.key;
+  int* sid = reinterpret_cast<int*>(skey + a.top_k + kSelChunk);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int X = int(cluster_size()), rank = int(cluster_rank());
+  grid_wait();  // (and plain loads from here on, as in the kernel above)
+  grid_release();
+  const int unit = blockIdx.x / X;
+  const int s = unit / a.groups, g = unit - s * a.groups;
+  const int c = s / a.H, h = s - c * a.H;
+  const SegView sg = segment(a.cu, s, a.kv_rows);
+  const int nblk = (sg.len + a.block - 1) / a.block;
+  int32_t* out = a.blocks + int64_t(unit) * a.top_k;
+  if (nblk <= a.top_k) {  // every block is kept (the whole cluster leaves)
+    if (rank == 0)
+      for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
+    return;
+  }
+  // ---- sum of the group's queries, float64 (exact for bf16 of like size;
+  // four rows are added in fp32 first, as block_means_kernel does) ----
+  const int r0 = g * a.query_block;
+  const int nr = min(a.query_block, a.rows_per_chunk - r0);
+  {
+    constexpr int kLanes = D / 8, kRows = kSelThreads / kLanes;
+    const int sub = tid / kLanes, d0 = (tid % kLanes) * 8;
+    const uint16_t* p =
+        a.q + (int64_t(c) * a.rows_per_chunk + r0) * a.q_rs + int64_t(h) * a.q_hs + d0;
+    double acc[8] = {};
+    for (int r = sub; r < nr; r += 4 * kRows) {
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = r + i * kRows < nr
+                   ? *reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs)
+                   : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float lo4[4], hi4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = word(w[i], e);
+          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
+          hi4[i] = __uint_as_float(u & 0xffff0000u);
+        }
+        acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
+        acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
+      }
+    }
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+    if (lane < kLanes)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sm.red[warp][d0 + e] = acc[e];
+    __syncthreads();
+    if (tid < D) {
+      double t = 0.0;
+#pragma unroll
+      for (int i = 0; i < kSelThreads / 32; ++i) t += sm.red[i][tid];
+      sm.q[tid] = t;
+    }
+    __syncthreads();
+  }
+  // ---- scores: 16 lanes a block, D / 16 products each; 4 blocks on their way ----
+  constexpr int kPer = D / 16, kVec = kPer / 4, kBatch = 4;
+  const int l16 = tid & 15;
+  double q[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) q[i] = sm.q[(i / 4) * 64 + l16 * 4 + (i & 3)];
+  const int64_t base = int64_t(a.cu[s]) / a.block + s;
+  const int stride = X * (kSelThreads / 16);
+  int kept = 0;
+  if (X > 1) cluster_barrier();  // the first CTA runs: its memory may be written
+  for (int b0 = 0; b0 < nblk; b0 += kSelChunk) {
+    const int m = min(kSelChunk, nblk - b0);
+    uint64_t mn = ~uint64_t(0), mx = 0;
+    for (int i0 = rank * (kSelThreads / 16) + (tid >> 4); i0 < kSelChunk; i0 += stride * kBatch) {
+      if (i0 - (lane >> 4) >= m) break;  // (the whole warp)
+      float4 f[kBatch][kVec];
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        const int64_t row = base + b0 + i0 + x * stride;
+        const bool ok = i0 + x * stride < m && row >= 0 && row < a.means_rows;
+        const float* p = a.means + row * D + l16 * 4;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          f[x][e] = ok ? *reinterpret_cast<const float4*>(p + e * 64)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        double t = 0.0;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          t = fma(double(f[x][e].x), q[4 * e], t);
+          t = fma(double(f[x][e].y), q[4 * e + 1], t);
+          t = fma(double(f[x][e].z), q[4 * e + 2], t);
+          t = fma(double(f[x][e].w), q[4 * e + 3], t);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        const int i = i0 + x * stride;
+        if (i < m && l16 == 0) st_leader(&skey[kept + i], order_key(t));
+      }
+    }
+    if (rank == 0)
+      for (int i = tid; i < m; i += kSelThreads) sid[kept + i] = b0 + i;
+    if (X > 1)
+      cluster_barrier();  // every score is in the first CTA's memory
+    else
+      __syncthreads();
+    const int total = kept + m;
+    const bool last = b0 + m == nblk;
+    if (rank != 0) {
+      if (last) return;
+      kept = min(total, a.top_k);
+      cluster_barrier();  // the first CTA has picked: its memory may be written
+      continue;
+    }
+    if (total <= a.top_k) {  // (not the last round: nblk > top_k)
+      kept = total;
+      if (X > 1) cluster_barrier();
+      continue;
+    }
+    // ---- the top_k-th key: digits of 8 bits from the highest that differs ----
+    for (int i = tid; i < total; i += kSelThreads) {
+      mn = min(mn, skey[i]);
+      mx = max(mx, skey[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (tid == 0) {
+      sm.lo = ~uint64_t(0);
+      sm.hi = 0;
+    }
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(reinterpret_cast<unsigned long long*>(&sm.lo), mn);
+      atomicMax(reinterpret_cast<unsigned long long*>(&sm.hi), mx);
+    }
+    __syncthreads();
+    mn = sm.lo;
+    mx = sm.hi;
+    int shift = mn == mx ? 0 : 64 - __clzll(mn ^ mx);  // bits below `shift` differ
+    uint64_t prefix = shift == 64 ? 0 : mx >> shift;
+    int need = a.top_k;
+    bool exact = false;  // every key with the prefix is kept
+    while (shift > 0 && !exact) {
+      const int bits = min(8, shift);
+      shift -= bits;
+      for (int i = tid; i < 256; i += kSelThreads) sm.hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < total; i += kSelThreads) {
+        const uint64_t key = skey[i];
+        const uint64_t up = shift + bits == 64 ? 0 : key >> (shift + bits);
+        if (up == prefix) atomicAdd(&sm.hist[int(key >> shift) & ((1 << bits) - 1)], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // lane owns bins 255 - 8 lane .. 248 - 8 lane: a scan from the top
+        int cnt[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += cnt[i] = sm.hist[255 - 8 * lane - i];
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        before -= sum;
+        if (before < need && before + sum >= need) {
+          int acc = before;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (acc < need && acc + cnt[i] >= need) {
+              sm.prefix = (prefix << bits) | uint64_t(255 - 8 * lane - i);
+              sm.need = need - acc;
+              sm.done = cnt[i] == need - acc;
+            }
+            acc += cnt[i];
+          }
+        }
+      }
+      __syncthreads();
+      prefix = sm.prefix;
+      need = sm.need;
+      exact = sm.done != 0;
+      __syncthreads();
+    }
+    // ---- keep: above the prefix, and the first `need` at it, in index order ----
+    int eq_seen = 0, written = 0;
+    for (int t0 = 0; t0 < total; t0 += kSelThreads) {
+      const int i = t0 + tid;
+      const uint64_t key = i < total ? skey[i] : 0;
+      const int id = i < total ? sid[i] : 0;
+      const uint64_t up = shift == 64 ? 0 : key >> shift;
+      const bool gt = i < total && up > prefix, eq = i < total && up == prefix;
+      const uint32_t be = __ballot_sync(0xffffffffu, eq);
+      if (lane == 0) sm.wsum[0][warp] = __popc(be);
+      __syncthreads();
+      int er = eq_seen + __popc(be & ((1u << lane) - 1));
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        if (w < warp) er += sm.wsum[0][w];
+        eq_seen += sm.wsum[0][w];
+      }
+      const bool keep = gt || (eq && er < need);
+      const uint32_t bk = __ballot_sync(0xffffffffu, keep);
+      if (lane == 0) sm.wsum[1][warp] = __popc(bk);
+      __syncthreads();
+      int at = written + __popc(bk & ((1u << lane) - 1));
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        if (w < warp) at += sm.wsum[1][w];
+        written += sm.wsum[1][w];
+      }
+      // at <= i, and every key of this tile is in registers: in place
+      if (keep && at < a.top_k) {
+        if (last)
+          out[at] = id;
+        else {
+          skey[at] = key;
+          sid[at] = id;
+        }
+      }
+      __syncthreads();
+    }
+    kept = a.top_k;
+    if (X > 1 && !last) cluster_barrier();
   }
 }
 
@@ -1250,10 +1482,39 @@ int select_shape(const SelectArgs& a, int64_t units, cudaStream_t stream) {
                       select_bytes(D, X, a.top_k), stream);
 }
 
-// Eight CTAs a cluster where that leaves room for all of them at once (a
-// cluster shares a few SMs of one GPC, so not every SM can be used), else four.
+template <int D>
+int select_few(const SelectArgs& a, int64_t groups, cudaStream_t stream) {
+  static std::mutex mu;
+  static int done[kMaxDevices] = {};
+  const auto bytes = [](int top_k) { return sizeof(GroupSmem) + size_t(top_k + kSelChunk) * 12; };
+  if (smem_opt_in(done, mu, select_group_kernel<D>, bytes(kMaxTopK)) <= 0) {
+    cudaGetLastError();
+    return PKV_ELAUNCH;
+  }
+  // a cluster while the groups leave SMs idle and the keys could make blocks
+  // enough to share (16 a round and CTA)
+  int X = 1;
+  while (X < kSelCluster && groups * X * 2 <= sm_count() && a.kv_rows / a.block >= int64_t(X) * 64)
+    X *= 2;
+  return launch_units(select_group_kernel<D>, a, groups, X, true, kSelThreads, bytes(a.top_k),
+                      stream);
+}
+
+// The form by what a group costs.  select_group_kernel reads the whole table
+// for every group; select_blocks_kernel reads it once for 16, but an mma has 16
+// rows however few groups a segment has.  Measured, us with D = 128 (group form
+// / tensor cores): one group a segment 9.9 / 12.7 (12 x 512 blocks), 36 / 69
+// (400 x 512), 107 / 169 (20 x 7812); 16 groups a segment 10.5 / 14.6 (8 x 128
+// blocks), 14.5 / 14.9 (8 x 256), 15.9 / 16.0 (4 x 512), 22 / 16.5 (8 x 512).
+// With more than one group they meet at about 220 blocks an SM in all.
+// On the tensor cores, eight CTAs a cluster where that leaves room for all of
+// them at once (a cluster shares a few SMs of one GPC, so not every SM can be
+// used; 16.3 / 18.0 us for 12 x 13 groups of 437 blocks), else four.
 template <int D>
 int launch_select(SelectArgs a, int64_t segs, cudaStream_t stream) {
+  const int64_t blocks = a.kv_rows / a.block + segs;  // of all segments, at most
+  if (a.groups == 1 || a.groups * blocks <= int64_t(220) * sm_count())
+    return select_few<D>(a, segs * a.groups, stream);
   a.packs = (a.groups + kSelGroups - 1) / kSelGroups;
   const int64_t units = segs * a.packs;
   if (units * 8 <= sm_count()) return select_shape<D, 8>(a, units, stream);

@@ -201,6 +201,83 @@ def test_select_blocks_huge_and_infinite(cuda):
     assert select_blocks(ones, inf, cu, nb * 64, 1, 3, 9).flatten().tolist() == want(ones, inf, 9)
 
 
+def _tc_select(q, means, cu, C, R, top, gr, B):
+    """select_blocks with a table of means and a row count as of a far larger
+    k: few groups then go over the tensor cores too."""
+    from pyramidkv.sparse import select_blocks
+    blocks = 17_000                                   # two groups: 34 000 > 220 an SM
+    assert -(-R // gr) >= 2
+    wide = torch.full((blocks + cu.numel(), means.shape[1]), float("nan"), device=means.device)
+    wide[:means.shape[0]] = means
+    return select_blocks(q, wide, cu, blocks * B, C, R, top, query_block=gr, block=B)
+
+
+@pytest.mark.parametrize("lens,C,H,R,D,top,gr,B", [
+    ([700, 0, 64, 3001], 2, 2, 300, 128, 5, 128, 64),
+    ([700, 1, 65, 3001], 1, 4, 130, 64, 7, 64, 128),
+    ([2000, 1999, 130], 1, 3, 40, 128, 3, 1, 64),       # 40 groups: the last 16 rows half full
+    ([500, 333] * 12, 2, 12, 17, 64, 1, 9, 64),          # clusters of four
+    ([70_000], 1, 1, 400, 64, 20, 1, 64),                # two rounds
+    ([70_000, 140_000], 1, 2, 10, 128, 1024, 5, 64),     # as many as can be asked for, three
+    ([66_000, 70_000], 1, 2, 33, 128, 700, 2, 64),
+])
+def test_select_blocks_on_tensor_cores(cuda, lens, C, H, R, D, top, gr, B):
+    from pyramidkv.sparse import block_means
+    q, k, _, cu = _case(cuda, lens, C, H, R, D, seed=len(lens) + R)
+    got = _tc_select(q, block_means(k, cu, B), cu, C, R, top, gr, B)
+    assert torch.equal(got, _exact_lists(q, k, cu, C, R, top, gr, B))
+
+
+def test_select_blocks_on_tensor_cores_ties_and_extremes(cuda):
+    """Equal scores by index, -0 equal to 0, NaN last, infinities and products
+    past fp32's range in order; one group's infinite query leaves the others'."""
+    D, nb = 128, 700
+    g = torch.Generator().manual_seed(21)
+    cu = torch.tensor([0, nb * 64], dtype=torch.int32, device=cuda)
+
+    def check(q, m, top):
+        got = _tc_select(q, m, cu, 1, q.shape[0], top, 1, 64)
+        s = (q[:, 0].double() @ m[:nb].double().T).cpu()
+        s = torch.where(torch.isnan(s), -torch.inf, s)
+        want = torch.argsort(s, dim=1, descending=True, stable=True)[:, :top].sort(1).values.int()
+        assert torch.equal(got[0].cpu(), want)
+    q = torch.randn(3, 1, D, generator=g).to(cuda, BF)
+    kinds = torch.randn(3, D, generator=g)[torch.arange(nb + 1) % 3].to(cuda)
+    for top in (1, 5, 233, 234, 300, 699):
+        check(q, kinds, top)
+    check(torch.zeros_like(q), kinds, 4)
+    signed = torch.zeros(nb + 1, D, device=cuda)
+    signed[::2] = -0.0
+    check(q.abs(), signed, 3)
+    means = torch.randn(nb + 1, D, generator=g).to(cuda)
+    for qs, ms in ((1e30, 1e30), (1e-30, 1e-30), (1.0, 3e38), (1e-38, 1.0), (1e38, 1.0)):
+        check((q.float() * qs).to(BF), means * ms, 33)
+    odd = means.clone()
+    odd[5, 3], odd[77, 3], odd[400, 3] = float("inf"), -float("inf"), float("nan")
+    check(q.abs(), odd, 9)
+    big = q.abs()
+    big[1, 0, 7] = float("inf")
+    check(big, means, 9)
+
+
+@pytest.mark.parametrize("nb,top", [(40, 7), (300, 20), (2500, 64)])
+def test_select_blocks_on_tensor_cores_scores_closer_than_fp32(cuda, nb, top):
+    from pyramidkv.sparse import block_means
+    D, B, R = 128, 64, 600
+    g = torch.Generator().manual_seed(nb)
+    base = torch.randn(B, D, generator=g)
+    base[:, :16] *= 1e-2
+    k = base.to(BF).repeat(nb, 1).view(nb, B, D)
+    at = torch.randint(0, 16, (nb,), generator=g)
+    step = torch.randint(-1, 2, (nb,), generator=g).short()
+    k[torch.arange(nb), 5, at] = (k[torch.arange(nb), 5, at].view(torch.int16) + step).view(BF)
+    k = k.reshape(nb * B, D).to(cuda)
+    cu = torch.tensor([0, nb * B], dtype=torch.int32, device=cuda)
+    q = torch.randn(R, 1, D, generator=g).to(cuda, BF)
+    got = _tc_select(q, block_means(k, cu, B), cu, 1, R, top, 128, B)
+    assert torch.equal(got, _exact_lists(q, k, cu, 1, R, top, 128, B))
+
+
 ATTEND = [
     # segment lengths, chunks, heads, rows, D, query_block, block: few rows ...
     ([700, 0, 64, 3001], 1, 4, 1, 128, 128, 64),
