@@ -1625,8 +1625,9 @@ extern "C" int pkv_select_blocks(const uint16_t* q, int64_t q_row_stride, int64_
   if (num_chunks == 0 || num_heads == 0 || rows_per_chunk == 0) return PKV_OK;
   if (!q || (means_rows > 0 && !means) || !cu_seqlens_k || !blocks) return PKV_EINVAL;
   if (top_k > kMaxTopK) return PKV_ECAPACITY;
-  if ((head_dim != 64 && head_dim != 128) || reinterpret_cast<uintptr_t>(q) % 16 ||
-      q_row_stride % 8 || q_head_stride % 8 || reinterpret_cast<uintptr_t>(means) % 16)
+  if ((head_dim != 64 && head_dim != 128) || kv_rows >= (int64_t(1) << 31) ||
+      int64_t(num_chunks) * rows_per_chunk >= (int64_t(1) << 31) - kBM ||
+      reinterpret_cast<uintptr_t>(q) % 16 || q_row_stride % 8 || q_head_stride % 8 || reinterpret_cast<uintptr_t>(means) % 16)
     return PKV_EUNSUPPORTED;
   SelectArgs a{};
   a.q = q;
@@ -1664,7 +1665,7 @@ extern "C" int pkv_block_attention(const uint16_t* q, int64_t q_row_stride, int6
   if (top_k > kMaxTopK) return PKV_ECAPACITY;
   const int64_t q_rows = int64_t(num_chunks) * rows_per_chunk;
   if ((head_dim != 64 && head_dim != 128) || kv_rows >= (int64_t(1) << 31) ||
-      q_rows >= (int64_t(1) << 31) || reinterpret_cast<uintptr_t>(q) % 16 ||
+      q_rows >= (int64_t(1) << 31) - kBM || reinterpret_cast<uintptr_t>(q) % 16 ||
       reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16 ||
       reinterpret_cast<uintptr_t>(out) % 16 || q_row_stride % 8 || q_head_stride % 8 ||
       o_row_stride % 8 || o_head_stride % 8 || q_row_stride <= 0 ||

@@ -159,3 +159,14 @@ def test_meta_shapes():
                                            3, 100, 5, 64, 64, None, None, None)
     assert out.shape == (300, 2, 128) and blocks.shape == (6, 2, 5)
     assert blocks.dtype == torch.int32
+
+
+def test_selection_refuses_counts_past_32_bits(lib):
+    p = PTR(256)
+
+    def select(rows=100, C=1, R=3, gr=128):
+        return lib.pkv_select_blocks(p, I64(256), I64(128), p, I64(4), p, I64(rows), INT(C), INT(2),
+                                     INT(R), INT(128), INT(gr), INT(64), INT(4), p, None)
+    for bad in (dict(rows=1 << 31), dict(rows=(1 << 63) - 1), dict(C=1 << 16, R=1 << 16),
+                dict(R=(1 << 31) - 1)):
+        assert select(**bad) == EUNSUPPORTED, bad
