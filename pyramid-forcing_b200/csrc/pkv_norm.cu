@@ -873,9 +873,10 @@ int launch_bwd(const NormBwdArgs& a, int64_t groups, cudaStream_t s) {
         if (nvec <= 8192) return row_bwd<TX, TW, V, 16, 512>(a, grid, s);
     }
   }
-  if (a.dx) norm_bwd_long_kernel<TX, TW><<<int(rows), 1024, 0, s>>>(a);
+  // (the column sums first: dx may be in dy's memory)
   const dim3 cols(unsigned(grid), unsigned((a.C + kNormThreads - 1) / kNormThreads));
   if (a.part) norm_cols_kernel<TX><<<cols, kNormThreads, 0, s>>>(a);
+  if (a.dx) norm_bwd_long_kernel<TX, TW><<<int(rows), 1024, 0, s>>>(a);
   return launch_status();
 }
 

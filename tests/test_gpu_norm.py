@@ -354,3 +354,34 @@ def test_layer_norm_refusals(cuda):
         layer_norm(x[:, :0])
     with pytest.raises(ValueError, match="one type"):
         layer_norm(x.to(BF), torch.ones(8, device=cuda, dtype=BF), torch.ones(8, device=cuda))
+
+
+@pytest.mark.parametrize("rows,cols,groups", [(37, 1536, 1), (24, 512, 24), (9, 40_000, 3), (40, 9000, 1)])
+def test_layer_norm_backward_in_place_through_the_abi(cuda, rows, cols, groups):
+    """pkv_layer_norm_backward with dx in dy's memory, rows in registers and
+    longer ones: the bits of separate memory."""
+    import ctypes
+    from pyramidkv import _scatter_ext
+    ops = torch.ops.adahead
+    _scatter_ext.load_library()
+    lib = ctypes.CDLL(_scatter_ext.KERNEL_PATH)
+    g = torch.Generator().manual_seed(cols)
+    x, dy = (torch.randn(rows, cols, generator=g).to(cuda, torch.bfloat16) for _ in range(2))
+    w, b = (torch.randn(groups, cols, generator=g).to(cuda) for _ in range(2))
+    _, mean, rstd = ops.pkv_layer_norm(x, w, b, 1e-6, True, True)
+    want = ops.pkv_layer_norm_backward(dy, x, w, b, mean, rstd, True, True, True, True)
+    ptr, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+    lib.pkv_layer_norm_workspace_bytes.restype = i64
+    need = lib.pkv_layer_norm_workspace_bytes(i64(rows), i64(cols), i64(groups))
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    both, dw, db = dy.clone(), torch.empty_like(w), torch.empty_like(b)
+    at = lambda t: ptr(t.data_ptr())
+    torch.cuda.synchronize()
+    rc = lib.pkv_layer_norm_backward(
+        at(both), i64(cols), at(x), i64(cols), at(w), at(mean), at(rstd), i32(0), i32(2),
+        i64(rows), i64(cols), i64(groups), i32(1), at(both), i64(cols), at(dw), at(db), at(ws),
+        i64(need), ptr(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert rc == 0
+    for got, ref in zip((both, dw, db), want):
+        assert torch.equal(got, ref)
