@@ -433,7 +433,7 @@ int pkv_layer_norm(const void *x, int64_t x_row_stride, const void *weight, cons
  * [groups, cols] (wtype); each may be NULL when it is not wanted.  mean /
  * rstd: those pkv_layer_norm saved.  The column sums go through `workspace`
  * (pkv_layer_norm_workspace_bytes, overwritten; needed when dweight or dbias
- * is) in a fixed order: the same inputs give the same bits.  dx may be dy.
+ * is; may be NULL where that is 0) in a fixed order: the same inputs give the same bits.  dx may be dy.
  */
 int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups);
 int pkv_layer_norm_backward(const void *dy, int64_t dy_row_stride, const void *x,

@@ -756,6 +756,10 @@ int64_t bwd_parts(int64_t rows_per_group, int64_t groups, int64_t cols) {
   return row_parts(rows_per_group, groups, per_sm, 4);
 }
 
+// A group of one part needs no second pass and no workspace (rows in registers
+// only: every width up to 8192 is).
+bool one_pass(int64_t parts, int64_t cols) { return parts == 1 && cols <= 8192; }
+
 constexpr int round_warp(int n) { return (n + 31) / 32 * 32; }
 
 template <typename TX, typename TW, int V, int L>
@@ -903,8 +907,7 @@ int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream
     return a.C % v == 0 && vec_ok(a.x, a.x_rs, v, sx) && vec_ok(a.dy, a.dy_rs, v, sx) &&
            vec_ok(a.dx, a.dx_rs, v, sx) && vec_ok(a.w, 0, sw, 1);
   };
-  // (a group of one part needs no second pass: rows in registers only)
-  const bool whole = a.parts == 1 && a.C <= 8192;
+  const bool whole = one_pass(a.parts, a.C);
   NormBwdArgs b = a;
   if (whole) {
     b.part = nullptr;
@@ -942,7 +945,8 @@ using namespace pkv;
 
 extern "C" int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups) {
   if (rows <= 0 || cols <= 0 || groups <= 0 || rows % groups != 0) return 0;
-  return groups * bwd_parts(rows / groups, groups, cols) * 2 * cols * 4;
+  const int64_t parts = bwd_parts(rows / groups, groups, cols);
+  return one_pass(parts, cols) ? 0 : groups * parts * 2 * cols * 4;
 }
 
 extern "C" int pkv_layer_norm(const void* x, int64_t x_row_stride, const void* weight,
@@ -989,8 +993,9 @@ extern "C" int pkv_layer_norm_backward(const void* dy, int64_t dy_row_stride, co
   if (cols > kMaxCols || rows >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (!sums && !dx) return PKV_OK;
-  if (sums && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
-               workspace_bytes < pkv_layer_norm_workspace_bytes(rows, cols, groups)))
+  const int64_t need = sums ? pkv_layer_norm_workspace_bytes(rows, cols, groups) : 0;
+  if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
+                   workspace_bytes < need))
     return PKV_EINVAL;
   NormBwdArgs a{};
   a.dy = dy;

@@ -71,11 +71,14 @@ def test_layer_norm_abi_checks(lib):
     assert fwd(rows=0) == 0
 
     lib.pkv_layer_norm_workspace_bytes.restype = I64
-    need = lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8), I64(2))
-    assert need == 2 * 1 * 2 * 8 * 4           # two rows a group: one part
+    need = lib.pkv_layer_norm_workspace_bytes(I64(16), I64(8), I64(2))
+    assert need == 2 * 2 * 2 * 8 * 4           # eight rows a group: two parts
+    # two rows a group: one part, whose sums need no second pass up to 8192 columns
+    assert lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8192), I64(2)) == 0
+    assert lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8193), I64(2)) == 2 * 1 * 2 * 8193 * 4
     assert lib.pkv_layer_norm_workspace_bytes(I64(4), I64(8), I64(3)) == 0
 
-    def bwd(dy=p, x=p, mean=p, dt=0, wt=0, rows=4, cols=8, groups=2, dw=p, ws=p, size=need):
+    def bwd(dy=p, x=p, mean=p, dt=0, wt=0, rows=16, cols=8, groups=2, dw=p, ws=p, size=need):
         return lib.pkv_layer_norm_backward(
             dy, I64(8), x, I64(8), p, mean, p, INT(dt), INT(wt), I64(rows), I64(cols),
             I64(groups), INT(0), p, I64(8), dw, None, ws, I64(size), None)
