@@ -420,8 +420,8 @@ int pkv_rope_q(const uint16_t *x, int64_t x_tok_stride, int64_t x_head_stride, u
  * weight / bias: [groups, cols] (either may be NULL), row r uses row
  * r / (rows / groups); groups divides rows.  dtype: x and y; wtype: weight and
  * bias (dtype or PKV_FP32).  Rows are x_row_stride / y_row_stride elements
- * apart, channels contiguous.  rows < 2^31, cols <= 2^20.  mean / rstd: fp32 [rows], saved for the backward pass
- * (nullable).
+ * apart, channels contiguous.  rows < 2^31, cols <= 2^20.  mean / rstd: fp32
+ * [rows], saved for the backward pass (nullable).
  */
 int pkv_layer_norm(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
                    int dtype, int wtype, int64_t rows, int64_t cols, int64_t groups, float eps,
@@ -433,7 +433,8 @@ int pkv_layer_norm(const void *x, int64_t x_row_stride, const void *weight, cons
  * [groups, cols] (wtype); each may be NULL when it is not wanted.  mean /
  * rstd: those pkv_layer_norm saved.  The column sums go through `workspace`
  * (pkv_layer_norm_workspace_bytes, overwritten; needed when dweight or dbias
- * is; may be NULL where that is 0) in a fixed order: the same inputs give the same bits.  dx may be dy.
+ * is; may be NULL where that is 0) in a fixed order: the same inputs give the
+ * same bits.  dx may be dy.
  */
 int64_t pkv_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t groups);
 int pkv_layer_norm_backward(const void *dy, int64_t dy_row_stride, const void *x,
@@ -451,8 +452,9 @@ int pkv_layer_norm_backward(const void *dy, int64_t dy_row_stride, const void *x
  * from 2 * pairs on are copied.  inverse != 0 turns the other way (the
  * gradient's pass).  Token t, head h starts at base + t * tok_stride + h *
  * head_stride (elements).  positions: int64 [tokens, axes] (1-4 axes);
- * inv_freq: float64 [pairs] radians a position; axis: int32 [pairs] (may be NULL for one axis;
- * entries outside 0 .. axes - 1 are clamped).  pairs <= 2048.  x and out may be the same memory.
+ * inv_freq: float64 [pairs] radians a position; axis: int32 [pairs] (may be
+ * NULL for one axis; entries outside 0 .. axes - 1 are clamped).  pairs <= 2048.
+ * x and out may be the same memory (with the same strides).
  */
 int pkv_rotary(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int q_heads,
                void *q_out, int64_t qo_tok_stride, int64_t qo_head_stride, const void *k,

@@ -205,8 +205,8 @@ extern "C" int pkv_rotary(const void* q, int64_t q_tok_stride, int64_t q_head_st
     return PKV_EINVAL;
   if (tokens == 0 || q_heads + k_heads == 0) return PKV_OK;
   if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || head_dim <= 0 || pairs < 0 ||
-      2 * int64_t(pairs) > head_dim || axes < 1 || axes > kRotAxes || (axes > 1 && !axis) ||
-      (pairs > 0 && (!positions || !inv_freq)))
+      2 * int64_t(pairs) > head_dim || axes < 1 || axes > kRotAxes ||
+      (pairs > 0 && (!positions || !inv_freq || (axes > 1 && !axis))))
     return PKV_EINVAL;
   if (pairs > kRotTable || head_dim > 65536 || q_heads > 65536 || k_heads > 65536)
     return PKV_EUNSUPPORTED;
