@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_wait();  // (from here on plain loads: the read-only path is for data that no
                 // kernel still running when this one started has written)
-  grid_release();  // the attention of few rows may queue up behind this grid
+  grid_release();  // the attention may queue up behind this grid
   const int rank = int(cluster_rank());
   const int unit = blockIdx.x / X;
   const int s = unit / a.packs, g0 = (unit - s * a.packs) * kSelGroups;
@@ -1215,6 +1215,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                  "r"(256));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  grid_wait();
   const SegView sg = segment(a.cu, s, a.kv_rows);
   if (warp == 1) {  // the listed 64-key halves that hold keys, in order
     const int nblk = (sg.len + a.block - 1) / a.block, per = a.block / 64;
@@ -1576,8 +1577,10 @@ int launch_tc(const SparseArgs& a, int num_chunks, int64_t units, cudaStream_t s
     cudaGetLastError();
     return PKV_ELAUNCH;
   }
-  sparse_tc_kernel<D><<<int(units), kTcThreads, smem, stream>>>(mq, mk, mv, a);
-  return launch_status();
+  // (early: 30.9 -> 29.9 us for 112 tiles of 16 steps with their selection and
+  // means, 146.4 -> 145.2 for 468)
+  return launch_clusters(sparse_tc_kernel<D>, dim3(unsigned(units)), 1, true, kTcThreads, smem,
+                         stream, mq, mk, mv, a);
 }
 
 }  // namespace
