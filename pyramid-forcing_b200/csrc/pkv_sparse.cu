@@ -1138,12 +1138,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 // has: their next loads have a step and a half to arrive in.
 //   Rows of V behind a segment's end are zeroed in shared memory: their weights
 // are 0, but 0 * inf would not be.
-//   468 tiles of 32 blocks of 64 take 82 us, 1872 tiles 283.  An SM spends 1790
-// cycles on a step of each of its two CTAs; their MMAs alone take 1349 (issued
-// without data; one of N = 64 takes as long as one of N = 128) and the softmax
-// 1300, both measured by clock64.  Steps of 128 keys with one S buffer took 89 to
-// 92 us; Q.K of 128 keys with the softmax and P.V in halves 93; pulling the next
-// keys into L2 86; a third K buffer 81, not worth its shared memory.
+//   Measured by clock64 on a CTA alone on its SM (D = 64): the softmax of a step
+// takes 1030 cycles (96 for its scores, 826 for maxima and weights, 100 to store
+// and signal).  The MMAs of two CTAs alone take 948 a step and CTA pair (D = 128;
+// one of N = 64 takes 48 cycles, bound by shared memory, one of N = 128 64).
+// Issued by lane 0 instead of an elected lane they took 1349 and the issuing
+// thread's loop was the longest part of a step: 468 tiles with their means and
+// selection took 142 us instead of 135, 1872 tiles 499 instead of 469.
+//   Not kept (with lane 0 issuing, 82 us for the 468 tiles): 128-key steps with one
+// S buffer 89 to 92; Q.K of 128 keys with the softmax and P.V in halves 93; the
+// next keys pulled into L2 86; a third K buffer 81.  With an elected lane: a
+// row's columns split over two warps, 192 tiles of 64 steps 61 -> 65 us.
 constexpr int kTcThreads = 192;
 constexpr int kStepKeys = 64;
 constexpr int kMaxHalves = 2 * kMaxTopK;
@@ -1246,7 +1251,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0 && steps > 0) {
+    if (elect_one() && steps > 0) {
       mbar_expect_tx(&sm.q_full, kBM * D * 2);
       const int row0 = ch * a.rows_per_chunk + r0;
 #pragma unroll
@@ -1284,7 +1289,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0 && steps > 0) {
+    if (elect_one() && steps > 0) {
       constexpr uint32_t kN = uint32_t(kBN >> 3) << 17;  // N of idesc_bf16
       constexpr uint32_t id_qk = (idesc_bf16(false) & ~kN) | (uint32_t(kStepKeys >> 3) << 17);
       constexpr uint32_t id_pv = (idesc_bf16(true) & ~kN) | (uint32_t(D >> 3) << 17);
@@ -1347,6 +1352,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     const uint32_t o_tm = tmem + 128 + lane_off;
     const float sc = a.scale_log2;
+    // the same answer in every lane: none leaves the loop alone
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, a.status)) != 0;
+    };
     float m_ref = -INFINITY, l_sum = 0.0f;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
@@ -1355,13 +1364,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const uint32_t s_tm = tmem + b * 64 + lane_off;
       const int valid = sg.len - sm.list[j] * kStepKeys;  // keys inside the segment
       const bool partial = valid < kStepKeys;
-      if (!mbar_wait(&sm.s_full[b], par, abort, a.status)) {
+      if (!wait(&sm.s_full[b], par)) {
         ok = false;
         break;
       }
       tc_fence_after();
       if (partial) {
-        if (!mbar_wait(&sm.v_full[b], par, abort, a.status)) {
+        if (!wait(&sm.v_full[b], par)) {
           ok = false;
           break;
         }
@@ -1419,7 +1428,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       l_sum = l_sum * alpha + (e0 + e1);
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
         // PV(j - 1) may still be running
-        if (!mbar_wait(&sm.pv_done[b ^ 1], ((j - 1) >> 1) & 1, abort, a.status)) {
+        if (!wait(&sm.pv_done[b ^ 1], ((j - 1) >> 1) & 1)) {
           ok = false;
           break;
         }
@@ -1445,8 +1454,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (row < nr)
         for (int e = 0; e < D; e += 8)
           *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
-    } else if (ok && mbar_wait(&sm.pv_done[(steps - 1) & 1], ((steps - 1) >> 1) & 1, abort,
-                               a.status)) {
+    } else if (ok && wait(&sm.pv_done[(steps - 1) & 1], ((steps - 1) >> 1) & 1)) {
       tc_fence_after();
       const float inv = l_sum > 0.0f ? 1.0f / l_sum : (l_sum == 0.0f ? 0.0f : l_sum);
 #pragma unroll
