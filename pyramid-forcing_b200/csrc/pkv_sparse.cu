@@ -1143,12 +1143,13 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 // and signal).  The MMAs of two CTAs alone take 948 a step and CTA pair (D = 128;
 // one of N = 64 takes 48 cycles, bound by shared memory, one of N = 128 64).
 // Issued by lane 0 instead of an elected lane they took 1349 and the issuing
-// thread's loop was the longest part of a step: 468 tiles with their means and
-// selection took 142 us instead of 135, 1872 tiles 499 instead of 469.
-//   Not kept (with lane 0 issuing, 82 us for the 468 tiles): 128-key steps with one
-// S buffer 89 to 92; Q.K of 128 keys with the softmax and P.V in halves 93; the
-// next keys pulled into L2 86; a third K buffer 81.  With an elected lane: a
-// row's columns split over two warps, 192 tiles of 64 steps 61 -> 65 us.
+// thread's loop was the longest part of a step: 36 segments (468 tiles) took 144.6
+// us with their means and selection instead of 141.4, 144 segments 507 instead of 495.
+//   Not kept, the first ones in separate runs, which differ by up to 3%: 128-key
+// steps with one S buffer 89 to 92 us against 82 for the 468 tiles; Q.K of 128 keys
+// with the softmax and P.V in halves 93; the next keys pulled into L2 86; a third K
+// buffer 81; a row's columns split over two warps 143.5 against 139.5 (in turn, with
+// means and selection).
 constexpr int kTcThreads = 192;
 constexpr int kStepKeys = 64;
 constexpr int kMaxHalves = 2 * kMaxTopK;
@@ -1352,10 +1353,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     const uint32_t o_tm = tmem + 128 + lane_off;
     const float sc = a.scale_log2;
-    // the same answer in every lane: none leaves the loop alone
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, a.status)) != 0;
-    };
+    // A lane whose wait ran out waits no more but stays with its warp to the end
+    // (its warp's votes and TMEM accesses need every lane): what it reads and writes
+    // is this CTA's own memory, and no row is stored.
     float m_ref = -INFINITY, l_sum = 0.0f;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
@@ -1364,16 +1364,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const uint32_t s_tm = tmem + b * 64 + lane_off;
       const int valid = sg.len - sm.list[j] * kStepKeys;  // keys inside the segment
       const bool partial = valid < kStepKeys;
-      if (!wait(&sm.s_full[b], par)) {
-        ok = false;
-        break;
-      }
+      ok = ok && mbar_wait(&sm.s_full[b], par, abort, a.status);
       tc_fence_after();
       if (partial) {
-        if (!wait(&sm.v_full[b], par)) {
-          ok = false;
-          break;
-        }
+        ok = ok && mbar_wait(&sm.v_full[b], par, abort, a.status);
         if (row < kStepKeys && row >= valid) {  // this row of V holds no key
 #pragma unroll
           for (int x = 0; x < kCols; ++x)
@@ -1428,10 +1422,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       l_sum = l_sum * alpha + (e0 + e1);
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
         // PV(j - 1) may still be running
-        if (!wait(&sm.pv_done[b ^ 1], ((j - 1) >> 1) & 1)) {
-          ok = false;
-          break;
-        }
+        ok = ok && mbar_wait(&sm.pv_done[b ^ 1], ((j - 1) >> 1) & 1, abort, a.status);
         tc_fence_after();
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
@@ -1454,7 +1445,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       if (row < nr)
         for (int e = 0; e < D; e += 8)
           *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
-    } else if (ok && wait(&sm.pv_done[(steps - 1) & 1], ((steps - 1) >> 1) & 1)) {
+    } else if (__all_sync(0xffffffffu,
+                          ok && mbar_wait(&sm.pv_done[(steps - 1) & 1], ((steps - 1) >> 1) & 1,
+                                          abort, a.status))) {
       tc_fence_after();
       const float inv = l_sum > 0.0f ? 1.0f / l_sum : (l_sum == 0.0f ? 0.0f : l_sum);
 #pragma unroll
