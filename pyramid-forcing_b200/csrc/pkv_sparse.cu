@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
       // near: at least lo (or all) and below hi
       auto is_near = [&](float x) { return all || (x >= lo && x < hi); };
       const int need = a.top_k - nsure;
-      // exact score of the block at index j of this round's scores
+      // exact score of the block at index j of the present scores
       auto score64 = [&](int j) {
         const int64_t row = base + (j < kept ? kd[j] : b0 + j - kept);
         double x = 0.0;
@@ -638,7 +638,7 @@ struct GroupSmem {
   uint64_t prefix, lo, hi;
   int need, done;
   // [top_k + kSelChunk] keys, then as many ids: the kept blocks of earlier
-  // rounds, then this round's
+  // rounds, then the present one's
   uint64_t key[1];
 };
 
