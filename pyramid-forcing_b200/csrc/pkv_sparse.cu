@@ -315,7 +315,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // twice over.  With T the top_k-th such score, a block above T + 2 e is in the
 // list for certain and one below T - 2 e is not; those between are scored in
 // float64 and ranked, unless all of them are in.  Infinite or NaN queries or
-// means make every block such a one.
+// means make every block such a one, and so do |q| |mean| whose products could
+// pass fp32's range: with scores of infinity T + 2 e would be infinite, and more
+// than top_k blocks could be above it.
 //   468 groups over 36 segments of 73 to 512 blocks take 19 us, 1872 groups over
 // 144 segments 48; float64 scores by a CTA a group 26 and 73.  Latency: loads,
 // cluster barriers, one warp's pick; issue slots 20% busy.
@@ -497,7 +499,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
       // 2.25 e, rounded up; the addend covers parts that underflow
       const float ql = sqrtf(float(qn)), ml = sqrtf(mm);
       const float e2 = 2.25f * 3.0517578125e-5f * 1.001f * ql * ml + 1e-35f * (ql + ml) + 1e-36f;
-      const bool all = !(e2 < INFINITY) || !(ql > 1e-15f) || !(ml > 1e-15f);
+      // (|q| |mean| bounds the products and their partial sums, which must be finite)
+      const bool all =
+          !(e2 < INFINITY) || !(ql * ml < 1e37f) || !(ql > 1e-15f) || !(ml > 1e-15f);
       const Scores held(sc, total);
       float lo = -INFINITY, hi = INFINITY;
       int nsure = 0, nnear = total;
