@@ -309,15 +309,20 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // shared memory, and every CTA picks for its groups.  A block's mean is read
 // once for 16 groups, and a single token's table by many SMs.
 //
-// Operands are split into bf16 hi + lo and multiplied as hi hi + hi lo + lo hi:
-// off by at most 3 * 2^-18 |q| |mean|, and the fp32 accumulation of 3 * 128
-// products by less than 2^-17 |q| |mean|; e = 2^-15 |q| |mean| bounds both
-// twice over.  With T the top_k-th such score, a block above T + 2 e is in the
-// list for certain and one below T - 2 e is not; those between are scored in
-// float64 and ranked, unless all of them are in.  Infinite or NaN queries or
-// means make every block such a one, and so do |q| |mean| whose products could
-// pass fp32's range: with scores of infinity T + 2 e would be infinite, and more
-// than top_k blocks could be above it.
+// Operands are split into bf16 hi + lo and multiplied as hi hi + hi lo + lo hi.
+// For x in [1, 2) hi is off by at most 2^-8 and lo, at most 2^-8, by 2^-17: the
+// product of two such loses at most 2^-16 (lo lo) + 2 * 2^-17, 8 * 2^-18 of |x y|,
+// and by Cauchy and Schwarz a score 8 * 2^-18 |q| |mean|.  Accumulation: 4 mma of 17
+// addends in a chain; with each addend cut off below 2^-22 of the largest (an
+// assumption with two bits to spare over 24-bit sums) at most 68 * 2^-22 = 4.3 *
+// 2^-18 of it; the summed query in fp32 and the sums of the chains stay below
+// 0.1 * 2^-18.  So e = 2^-14 |q| |mean| = 16 * 2^-18 bounds the error 1.29 times over
+// (1.75 times if addends are cut off at 2^-24).  With T the top_k-th such score, a
+// block above T + 2 e is in the list for certain and one below T - 2 e is not; those
+// between are scored in float64 and ranked, unless all of them are in.  Infinite or
+// NaN queries or means make every block such a one, and so do |q| |mean| whose
+// products could pass fp32's range: with scores of infinity T + 2 e would be
+// infinite, and more than top_k blocks could be above it.
 //   468 groups over 36 segments of 73 to 512 blocks take 19 us, 1872 groups over
 // 144 segments 48; float64 scores by a CTA a group 26 and 73.  Latency: loads,
 // cluster barriers, one warp's pick; issue slots 20% busy.
@@ -496,9 +501,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
         qn += __shfl_xor_sync(kAll, qn, o);
         mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
       }
-      // 2.25 e, rounded up; the addend covers parts that underflow
+      // 2.25 e, rounded up: T may be 0.1 e2 low, so 2 e + 0.1 e2 <= e2 has to hold,
+      // e2 >= 2.23 e; the addend covers parts that underflow
       const float ql = sqrtf(float(qn)), ml = sqrtf(mm);
-      const float e2 = 2.25f * 3.0517578125e-5f * 1.001f * ql * ml + 1e-35f * (ql + ml) + 1e-36f;
+      const float e2 = 2.25f * 6.103515625e-5f * 1.001f * ql * ml + 1e-35f * (ql + ml) + 1e-36f;
       // (|q| |mean| bounds the products and their partial sums, which must be finite)
       const bool all =
           !(e2 < INFINITY) || !(ql * ml < 1e37f) || !(ql > 1e-15f) || !(ml > 1e-15f);
