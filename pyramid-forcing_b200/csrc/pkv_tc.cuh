@@ -185,31 +185,37 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x for a pair, on the FMA pipe: Cody-Waite reduction x = n + f with
-// n = rint(x) (the 1.5 * 2^23 addend leaves n in the low mantissa bits) and
-// f in [-0.5, 0.5], a cubic for 2^f, and n added to the exponent field.
-// Cubic coefficients: minimax relative-error fit of 2^f on [-0.5, 0.5]
-// (exp2_poly_fit.py beside this file), max relative error 7.5e-5 -- far below
-// the 2^-8 step of the bf16 P it produces.  x is clamped at -125 so 2^n stays
-// a normal number; such weights are below 2^-125 and vanish in the sums.
+// Larger of two, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x for a pair (x <= 126), on the FMA pipe: Cody-Waite reduction x = n + f with
+// n = rint(x) (the addend of 1.5 * 2^23, and 128 for an exponent field, leaves
+// n + 128 in the low mantissa bits) and f in [-0.5, 0.5], half a cubic for 2^f,
+// times 2^(n + 1).  Cubic coefficients: minimax relative-error fit of 2^f on
+// [-0.5, 0.5] (exp2_poly_fit.py beside this file), max relative error 7.5e-5 -- far
+// below the 2^-8 step of the bf16 P it produces.  x is clamped at -128, whose field
+// is 0: anything from there down, -inf too, gives 0, and NaN stays NaN.
 __device__ __forceinline__ f2 exp2_poly2(f2 x) {
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
+  constexpr float kRound = 12582912.0f + 128.0f;  // 1.5 * 2^23 + 128
   float x0, x1;
   un2(x, x0, x1);
-  x = mk2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+  x = mk2(max_nan(x0, -128.0f), max_nan(x1, -128.0f));
   const f2 rnd = mk2(kRound, kRound);
-  const f2 t = add2(x, rnd);                            // n in the low bits of t
+  const f2 t = add2(x, rnd);                            // n + 128 in the low bits of t
   const f2 f = sub2(x, sub2(t, rnd));                   // f = x - n
-  f2 p = fma2(mk2(0.0551716685295105f, 0.0551716685295105f), f,
-              mk2(0.2426111251115799f, 0.2426111251115799f));
-  p = fma2(p, f, mk2(0.6932609677314758f, 0.6932609677314758f));
-  p = fma2(p, f, mk2(0.9999280571937561f, 0.9999280571937561f));
-  float p0, p1, t0, t1;
-  un2(p, p0, p1);
+  auto half2 = [](float c) { return mk2(0.5f * c, 0.5f * c); };
+  f2 p = fma2(half2(0.0551716685295105f), f, half2(0.2426111251115799f));
+  p = fma2(p, f, half2(0.6932609677314758f));
+  p = fma2(p, f, half2(0.9999280571937561f));
+  float t0, t1;
   un2(t, t0, t1);
-  // t's bit pattern is 0x4B400000 + n; shifting it left by 23 leaves n << 23
-  const uint32_t e0 = __float_as_uint(t0) << 23, e1 = __float_as_uint(t1) << 23;
-  return mk2(__uint_as_float(__float_as_uint(p0) + e0), __uint_as_float(__float_as_uint(p1) + e1));
+  // t's bit pattern is 0x4B400000 + n + 128; shifted left by 23 it is 2^(n + 1)
+  return mul2(p, mk2(__uint_as_float(__float_as_uint(t0) << 23),
+                     __uint_as_float(__float_as_uint(t1) << 23)));
 }
 
 // UMMA shared-memory descriptor, 128-byte swizzle (SM100 version bits = 1).
