@@ -52,15 +52,27 @@ __device__ __forceinline__ uint32_t word(const uint4& w, int i) {
   return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
 }
 
+// Eight bf16 elements into float64 sums.  (Four rows at a time added in fp32 first,
+// 12% faster, lose low bits where exponents differ by more than 14 and overflow near
+// the end of the range; doubles put together by integer operations instead of
+// conversions made the means of 2.8 M keys 8% slower.)
+__device__ __forceinline__ void add8(double (&acc)[8], const uint4& v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t u = word(v, e);
+    acc[2 * e] += double(bf16_bits_to_f32(u & 0xffffu));
+    acc[2 * e + 1] += double(__uint_as_float(u & 0xffff0000u));
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Block means
 // ---------------------------------------------------------------------------
 // W warps a table row (1, or 4 where there are few rows: each then has its
 // quarter of the keys on its way at once); 16 (D = 128) or 8 lanes a key, 8
-// elements each.  Four keys are added in fp32 (exact unless their exponents
-// differ by 14) before a float64 add, which keeps the conversions off the
-// critical pipe.  663 000 keys of 128 take 34 us, 5.0 TB/s; 2.8 M keys 113 us,
-// 6.3 TB/s.
+// elements each.  663 000 keys of 128 take 38 us, 4.6 TB/s; 2.8 M keys 130 us, 5.5
+// TB/s: the conversions to float64 are what bounds it (34 and 114 us without most
+// of them).
 template <int D, int W>
 __global__ void __launch_bounds__(256)
     block_means_kernel(const uint16_t* __restrict__ k, int64_t kv_rows,
@@ -101,19 +113,7 @@ __global__ void __launch_bounds__(256)
                    ? __ldg(reinterpret_cast<const uint4*>(p + int64_t(r + i * kKeys) * D))
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 8; i += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float lo4[4], hi4[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t u = word(v[i + x], e);
-            lo4[x] = bf16_bits_to_f32(u & 0xffffu);
-            hi4[x] = __uint_as_float(u & 0xffff0000u);
-          }
-          acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
-          acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
-        }
+      for (int i = 0; i < 8; ++i) add8(acc, v[i]);
     }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1)
@@ -359,8 +359,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
     }
     return;
   }
-  // ---- sums of this CTA's groups' queries in float64 (exact for bf16 of like
-  // size; four rows are added in fp32 first, as block_means_kernel does) ----
+  // ---- sums of this CTA's groups' queries in float64 ----
   for (int i = tid; i < (kSelGroups - ng) * kQs; i += kSelThreads) qf[ng * kQs + i] = 0.0f;
   {
     constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes, kWarps = kSelWarps / kMine;
@@ -380,19 +379,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
                    ? *reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs)
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float lo4[4], hi4[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t u = word(v[i + x], e);
-            lo4[x] = bf16_bits_to_f32(u & 0xffffu);
-            hi4[x] = __uint_as_float(u & 0xffff0000u);
-          }
-          acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
-          acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
-        }
+      for (int i = 0; i < 16; ++i) add8(acc, v[i]);
     }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1)
@@ -676,8 +663,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) select_group_kernel(SelectArgs
       for (int i = tid; i < a.top_k; i += kSelThreads) out[i] = i < nblk ? i : -1;
     return;
   }
-  // ---- sum of the group's queries, float64 (exact for bf16 of like size;
-  // four rows are added in fp32 first, as block_means_kernel does) ----
+  // ---- sum of the group's queries in float64 ----
   const int r0 = g * a.query_block;
   const int nr = min(a.query_block, a.rows_per_chunk - r0);
   {
@@ -694,17 +680,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) select_group_kernel(SelectArgs
                    ? *reinterpret_cast<const uint4*>(p + int64_t(r + i * kRows) * a.q_rs)
                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float lo4[4], hi4[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u = word(w[i], e);
-          lo4[i] = bf16_bits_to_f32(u & 0xffffu);
-          hi4[i] = __uint_as_float(u & 0xffff0000u);
-        }
-        acc[2 * e] += double((lo4[0] + lo4[1]) + (lo4[2] + lo4[3]));
-        acc[2 * e + 1] += double((hi4[0] + hi4[1]) + (hi4[2] + hi4[3]));
-      }
+      for (int i = 0; i < 4; ++i) add8(acc, w[i]);
     }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1)
