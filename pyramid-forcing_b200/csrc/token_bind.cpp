@@ -170,6 +170,7 @@ void refuse_twice(const char* op) {
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, Tensor x, std::optional<Tensor> weight,
                         std::optional<Tensor> bias, double eps, bool one_plus) {
+    at::AutoDispatchBelowADInplaceOrView guard;  // (a tracked view may not be changed in place)
     const Tensor rows = norm_rows(x);
     auto [y, mean, rstd] = op_layer_norm(rows, weight, bias, eps, one_plus, true);
     ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), mean, rstd});
@@ -291,6 +292,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
                                Tensor positions, int64_t axes, Tensor inv_freq,
                                std::optional<Tensor> axis, bool half, double scale) {
     TORCH_CHECK(q.dim() >= 3, "pkv_rotary: q must be [..., heads, dim]");
+    at::AutoDispatchBelowADInplaceOrView guard;  // (a tracked view may not be changed in place)
     positions = pos_rows(q, positions, axes);
     auto [qo, ko] = op_rotary_apply(q, k, positions, axes, inv_freq, axis, half, scale);
     ctx->save_for_backward({positions, inv_freq, axis.value_or(Tensor())});
