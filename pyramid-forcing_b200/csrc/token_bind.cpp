@@ -547,27 +547,64 @@ TORCH_LIBRARY_IMPL(adahead, AutogradCUDA, m) {
 
 // Shapes only.
 TORCH_LIBRARY_IMPL(adahead, Meta, m) {
-  m.impl("pkv_norm", [](Tensor x, std::optional<Tensor>, std::optional<Tensor>, double, bool) {
-    return at::empty(x.sizes(), x.options());
+  using Opt = std::optional<Tensor>;
+  auto given = [](const Opt& t) { return t.has_value() && t->defined(); };
+  auto like = [](const Tensor& t) { return at::empty_symint(t.sym_sizes(), t.options()); };
+  m.impl("pkv_norm", [like](Tensor x, Opt, Opt, double, bool) { return like(x); });
+  m.impl("pkv_layer_norm", [like](Tensor x, Opt, Opt, double, bool, bool stats) {
+    Tensor mean, rstd;
+    if (stats) {
+      mean = at::empty_symint({x.sym_size(0)}, x.options().dtype(at::kFloat));
+      rstd = at::empty_like(mean);
+    }
+    return std::tuple<Tensor, Tensor, Tensor>(like(x), mean, rstd);
   });
-  m.impl("pkv_rotary_apply", [](Tensor q, std::optional<Tensor> k, Tensor, int64_t, Tensor,
-                                std::optional<Tensor>, bool, double) {
-    const bool two = k.has_value() && k->defined();
-    return std::tuple<Tensor, Tensor>(at::empty(q.sizes(), q.options()),
-                                      two ? at::empty(k->sizes(), k->options()) : Tensor());
+  m.impl("pkv_layer_norm_backward", [like, given](Tensor, Tensor x, Opt w, Opt b, Tensor, Tensor,
+                                                  bool, bool need_x, bool need_weight,
+                                                  bool need_bias) {
+    TORCH_CHECK((!need_weight || given(w)) && (!need_bias || given(b)),
+                "pkv_layer_norm_backward: no weight / bias to differentiate");
+    return std::tuple<Tensor, Tensor, Tensor>(need_x ? like(x) : Tensor(),
+                                              need_weight ? like(*w) : Tensor(),
+                                              need_bias ? like(*b) : Tensor());
   });
+  auto rotate = [like, given](const Tensor& q, const Opt& k) {
+    return std::tuple<Tensor, Tensor>(like(q), given(k) ? like(*k) : Tensor());
+  };
+  m.impl("pkv_rotary", [rotate](Tensor q, Opt k, Tensor, Tensor, Opt, bool, double, bool) {
+    return rotate(q, k);
+  });
+  m.impl("pkv_rotary_apply",
+         [rotate](Tensor q, Opt k, Tensor, int64_t, Tensor, Opt, bool, double) {
+           return rotate(q, k);
+         });
   m.impl("pkv_block_means", [](Tensor k, Tensor cu, int64_t block, bool) {
-    const int64_t D = k.size(-1);
-    return at::empty({pkv_block_rows(k.numel() / D, int(cu.numel() - 1), int(block)), D},
-                     k.options().dtype(at::kFloat));
+    TORCH_CHECK(k.dim() >= 2 && (k.size(-1) == 64 || k.size(-1) == 128) &&
+                    (block == 64 || block == 128),
+                "pkv_block_means: head size and block must be 64 or 128");
+    const c10::SymInt D = k.size(-1);
+    return at::empty_symint({k.sym_numel() / D / block + cu.sym_numel() - 1, D},
+                            k.options().dtype(at::kFloat));
   });
+  auto lists = [](const Tensor& q, const Tensor& cu, int64_t chunks, int64_t rows, int64_t top_k,
+                  int64_t query_block) {
+    TORCH_CHECK(query_block >= 1, "query_block must be 1 to 128");
+    return at::empty_symint({chunks * q.sym_size(1), (rows + query_block - 1) / query_block, top_k},
+                            cu.options());
+  };
+  m.impl("pkv_select_blocks",
+         [lists](Tensor q, Tensor, Tensor cu, int64_t, int64_t chunks, int64_t rows,
+                 int64_t top_k, int64_t query_block, int64_t) {
+           return lists(q, cu, chunks, rows, top_k, query_block);
+         });
+  m.impl("pkv_block_attention",
+         [like](Tensor q, Tensor, Tensor, Tensor, int64_t, int64_t, Tensor, int64_t, int64_t,
+                double, Opt) { return like(q); });
   m.impl("pkv_sparse_attention",
-         [](Tensor q, Tensor, Tensor, Tensor cu, int64_t chunks, int64_t rows, int64_t top_k,
-            int64_t query_block, int64_t, std::optional<double>, std::optional<Tensor>,
-            std::optional<Tensor>) {
-           return std::tuple<Tensor, Tensor>(
-               at::empty(q.sizes(), q.options()),
-               at::empty({chunks * q.size(1), (rows + query_block - 1) / query_block, top_k},
-                         cu.options()));
+         [like, lists](Tensor q, Tensor, Tensor, Tensor cu, int64_t chunks, int64_t rows,
+                       int64_t top_k, int64_t query_block, int64_t, std::optional<double>, Opt,
+                       Opt) {
+           return std::tuple<Tensor, Tensor>(like(q),
+                                             lists(q, cu, chunks, rows, top_k, query_block));
          });
 }
