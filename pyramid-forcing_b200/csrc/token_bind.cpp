@@ -4,6 +4,7 @@
 // CUDA stream.  A fragment of the `adahead` library registered in
 // adahead_bind.cpp.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -19,6 +20,13 @@ namespace pkv_torch {
 namespace {
 
 using at::Tensor;
+
+// The registered op of a kernel below.  The autograd kernels call it rather than the
+// CUDA body, so that dispatch modes, fake tensors and tensor subclasses see the call.
+template <typename F>
+c10::TypedOperatorHandle<F> registered(const char* name, F&) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
 
 void check_rc(int rc, const char* what) {
   TORCH_CHECK(rc == PKV_OK, what, ": ", pkv_error_string(rc), " (code ", rc, ")");
@@ -155,8 +163,9 @@ bool wants_grad(const std::optional<Tensor>& t) {
 
 // Layer norm over the last dimension of any x, with its gradient.
 Tensor norm_rows(const Tensor& x) {
-  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "pkv_layer_norm: x has no channels");
-  return x.reshape({x.numel() / x.size(-1), x.size(-1)});
+  TORCH_CHECK(x.dim() >= 1 && x.sym_size(-1) > 0, "pkv_layer_norm: x has no channels");
+  return x.dim() == 2 ? x
+                      : x.reshape_symint({x.sym_numel() / x.sym_size(-1), x.sym_size(-1)});
 }
 
 using torch::autograd::AutogradContext;
@@ -172,22 +181,26 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                         std::optional<Tensor> bias, double eps, bool one_plus) {
     at::AutoDispatchBelowADInplaceOrView guard;  // (a tracked view may not be changed in place)
     const Tensor rows = norm_rows(x);
-    auto [y, mean, rstd] = op_layer_norm(rows, weight, bias, eps, one_plus, true);
+    static const auto op = registered("adahead::pkv_layer_norm", op_layer_norm);
+    auto [y, mean, rstd] = op.call(rows, weight, bias, eps, one_plus, true);
     ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), mean, rstd});
     ctx->saved_data["one_plus"] = one_plus;
-    return y.view(x.sizes());
+    return y.view_symint(x.sym_sizes());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_twice("pkv_norm");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op =
+        registered("adahead::pkv_layer_norm_backward", op_layer_norm_backward);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
     const bool need_w = w.defined() && ctx->needs_input_grad(1);
     const bool need_b = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
     auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-    auto [dx, dw, db] = op_layer_norm_backward(
+    auto [dx, dw, db] = op.call(
         norm_rows(grads[0]), norm_rows(x), opt(w), opt(b), saved[3], saved[4],
         ctx->saved_data["one_plus"].toBool(), ctx->needs_input_grad(0), need_w, need_b);
-    if (dx.defined()) dx = dx.view(x.sizes());
+    if (dx.defined()) dx = dx.view_symint(x.sym_sizes());
     return {dx, dw, db, Tensor(), Tensor()};
   }
 };
@@ -203,7 +216,8 @@ Tensor op_norm_autograd(Tensor x, std::optional<Tensor> weight, std::optional<Te
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
     return LayerNormFn::apply(x, weight, bias, eps, one_plus);
   at::AutoDispatchBelowADInplaceOrView guard;
-  return op_norm(x, weight, bias, eps, one_plus);
+  static const auto op = registered("adahead::pkv_norm", op_norm);
+  return op.call(x, weight, bias, eps, one_plus);
 }
 
 // ---- rotary positions --------------------------------------------------------
@@ -261,18 +275,19 @@ std::tuple<Tensor, Tensor> op_rotary(Tensor q, std::optional<Tensor> k, Tensor p
 // Rotary positions of q and k [..., heads, D], with their gradients.
 Tensor rot_rows(const Tensor& x) {
   TORCH_CHECK(x.dim() >= 3, "pkv_rotary: q and k must be [..., heads, dim]");
-  int64_t n = 1;
-  for (int64_t i = 0; i < x.dim() - 2; ++i) n *= x.size(i);
-  return x.dim() == 3 ? x : x.reshape({n, x.size(-2), x.size(-1)});
+  c10::SymInt n = 1;
+  for (int64_t i = 0; i < x.dim() - 2; ++i) n *= x.sym_size(i);
+  return x.dim() == 3 ? x : x.reshape_symint({n, x.sym_size(-2), x.sym_size(-1)});
 }
 
 // Positions of any leading shape and whole-number type as int64 [tokens, axes].
 Tensor pos_rows(const Tensor& q, const Tensor& positions, int64_t axes) {
-  const int64_t per = q.size(-2) * q.size(-1), n = per > 0 ? q.numel() / per : 0;
+  const c10::SymInt per = q.sym_size(-2) * q.sym_size(-1);
+  const c10::SymInt n = per > 0 ? q.sym_numel() / per : c10::SymInt(0);
   Tensor p = positions.scalar_type() == at::kLong ? positions : positions.to(at::kLong);
-  TORCH_CHECK(axes >= 1 && (per == 0 || p.numel() == n * axes),
+  TORCH_CHECK(axes >= 1 && (per == 0 || p.sym_numel() == n * axes),
               "pkv_rotary: positions must hold ", axes, " axes for each of ", n, " tokens");
-  if (p.dim() != 2 || p.size(1) != axes) p = p.reshape({p.numel() / axes, axes});
+  if (p.dim() != 2 || p.sym_size(1) != axes) p = p.reshape_symint({p.sym_numel() / axes, axes});
   return p.contiguous();
 }
 
@@ -294,18 +309,26 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     TORCH_CHECK(q.dim() >= 3, "pkv_rotary: q must be [..., heads, dim]");
     at::AutoDispatchBelowADInplaceOrView guard;  // (a tracked view may not be changed in place)
     positions = pos_rows(q, positions, axes);
-    auto [qo, ko] = op_rotary_apply(q, k, positions, axes, inv_freq, axis, half, scale);
+    const bool two = k.has_value() && k->defined();
+    static const auto op = registered("adahead::pkv_rotary", op_rotary);
+    auto [qo, ko] =
+        op.call(rot_rows(q), two ? std::optional<Tensor>(rot_rows(*k)) : std::nullopt, positions,
+                inv_freq, axis, half, scale, false);
+    qo = qo.view_symint(q.sym_sizes());
+    if (two) ko = ko.view_symint(k->sym_sizes());
     ctx->save_for_backward({positions, inv_freq, axis.value_or(Tensor())});
     ctx->saved_data["half"] = half;
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["k"] = ko.defined();
+    ctx->saved_data["k"] = two;
     ctx->set_materialize_grads(false);
-    if (!ko.defined()) return {qo};
+    if (!two) return {qo};
     return {qo, ko};
   }
   // the transpose of a rotation: the same turn the other way
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_twice("pkv_rotary_apply");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = registered("adahead::pkv_rotary", op_rotary);
     const auto saved = ctx->get_saved_variables();
     const bool two = ctx->saved_data["k"].toBool();
     Tensor dq = grads[0], dk = two ? grads[1] : Tensor();
@@ -315,12 +338,12 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     const Tensor first = dq.defined() ? dq : dk;
     if (!first.defined()) return out;
     const bool both = dq.defined() && dk.defined();
-    auto [g0, g1] = op_rotary(
+    auto [g0, g1] = op.call(
         rot_rows(first), both ? std::optional<Tensor>(rot_rows(dk)) : std::nullopt, saved[0],
         saved[1], saved[2].defined() ? std::optional<Tensor>(saved[2]) : std::nullopt,
         ctx->saved_data["half"].toBool(), ctx->saved_data["scale"].toDouble(), true);
-    out[dq.defined() ? 0 : 1] = g0.view(first.sizes());
-    if (both) out[1] = g1.view(dk.sizes());
+    out[dq.defined() ? 0 : 1] = g0.view_symint(first.sym_sizes());
+    if (both) out[1] = g1.view_symint(dk.sym_sizes());
     return out;
   }
 };
@@ -336,7 +359,8 @@ std::tuple<Tensor, Tensor> op_rotary_autograd(Tensor q, std::optional<Tensor> k,
     return {r[0], r.size() > 1 ? r[1] : Tensor()};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return op_rotary_apply(q, k, positions, axes, inv_freq, axis, half, scale);
+  static const auto op = registered("adahead::pkv_rotary_apply", op_rotary_apply);
+  return op.call(q, k, positions, axes, inv_freq, axis, half, scale);
 }
 
 // ---- block-sparse attention ----------------------------------------------------

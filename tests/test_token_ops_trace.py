@@ -1,5 +1,6 @@
 """The token-path ops on fake CUDA tensors, without a GPU: shapes, types and
-strides of the plain ops, and what a shape alone can refuse."""
+strides of every op, with gradients wanted too, and what a shape alone can refuse.
+(A backward pass needs the device: test_gpu_token_transforms.)"""
 from __future__ import annotations
 
 import pytest
@@ -21,6 +22,31 @@ def fake():
 def _is(t, shape, dtype=torch.float32):
     assert tuple(t.shape) == shape and t.dtype == dtype and t.device.type == "cuda"
     assert t.is_contiguous()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("shape", [(6, 8), (2, 3, 8), (8,)])
+def test_norm(fake, grad, shape):
+    ops = torch.ops.adahead
+    x, w, b = fake(*shape, dtype=BF, grad=grad), fake(8, grad=grad), fake(8, grad=grad)
+    y = ops.pkv_norm(x, w, b, 1e-6, True)
+    _is(y, shape, BF)
+    assert y.requires_grad == grad
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("lead", [(6,), (2, 3)])
+def test_rotary(fake, grad, lead):
+    ops = torch.ops.adahead
+    q, k = fake(*lead, 4, 16, grad=grad), fake(*lead, 2, 16, grad=grad)
+    pos, inv = fake(*lead, dtype=torch.int64), fake(8, dtype=torch.float64)
+    a, b = ops.pkv_rotary_apply(q, k, pos, 1, inv, None, True, 1.0)
+    _is(a, lead + (4, 16))
+    _is(b, lead + (2, 16))
+    assert a.requires_grad == b.requires_grad == grad
+    one = ops.pkv_rotary_apply(q, None, pos, 1, inv, None, True, 1.0)
+    _is(one[0], lead + (4, 16))
+    assert one[1] is None
 
 
 def test_plain_ops(fake):
