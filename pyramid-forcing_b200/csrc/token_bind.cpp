@@ -176,6 +176,18 @@ void refuse_twice(const char* op) {
               ": the gradient is not differentiable (no create_graph)");
 }
 
+// A dual tensor does not require a gradient by itself: without this its tangent
+// would be lost.
+void refuse_forward(const char* op, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op,
+                ": forward-mode derivatives are not implemented");
+}
+const Tensor& or_none(const std::optional<Tensor>& t) {
+  static const Tensor none;
+  return t.has_value() ? *t : none;
+}
+
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, Tensor x, std::optional<Tensor> weight,
                         std::optional<Tensor> bias, double eps, bool one_plus) {
@@ -213,6 +225,7 @@ Tensor op_norm(Tensor x, std::optional<Tensor> weight, std::optional<Tensor> bia
 
 Tensor op_norm_autograd(Tensor x, std::optional<Tensor> weight, std::optional<Tensor> bias,
                         double eps, bool one_plus) {
+  refuse_forward("pkv_norm", {&x, &or_none(weight), &or_none(bias)});
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
     return LayerNormFn::apply(x, weight, bias, eps, one_plus);
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -352,6 +365,7 @@ std::tuple<Tensor, Tensor> op_rotary_autograd(Tensor q, std::optional<Tensor> k,
                                               int64_t axes, Tensor inv_freq,
                                               std::optional<Tensor> axis, bool half,
                                               double scale) {
+  refuse_forward("pkv_rotary_apply", {&q, &or_none(k), &inv_freq});
   TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
               "pkv_rotary_apply: inv_freq has no gradient here; detach it");
   if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) {

@@ -17,11 +17,19 @@ the packed cache.  The reference attends the whole cache
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ops
 
 
+def _no_tangent(*tensors) -> None:
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("block-sparse attention has no forward-mode derivative")
+
+
 def _no_grad(*tensors) -> None:
+    _no_tangent(*tensors)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("block-sparse attention has no gradient: call it under "
                            "torch.no_grad()")
@@ -34,6 +42,7 @@ def block_means(k: torch.Tensor, cu_seqlens_k: torch.Tensor, block: int = 64) ->
     cu_seqlens_k[s + 1], its block j the row cu_seqlens_k[s] // block + s + j
     of the table.  Rows between segments and behind the last are zero.
     """
+    _no_tangent(k)
     return _ops.overload("pkv_block_means")(k, cu_seqlens_k, int(block), True)
 
 

@@ -1,14 +1,49 @@
 """The token-path ops under torch's dispatch modes, tracing and vmap: the eager
-bits."""
+bits.  Forward-mode derivatives are refused, not dropped."""
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from test_gpu_token_autograd import BF, _rotary_inputs
 
 pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_is_refused(cuda):
+    """A dual tensor's tangent is not dropped."""
+    from pyramidkv import sparse
+    from pyramidkv.norm import layer_norm
+    from pyramidkv.rope import rotary_apply
+    q, k, pos, inv = _rotary_inputs(cuda)
+    x, w = torch.randn(6, 64, device=cuda), torch.randn(64, device=cuda)
+    sq = torch.randn(3, 2, 64, device=cuda).to(BF)
+    sk = torch.randn(300, 64, device=cuda).to(BF)
+    cu = torch.tensor([0, 100, 300], dtype=torch.int32, device=cuda)
+    lists = torch.zeros(2, 1, 2, dtype=torch.int32, device=cuda)
+    with fwAD.dual_level():
+        def dual(t):
+            return fwAD.make_dual(t, torch.ones_like(t))
+        for call in (lambda: layer_norm(dual(x)), lambda: layer_norm(x, dual(w)),
+                     lambda: layer_norm(x, w, dual(w)),
+                     lambda: rotary_apply(dual(q), pos, inv),
+                     lambda: rotary_apply((q, dual(k)), pos, inv),
+                     lambda: rotary_apply(q, pos, dual(inv)),
+                     lambda: sparse.block_means(dual(sk), cu),
+                     lambda: sparse.block_attention(sq, dual(sk), sk, cu, 1, 3, lists),
+                     lambda: sparse.sparse_attention(dual(sq), sk, sk, cu, 1, 3, 2)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError,
+                                                                 match="forward|gradient"):
+                    call()
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.func.jvp(layer_norm, (x,), (x,))
+        # no dual tensor among the inputs: as ever
+        assert torch.equal(layer_norm(x, w), layer_norm(x.clone(), w))
+        rotary_apply(q, pos, inv)
+        sparse.sparse_attention(sq, sk, sk, cu, 1, 3, 2)
 
 
 class _Names(TorchDispatchMode):
