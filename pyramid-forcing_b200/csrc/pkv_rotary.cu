@@ -12,11 +12,12 @@
 // tokens: its threads first work out the tokens' cosines and sines once into
 // shared memory (the angle is the same in every head of q and of k), then
 // stream the heads of q and k through registers in accesses of up to 16
-// bytes.  No frequency tables in memory, so a position may be any int64: the
-// turn count position * inv_freq / 2 pi is formed and reduced in float64 (a
-// position of 10^6 at fp32 would be off by a tenth of a radian), and the
-// reduced angle goes through sincospif with its rounding remainder added back
-// to first order, so cos and sin are good to fp32's last bit.
+// bytes.  No frequency tables in memory.  The turn count position * inv_freq /
+// 2 pi is formed and reduced in pairs of float64 (a position of 10^6 at fp32
+// would be off by a tenth of a radian, one of 2^40 in a single float64 by 10^-4),
+// and the reduced angle goes through sincospif with its rounding remainder added
+// back to first order, so cos and sin are good to fp32's last bit for every
+// int64 position while |position * inv_freq| < 2^64.
 #include "pkv_vec.cuh"
 
 namespace pkv {
@@ -58,6 +59,20 @@ struct RotArgs {
   float scale, sign;
 };
 
+// Fraction of a turn, [-1/2, 1/2], of n * f radians.  f / 2 pi and its products
+// with the halves of n are kept as hi + lo (the rounding error of a product is
+// fma(a, b, -a b)); whole turns leave each part before they are added.  Off by
+// about 2^-53 + 2^-105 |n f| turns.
+__device__ __forceinline__ double turn_fraction(int64_t n, double f) {
+  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1 / (2 pi)
+  const double w = f * kHi, wl = fma(f, kLo, fma(f, kHi, -w));
+  const double up = double(n >> 32) * 4294967296.0, dn = double(uint32_t(n));
+  const double p = up * w, q = dn * w;
+  const double e = fma(up, wl, fma(up, w, -p)) + fma(dn, wl, fma(dn, w, -q));
+  const double r = ((p - rint(p)) + (q - rint(q))) + (e - rint(e));
+  return r - rint(r);
+}
+
 // Eight blocks an SM (32 registers; a few spilled words) keep enough loads on
 // their way: 65521 tokens of 24 heads x 128 fp16, a quarter of them turned,
 // take 127 us a pass, 806 MB at 6.3 TB/s, 0.97 of the copy rate; with 36
@@ -86,9 +101,7 @@ __global__ void __launch_bounds__(kRotThreads, V >= 4 ? 8 : 6) rotary_kernel(Rot
     const int t = i / a.P, p = i - t * a.P;
     int ax = a.axis ? a.axis[p] : 0;
     ax = ax < 0 ? 0 : (ax >= a.n_axes ? a.n_axes - 1 : ax);
-    const double turns = double(a.pos[(t0 + t) * a.n_axes + ax]) *
-                         (a.inv_freq[p] * 0.15915494309189533577);  // 1 / (2 pi)
-    const double x = 2.0 * (turns - rint(turns));                   // half turns, [-1, 1]
+    const double x = 2.0 * turn_fraction(a.pos[(t0 + t) * a.n_axes + ax], a.inv_freq[p]);
     const float hi = float(x), lo = float(x - double(hi)) * 3.14159265f;
     float s, c;
     sincospif(hi, &s, &c);
