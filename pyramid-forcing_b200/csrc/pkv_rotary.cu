@@ -244,7 +244,8 @@ extern "C" int pkv_rotary(const void* q, int64_t q_tok_stride, int64_t q_head_st
   if (tile > 8) tile = 8;
   if (tile > fill) tile = fill;
   if (tile < 1) tile = 1;
-  if (tile * row >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
+  // (a thread steps past the last one by up to kRotThreads)
+  if (tile * row > INT32_MAX - kRotThreads) return PKV_EUNSUPPORTED;
   a.tile = int(tile);
   const int64_t grid = (tokens + tile - 1) / tile;
   if (grid >= (int64_t(1) << 31)) return PKV_EUNSUPPORTED;
