@@ -913,7 +913,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
   extern __shared__ __align__(16) uint8_t raw[];
   FewSmem<D>& sm = *reinterpret_cast<FewSmem<D>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_wait();
+  grid_wait();  // (plain loads from here on, of K and V too: the kernel before this one
+                // may be what wrote them, and may have let this one start early)
   const int X = int(cluster_size()), rank = int(cluster_rank());
   const int unit = blockIdx.x / X;
   const int s = unit / a.groups, grp = unit - s * a.groups;
@@ -966,7 +967,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 #pragma unroll
       for (int e = 0; e < D / 32; ++e)
         kw[t][e] = t * 8 + g < valid
-                       ? __ldg(reinterpret_cast<const uint4*>(kp + (t * 8 + g) * D + 32 * e + 8 * c))
+                       ? *reinterpret_cast<const uint4*>(kp + (t * 8 + g) * D + 32 * e + 8 * c)
                        : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -974,7 +975,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 #pragma unroll
       for (int e = 0; e < D / 64; ++e)
         vw[t][e] = key < valid
-                       ? __ldg(reinterpret_cast<const uint4*>(vp + key * D + 64 * e + 8 * g))
+                       ? *reinterpret_cast<const uint4*>(vp + key * D + 64 * e + 8 * g)
                        : make_uint4(0, 0, 0, 0);
     }
     float sc[2][4];
