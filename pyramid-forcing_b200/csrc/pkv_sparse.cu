@@ -562,39 +562,86 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArg
         }
         continue;
       }
+      // ---- float64 scores of the near ones, in index order: a lane a block where
+      // there are many, the warp a block else (either adds in its own order, so one
+      // of them for all).  Of those, `bar` and the first `ties` at it are kept ----
+      uint64_t bar = 0;
+      int ties = need;
       if (nnear > need) {
-        // float64 scores of the near ones
+        uint64_t mn = ~uint64_t(0), mx = 0;
+        int at = 0;
         for (int t0 = 0; t0 < total; t0 += 32) {
           const int i = t0 + lane;
-          uint32_t todo = __ballot_sync(kAll, i < total && is_near(sc[i]));
-          while (todo) {
-            const int j = t0 + __ffs(todo) - 1;
-            todo &= todo - 1;
-            const uint64_t x = score64(j);
-            if (lane == 0) ex[j] = x;
+          const bool is = i < total && is_near(sc[i]);
+          uint32_t todo = __ballot_sync(kAll, is);
+          const int to = at + __popc(todo & ((1u << lane) - 1));
+          at += __popc(todo);
+          uint64_t mine = 0;
+          if (nnear > 32) {
+            const int64_t row = base + (i < kept ? kd[i] : b0 + i - kept);
+            double x[4] = {};
+            if (is && row >= 0 && row < a.means_rows)
+#pragma unroll 4
+              for (int d = 0; d < D; d += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(a.means + row * D + d);
+                x[0] = fma(double(m.x), qg[d], x[0]);
+                x[1] = fma(double(m.y), qg[d + 1], x[1]);
+                x[2] = fma(double(m.z), qg[d + 2], x[2]);
+                x[3] = fma(double(m.w), qg[d + 3], x[3]);
+              }
+            mine = order_key((x[0] + x[1]) + (x[2] + x[3]));
+          } else {
+            while (todo) {
+              const int l = __ffs(todo) - 1;
+              todo &= todo - 1;
+              const uint64_t x = score64(t0 + l);
+              if (lane == l) mine = x;
+            }
+          }
+          if (is) {
+            ex[to] = mine;
+            mn = min(mn, mine);
+            mx = max(mx, mine);
           }
         }
         __syncwarp();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          mn = min(mn, __shfl_xor_sync(kAll, mn, o));
+          mx = max(mx, __shfl_xor_sync(kAll, mx, o));
+        }
+        // the need-th highest bit by bit, from the highest that differs
+        auto count = [&](uint64_t x) {
+          int c = 0;
+          for (int i = lane; i < nnear; i += 32) c += ex[i] >= x;
+          return __reduce_add_sync(kAll, c);
+        };
+        int bit = mn == mx ? -1 : 63 - __clzll(mn ^ mx);
+        bar = bit < 0 ? mx : bit == 63 ? 0 : mx >> (bit + 1) << (bit + 1);
+        for (; bit >= 0; --bit) {
+          const uint64_t x = bar | uint64_t(1) << bit;
+          const int c = count(x);
+          if (c >= need) bar = x;
+          if (c == need) break;
+        }
+        ties = need - (bar == ~uint64_t(0) ? 0 : count(bar + 1));
       }
-      // ---- which to keep: a near one by its rank among the near (or all of
-      // them).  Lane t holds the flags of tiles t and t + 32 ----
+      // ---- which to keep.  Lane t holds the flags of tiles t and t + 32 ----
       uint32_t flags[2] = {0, 0};
+      int seen = 0, even = 0;  // near ones so far, and those at the bar
       for (int t0 = 0; t0 < total; t0 += 32) {
+        const uint32_t below = (1u << lane) - 1;
         const int i = t0 + lane;
         const float v = i < total ? sc[i] : -INFINITY;
+        const bool is = i < total && is_near(v);
         bool keep = !all && i < total && v >= (nnear > need ? hi : lo);
         if (nnear > need) {
-          uint32_t todo = __ballot_sync(kAll, i < total && is_near(v));
-          while (todo) {
-            const int j = t0 + __ffs(todo) - 1;
-            todo &= todo - 1;
-            const uint64_t mine = ex[j];
-            int ahead = 0;
-            for (int x = lane; x < total; x += 32)
-              if (is_near(sc[x])) ahead += ex[x] > mine || (ex[x] == mine && x < j);
-            ahead = __reduce_add_sync(kAll, ahead);
-            if (i == j) keep = ahead < need;
-          }
+          const uint32_t nb = __ballot_sync(kAll, is);
+          const uint64_t x = is ? ex[seen + __popc(nb & below)] : 0;
+          const uint32_t eb = __ballot_sync(kAll, is && x == bar);
+          keep = keep || (is && (x > bar || (x == bar && even + __popc(eb & below) < ties)));
+          seen += __popc(nb);
+          even += __popc(eb);
         }
         const uint32_t kb = __ballot_sync(kAll, keep);
         if (lane == ((t0 >> 5) & 31)) (t0 < 1024 ? flags[0] : flags[1]) = kb;
