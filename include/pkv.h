@@ -301,7 +301,8 @@ int pkv_select_blocks(const uint16_t *q, int64_t q_row_stride, int64_t q_head_st
 /*
  * pkv_attention over the listed blocks only (a caller may list any: entries
  * outside the segment are skipped, a block listed twice counts twice, a row
- * with no keys gives zeros).  softmax_scale > 0.  status (nullable):
+ * with no keys, or whose scores are all -inf, gives zeros; a score of NaN or +inf
+ * makes its row NaN).  softmax_scale > 0.  status (nullable):
  * PKV_ST_TIMEOUT when a bounded device wait expired.
  */
 int pkv_block_attention(const uint16_t *q, int64_t q_row_stride, int64_t q_head_stride,
@@ -453,7 +454,9 @@ int pkv_layer_norm_backward(const void *dy, int64_t dy_row_stride, const void *x
  * gradient's pass).  Token t, head h starts at base + t * tok_stride + h *
  * head_stride (elements).  positions: int64 [tokens, axes] (1-4 axes);
  * inv_freq: float64 [pairs] radians a position; axis: int32 [pairs] (may be
- * NULL for one axis; entries outside 0 .. axes - 1 are clamped).  pairs <= 2048.
+ * NULL for one axis; entries outside 0 .. axes - 1 are clamped).  pairs <= 2048,
+ * (q_heads + k_heads) * head_dim < 2^31 - 256.  Any position is exact to fp32's
+ * last bit while |position * inv_freq| < 2^64.
  * x and out may be the same memory (with the same strides).
  */
 int pkv_rotary(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int q_heads,

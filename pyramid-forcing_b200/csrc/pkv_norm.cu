@@ -39,9 +39,9 @@ struct NormArgs {
   float eps, plus;
 };
 
-// s / c, c = 1 / inv: for fp32 rows the product's rounding is corrected once
-// (two operations instead of a division's dozen in every thread); 16-bit rows
-// would not show it, and 37440 of 1536 take 36 us without and 42 with it.
+// s / c, c = 1 / inv: for fp32 rows one step of Newton's method takes the product's
+// rounding out, m + (s - m c) / c; 16-bit rows would not show it, and 37440 of 1536
+// take 36 us without and 42 with it.
 template <typename T>
 __device__ __forceinline__ float mean_of(float s, float c, float inv) {
   const float m = s * inv;
@@ -50,8 +50,8 @@ __device__ __forceinline__ float mean_of(float s, float c, float inv) {
   return fabsf(m) < INFINITY ? fixed : m;
 }
 
-// 1 / sqrt(v), v > 0: the approximation of 2 units in the last place, corrected
-// once for fp32 rows.
+// 1 / sqrt(v), v > 0: the approximation of 2 units in the last place, with one step
+// of Newton's method for fp32 rows, y + y (1 - v y y) / 2.
 template <typename T>
 __device__ __forceinline__ float rstd_of(float v) {
   const float y = rsqrtf(v);
@@ -280,8 +280,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_short_kernel(NormArgs a) {
 // the backward pass): weight and bias are read once and stay in registers,
 // R rows share the two barriers of their statistics, and the next
 // rounds' rows are on their way into shared memory meanwhile.  37440 rows of
-// 1536 bf16 take 36 us, 230 MB at 6.4 TB/s, the copy rate; a warp a row, loading
-// the weights for every row, took 62.
+// 1536 bf16 take 36 us, 230 MB at 6.4 TB/s, the copy rate (one launch behind an L2
+// flush; 43 in a steady loop); a warp a row, loading the weights for every row,
+// took 62.
 // (16-bit single elements are too small for asynchronous copies: loaded
 // directly.)
 constexpr int kColStages = 3;
@@ -483,8 +484,8 @@ __host__ __device__ constexpr int bwd_stages(int stage_bytes) { return stage_byt
 __host__ __device__ constexpr int bwd_rows(int elems) { return elems <= 8 ? 2 : 1; }
 
 // CTA (group, part): its rows, every column; V * NV columns a thread.  37440 rows
-// of 1536 bf16 take 64 us, 345 MB at 5.4 TB/s: about 1000 warp instructions a
-// row keep the issue slots 56% busy.  Rows loaded when needed 154 us, the same
+// of 1536 bf16 take 64 us, 345 MB at 5.4 TB/s (70 in a steady loop, with the sum of
+// the parts): about 1000 warp instructions a row keep the issue slots 56% busy.  Rows loaded when needed 154 us, the same
 // through shared memory ahead of use 102, conversions in pairs 82; the rest came
 // from a grid of one wave (448 blocks on 444 places had cost a second one).
 // 16-bit single elements (V = 1) are too small for asynchronous copies and
@@ -748,8 +749,11 @@ int64_t row_parts(int64_t rows_per_group, int64_t groups, int per_sm, int least)
   const int64_t p = want < most ? want : most;
   return p < 1 ? 1 : p;
 }
-// Backward: three blocks of 192 threads an SM, more of the smaller ones that
-// short rows (16-byte vectors) leave.
+// Backward: three blocks of 192 threads an SM (what the registers allow), more of the
+// smaller ones that short rows (16-byte vectors) leave.  us with two thirds / this /
+// four thirds of them, 60 M elements of bf16: 1536 columns 69.4 / 69.8 / 79.7, 1024
+// 78.5 / 70.0 / 71.2, 64 columns 170 / 172 / 172; but 256 85.8 / 97.6 / 118.7 and 128
+// 132 / 147 / 167, where fewer would do.
 int64_t bwd_parts(int64_t rows_per_group, int64_t groups, int64_t cols) {
   const int64_t thr = (cols / 8 + 31) / 32 * 32;
   const int per_sm = thr >= 192 ? 3 : thr <= 32 ? 18 : int(576 / thr);
@@ -797,7 +801,11 @@ int launch_fwd(const NormArgs& a, cudaStream_t s) {
   if (a.rows >= int64_t(sm_count()) * 16) {
     // rows enough to fill the GPU.  Short ones: a few lanes a row; longer
     // ones, in groups that give a block rows to share its weights over: fixed
-    // columns
+    // columns.  us, a block a row / these forms, at 8, 16 and 64 rows an SM: 256 bf16
+    // 2.5 / 2.3, 3.0 / 2.5, 6.7 / 4.8; 1536 bf16 4.0 / 4.1, 6.2 / 4.8, 18.9 / 10.4;
+    // 520 fp32 3.3 / 3.9, 5.0 / 4.3, 13.8 / 8.2; 1535 bf16 8.3 / 10.0, 12.0 / 11.3,
+    // 39 / 29.  Rows of 8 KB and odd fp32 ones gain nothing from them: 4096 bf16
+    // 5.9 / 6.4, 9.8 / 10.4, 35.2 / 36.0; 1111 fp32 5.4 / 8.9, 9.1 / 9.9, 29.5 / 35.9.
     if constexpr (V * sizeof(TX) >= 4) {
       if (nvec <= 4) return short_fwd<TX, TW, V, 4>(a, s);
       if (nvec <= 8) return short_fwd<TX, TW, V, 8>(a, s);
@@ -915,6 +923,8 @@ int run_bwd(const NormBwdArgs& a, int64_t groups, void* dw, void* db, cudaStream
     b.db = db;
   }
   int rc = PKV_OK;
+  // (short 16-bit rows leave too few threads with 16-byte vectors.  us with those / with
+  // 4 bytes, 200 000 rows: 64 columns 86 / 69, 96 90 / 96, 128 86 / 96, 256 90 / 150)
   if (fits(V) && (sizeof(TX) == 4 || a.C >= 128))
     rc = launch_bwd<TX, TW, V>(b, groups, s);
   else if (sizeof(TX) == 2 && fits(2))

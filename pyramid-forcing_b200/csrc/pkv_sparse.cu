@@ -10,13 +10,14 @@
 //   out_r    = softmax(scale * q_r . k) v over the keys of sel_g
 //
 // Its steps:
-//  * block_means_kernel -- one pass over K, bound by HBM.  Segment s's block j
+//  * block_means_kernel -- one pass over K, bound by the conversions to float64
+//    and by HBM.  Segment s's block j
 //    has row cu[s] / block + s + j of the table: a closed form, so the table
 //    needs no offsets of its own (ceil(n / B) <= floor((a + n) / B) - floor(a / B) + 1).
 //  * select_blocks_kernel -- scores on the tensor cores with a bound on their
 //    error; only blocks within that bound of the last place are scored again in
-//    float64 (queries summed in float64, products of fp32 means exact before
-//    their float64 sum), so the lists are those of the definition.
+//    float64 (queries summed in float64, times the fp32 means), so the lists are
+//    those of the definition.
 //    select_group_kernel -- the same for few groups, in float64 throughout: a
 //    mma has 16 rows however few groups share a segment's means.
 //  * attention over the listed blocks, by the rows of a group:
@@ -323,9 +324,11 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // NaN queries or means make every block such a one, and so do |q| |mean| whose
 // products could pass fp32's range: with scores of infinity T + 2 e would be
 // infinite, and more than top_k blocks could be above it.
-//   468 groups over 36 segments of 73 to 512 blocks take 19 us, 1872 groups over
-// 144 segments 48; float64 scores by a CTA a group 26 and 73.  Latency: loads,
-// cluster barriers, one warp's pick; issue slots 20% busy.
+//   468 groups over 36 segments of 73 to 512 blocks take 20 us, 1872 groups over
+// 144 segments 47; float64 scores by a CTA a group took 26 and 73.  Latency: loads,
+// cluster barriers, one warp's pick; issue slots 20% busy.  Where all scores of the
+// groups are near (zero queries, an infinite mean in every segment) the first takes
+// 80 to 100 us.
 template <int D, int X>
 __global__ void __launch_bounds__(kSelThreads, 2) select_blocks_kernel(SelectArgs a) {
   constexpr uint32_t kAll = 0xffffffffu;
@@ -1172,13 +1175,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) sparse_few_kernel(SparseArgs a
 // has: their next loads have a step and a half to arrive in.
 //   Rows of V behind a segment's end are zeroed in shared memory: their weights
 // are 0, but 0 * inf would not be.
-//   Measured by clock64 on a CTA alone on its SM (D = 64): the softmax of a step
-// takes 1030 cycles (96 for its scores, 826 for maxima and weights, 100 to store
-// and signal).  The MMAs of two CTAs alone take 948 a step and CTA pair (D = 128;
-// one of N = 64 takes 48 cycles, bound by shared memory, one of N = 128 64).
-// Issued by lane 0 instead of an elected lane they took 1349 and the issuing
-// thread's loop was the longest part of a step: 36 segments (468 tiles) took 144.6
-// us with their means and selection instead of 141.4, 144 segments 507 instead of 495.
+//   What bounds it: neither pipe by itself.  468 tiles of 32 steps on 296 places (two
+// waves, the second 58% full) take 77 us, about 2200 cycles a step of an SM's two
+// CTAs.  Their MMAs take 1280 of these (one of N = 64 takes 48 cycles, bound by
+// shared memory, one of N = 128 64; 16 and 8 of them a step), the softmax of a CTA
+// alone on its SM 1030 (clock64, D = 64: 96 for the scores, 826 for maxima and
+// weights, 100 to store and signal); the rest is the way from one role to the next.
+// Issued by lane 0 instead of an elected lane an MMA of N = 64 takes 55 to 66 cycles:
+// 36 segments (468 tiles) took 144.6 us with their means and selection instead of
+// 141.4, 144 segments 507 instead of 495.
+//   Groups of 17 to 64 rows take a tile of 128 all the same: half of every MMA and
+// two of the four softmax warps have nothing to do then.
 //   Not kept, the first ones in separate runs, which differ by up to 3%: 128-key
 // steps with one S buffer 89 to 92 us against 82 for the 468 tiles; Q.K of 128 keys
 // with the softmax and P.V in halves 93; the next keys pulled into L2 86; a third K
@@ -1550,13 +1557,16 @@ int select_few(const SelectArgs& a, int64_t groups, cudaStream_t stream) {
 // The form by what a group costs.  select_group_kernel reads the whole table
 // for every group; select_blocks_kernel reads it once for 16, but an mma has 16
 // rows however few groups a segment has.  Measured, us with D = 128 (group form
-// / tensor cores): one group a segment 9.9 / 12.7 (12 x 512 blocks), 36 / 69
-// (400 x 512), 107 / 169 (20 x 7812); 16 groups a segment 10.5 / 14.6 (8 x 128
-// blocks), 14.5 / 14.9 (8 x 256), 15.9 / 16.0 (4 x 512), 22 / 16.5 (8 x 512).
-// With more than one group they meet at about 220 blocks an SM in all.
+// / tensor cores): one group a segment 9.4 / 12.5 (12 x 512 blocks), 43 / 87
+// (400 x 512), 100 / 148 (20 x 7812); 16 groups a segment 9.8 / 13.8 (8 x 128
+// blocks), 13.0 / 13.9 (8 x 256), 14.6 / 14.0 (4 x 512), 15.3 / 13.7 (8 x 300),
+// 19.7 / 13.9 (8 x 512).  With more than one group they meet at about 220 blocks an
+// SM in all.  (Not so for a few very long segments: 4 x 13 groups of 4000 blocks take
+// 75 / 102 and go to the tensor cores all the same.)
 // On the tensor cores, eight CTAs a cluster where that leaves room for all of
 // them at once (a cluster shares a few SMs of one GPC, so not every SM can be
-// used; 16.3 / 18.0 us for 12 x 13 groups of 437 blocks), else four.
+// used; 14.2 us against 16.0 with four for 12 x 13 groups of 437 blocks), else four
+// (19.6 against 26.1 with eight for 36 x 13 groups of 300).
 template <int D>
 int launch_select(SelectArgs a, int64_t segs, cudaStream_t stream) {
   const int64_t blocks = a.kv_rows / a.block + segs;  // of all segments, at most
