@@ -1442,8 +1442,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         alpha = (j == 0 || m_ref == -INFINITY) ? 0.0f : fast_exp2(m_ref - m_new);
         m_ref = m_new;
       }
-      // a row whose scores are all -inf keeps a reference of 0
-      const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
+      // a row whose scores are all -inf keeps a reference of 0; one of +inf (a finite
+      // score that overflows when scaled too) makes the row NaN: inf * 0
+      const float m_use = m_ref == -INFINITY ? 0.0f : fmaf(m_ref, 0.0f, m_ref);
       const f2 scale2 = mk2(sc, sc), negm2 = mk2(-m_use, -m_use);
       f2 acc[4];
 #pragma unroll

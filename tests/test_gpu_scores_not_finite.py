@@ -90,3 +90,20 @@ def test_rows_of_scores_that_are_all_minus_infinity_give_zeros(cuda, kernel, R, 
     out = _attend(kernel, q, k, v, cu, D)
     assert (out[:, 1] == 0).all()
     assert torch.isfinite(out.float()).all() and (out[:, 0] != 0).any() and (out[:, 2] != 0).any()
+
+
+@pytest.mark.parametrize("kernel,R,D", [c for c in KERNELS if c[0] == "sparse"])
+def test_scores_that_pass_the_range_when_scaled_are_not_zeros(cuda, kernel, R, D):
+    """Finite scores times a scale past fp32's range: infinite, so NaN, as in
+    fp32 operations; a head whose scores stay in range keeps its result."""
+    from pyramidkv.sparse import block_attention
+    q, k, v, cu = _heads(cuda, 2, R, D, 4)
+    q[:, 1], k[N:] = 0.0, 1.0                   # head 1: scores of 0
+    every = torch.arange(N // 64, dtype=torch.int32, device=cuda)
+    out = block_attention(q, k, v, cu, 1, R, every.expand(2, -(-R // 128), -1).contiguous(),
+                          softmax_scale=2e38)
+    scores = q[:, 0].float() @ k[:N].float().T * 2e38
+    assert torch.isinf(scores.amax(1)).all()
+    assert torch.isnan(out[:, 0]).all()
+    mean = v[N:].double().mean(0)
+    assert ((out[:, 1].double() - mean).abs() <= 2.0 ** -7 * v[N:].double().abs().mean(0)).all()
